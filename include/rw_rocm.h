@@ -62,6 +62,9 @@ extern "C" {
 #define RW_EIO (-5)     /* a model file cannot be opened, read or mapped */
 
 /* ggml dtype ids (src/quant.rs:43-52) */
+#define RW_F32 0
+#define RW_F16 1
+#define RW_BF16 30
 #define RW_Q4_0 2
 #define RW_Q4_1 3
 #define RW_Q5_0 6
@@ -414,6 +417,139 @@ int rw_rocm_decoder_forward_beams_dev(rw_decoder *const *beams, size_t n_beams, 
 int rw_rocm_logits_topk_dev(const float *logits, size_t rows, size_t n_vocab, size_t k, uint32_t *ids,
                             float *logprobs, void *workspace, size_t workspace_len, void *stream);
 size_t rw_rocm_logits_topk_workspace_size(size_t rows, size_t n_vocab, size_t k);
+
+/* ---- Keys and values in pages ----
+ *
+ * rw_decoder keeps one contiguous f32 cache of n_ctx rows per beam and copies
+ * it at every fork (src/decoder.rs:70-79).  A program that serves many
+ * sequences, or searches with many beams, keeps their keys and values in
+ * pages instead: a pool of n_pages pages of page_rows rows each, and per
+ * sequence the list of the pages that hold its rows (its row of the table),
+ * so that a sequence takes only the memory of its rows and a fork shares them.
+ * No counterpart in the reference.
+ *
+ * rw_kv_pages describes the pool, in device memory the caller allocates:
+ *   k  [n_layer][n_pages][n_head][page_rows][head_size]
+ *   v  [n_layer][n_pages][n_head][head_size][page_rows]
+ * (v with the rows of a page innermost: the order in which attention's
+ * products read it).  dtype is RW_F32, RW_F16 or RW_BF16, head_size 32, 64, 96
+ * or 128, page_rows 16, 32, 64, 128 or 256; n_head counts key/value heads; k and v
+ * are 16-byte aligned.  The struct is read during the calls only.
+ *
+ * The entries below take device pointers on the current device and are queued
+ * on `stream`.  The table is [n_seqs][ld_table] page ids: row s lists the pages
+ * of sequence s in order, entry pos / page_rows the page of its row `pos`.
+ * `seq` gives the sequence (table row) of every row of the call; NULL where
+ * row r is sequence r.  All index arrays are int32 on the device, read when
+ * the work runs: a captured graph may be replayed with other contents.  The
+ * kernels check them: a row whose sequence or position the table does not
+ * have is not written, and attends to nothing; a page id outside the pool
+ * holds no rows. */
+typedef struct rw_kv_pages {
+  int dtype;
+  int n_head, head_size, page_rows;
+  size_t n_layer, n_pages;
+  void *k, *v;
+} rw_kv_pages;
+
+/* Rows k[r], v[r] (f32 [rows, n_head * head_size], row strides ldk, ldv in
+ * floats, 16-byte aligned) become row pos[r] of sequence seq[r] in `layer`,
+ * rounded once to the pool's type.  Where two rows of a call have the same
+ * place, the place holds values of either. */
+int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k, size_t ldk, const float *v, size_t ldv,
+                         size_t rows, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,
+                         const int32_t *pos, void *stream);
+
+/* Pages src[i] -> dst[i] of every layer (k and v), i < n.  src and dst are host
+ * arrays, used before the call returns (so a captured graph repeats these
+ * copies).  No dst may be listed twice or be a src: RW_EINVAL. */
+int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, const int32_t *dst, size_t n, void *stream);
+
+/* Attention of one new token per row over its sequence's pages in `layer`:
+ * out[r, n_head * head_size] = concat over heads h of softmax(q_h K^T /
+ * sqrt(head_size)) V over rows 0 .. len[r] - 1 of sequence seq[r], K and V
+ * those of key/value head h / (n_head / pages->n_head).  n_head is a
+ * multiple of pages->n_head; q and out are f32, row strides ldq, ldo in
+ * floats, 16-byte aligned; they may not overlap.  len[r] counts the visible rows (the
+ * token's own among them, if it was written before) and is cut at max_len
+ * and at what the table holds; a row with len[r] <= 0 gets zeros.  Several rows
+ * may attend to one sequence, with lengths of their own (the tokens of a prompt,
+ * drafted tokens).  max_len sizes the launch: give the longest length, or for a
+ * graph the longest that replays will see.  Scores, softmax and sums are f32,
+ * products f32-equivalent for every type of pool.  The rows seen and q must
+ * be finite; what the pool holds behind a sequence's length is not looked at.
+ * The workspace (NULL: one kept per (device, stream), not for a stream that
+ * is being captured) holds rw_rocm_paged_attention_workspace_size bytes, 16-byte
+ * aligned; 0 for arguments the call would refuse. */
+size_t rw_rocm_paged_attention_workspace_size(const rw_kv_pages *pages, size_t rows, int n_head, size_t max_len);
+int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const float *q, size_t ldq, size_t rows,
+                                int n_head, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,
+                                const int32_t *len, size_t max_len, float *out, size_t ldo, void *workspace,
+                                size_t workspace_len, void *stream);
+
+/* The book of a pool: which sequence holds which pages (host memory only; no
+ * device is needed).  A step of a serving program: extend the sequences by
+ * their new rows, queue the copies that extend asks for
+ * (rw_rocm_kv_copy_pages_dev), then per layer rw_rocm_kv_write_dev and
+ * rw_rocm_paged_attention_dev with the tables of rw_rocm_kv_book_table.  The
+ * lowest free page and sequence ids are handed out first.  A call that fails
+ * changes nothing: RW_ENOMEM where pages or sequences run out, RW_EINVAL for
+ * a sequence that does not exist or is listed twice (fork may list one twice).  A
+ * book's calls must not overlap.  Pages given back may be handed out at once:
+ * work that still reads them, and the copies of earlier calls, go before the
+ * new work on the same stream.
+ *
+ *   add       n empty sequences -> seqs
+ *   fork      n sequences with the rows of from[i], sharing their pages
+ *   extend    more[i] further rows for seqs[i]; src/dst (n entries each) and
+ *             *n_copies: the shared pages to copy before rows are written
+ *   truncate  drops a sequence's rows from `len` on
+ *   release   ends sequences, whose pages no other sequence lists become free
+ *   compact   moves the used pages to the ids 0 .. used - 1: src/dst (`cap` entries
+ *             each) and *n: the pages to copy; with a smaller `cap` than needed,
+ *             RW_EINVAL, *n the number needed and nothing moved.  Tables change.
+ *   table     the page lists of seqs -> table (host) [n][ld], 0 behind each
+ *   len       rows of a sequence
+ *   info      free pages, pages in use, sequences (each may be NULL) */
+typedef struct rw_kv_book rw_kv_book;
+int rw_rocm_kv_book_create(size_t n_pages, size_t page_rows, size_t max_seqs, rw_kv_book **out);
+void rw_rocm_kv_book_free(rw_kv_book *b);
+int rw_rocm_kv_book_add(rw_kv_book *b, size_t n, int32_t *seqs);
+int rw_rocm_kv_book_fork(rw_kv_book *b, const int32_t *from, size_t n, int32_t *seqs);
+int rw_rocm_kv_book_extend(rw_kv_book *b, const int32_t *seqs, size_t n, const size_t *more, int32_t *src, int32_t *dst,
+                           size_t *n_copies);
+int rw_rocm_kv_book_truncate(rw_kv_book *b, int32_t seq, size_t len);
+int rw_rocm_kv_book_release(rw_kv_book *b, const int32_t *seqs, size_t n);
+int rw_rocm_kv_book_compact(rw_kv_book *b, int32_t *src, int32_t *dst, size_t cap, size_t *n);
+int rw_rocm_kv_book_table(const rw_kv_book *b, const int32_t *seqs, size_t n, int32_t *table, size_t ld);
+int rw_rocm_kv_book_len(const rw_kv_book *b, int32_t seq, size_t *len);
+int rw_rocm_kv_book_info(const rw_kv_book *b, size_t *free_pages, size_t *used_pages, size_t *n_seqs);
+
+/* Log-probs of given tokens, the entropy and the top alternatives of every row
+ * of logits [rows, n_vocab] (device, dtype RW_F32, RW_F16 or RW_BF16, row
+ * stride ld in elements): log_softmax as src/transcribe.rs:482-486 has it, for
+ * what rw_rocm_logits_topk_dev does not give -- a transcript's average
+ * log-prob, the no-speech probability, the
+ * language tokens' probabilities, an entropy threshold.
+ *   logprobs[rows, n_tok]  of tokens[rows, n_tok] (ids on the device); the id
+ *                          0xFFFFFFFF ("no token", padding) gets 0, any other id outside
+ *                          the vocabulary NaN.  n_tok = 0: neither is used.
+ *   entropy[rows]          -sum p ln p in nats (NULL: not formed)
+ *   top_ids, top_logprobs  [rows, k]: the k largest logits, equal ones lowest id
+ *                          first; exactly -inf is not listed: places left over
+ *                          hold id 0xFFFFFFFF and -inf.  k <= 32; 0: neither is used.
+ * Logits of -inf (suppressed tokens) have log-prob -inf and add nothing to
+ * the entropy.  A row holding NaN or +inf, or only -inf, has NaN log-probs and
+ * entropy, and ids 0xFFFFFFFF with NaN for its alternatives.  Every logit is
+ * read once; sums are f32 in a fixed order.  n_vocab < 2^31.  The workspace
+ * (NULL: one kept per (device, stream), not for a stream that is being
+ * captured) holds rw_rocm_token_logprobs_workspace_size bytes, 16-byte
+ * aligned. */
+size_t rw_rocm_token_logprobs_workspace_size(size_t rows, size_t n_vocab, size_t k);
+int rw_rocm_token_logprobs_dev(int dtype, const void *logits, size_t ld, size_t rows, size_t n_vocab,
+                               const uint32_t *tokens, size_t n_tok, float *logprobs, float *entropy, size_t k,
+                               uint32_t *top_ids, float *top_logprobs, void *workspace, size_t workspace_len,
+                               void *stream);
 
 /* ---- Model files straight to resident weights ----
  *

@@ -22,6 +22,7 @@ CODE_NAMES = {RW_EINVAL: "RW_EINVAL", RW_ENODEV: "RW_ENODEV", RW_EHIP: "RW_EHIP"
               RW_EIO: "RW_EIO"}
 Q4_0, Q4_1, Q5_0, Q5_1, Q8_0 = 2, 3, 6, 7, 8
 DTYPES = (Q4_0, Q4_1, Q5_0, Q5_1, Q8_0)
+F32, F16, BF16 = 0, 1, 30
 QK = 32
 GEMV_MAX_M = 8
 
@@ -41,6 +42,12 @@ class rw_linear(C.Structure):
         ("out", C.c_void_p),
         ("m", C.c_size_t),
     ]
+
+
+class RwKvPages(C.Structure):
+    """struct rw_kv_pages (include/rw_rocm.h)."""
+    _fields_ = [("dtype", C.c_int), ("n_head", C.c_int), ("head_size", C.c_int), ("page_rows", C.c_int),
+                ("n_layer", C.c_size_t), ("n_pages", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p)]
 
 
 _SIGNATURES = {
@@ -106,6 +113,31 @@ _SIGNATURES = {
     "rw_rocm_logits_topk_dev": (C.c_int, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
                                           C.c_void_p, C.c_size_t, C.c_void_p]),
     "rw_rocm_logits_topk_workspace_size": (C.c_size_t, [C.c_size_t, C.c_size_t, C.c_size_t]),
+    "rw_rocm_kv_write_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t,
+                                       C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
+                                       C.c_void_p]),
+    "rw_rocm_kv_copy_pages_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rw_rocm_paged_attention_workspace_size": (C.c_size_t, [C.POINTER(RwKvPages), C.c_size_t, C.c_int, C.c_size_t]),
+    "rw_rocm_paged_attention_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
+                                              C.c_int, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
+                                              C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rw_rocm_kv_book_create": (C.c_int, [C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(C.c_void_p)]),
+    "rw_rocm_kv_book_free": (None, [C.c_void_p]),
+    "rw_rocm_kv_book_add": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rw_rocm_kv_book_fork": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rw_rocm_kv_book_extend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p,
+                                         C.POINTER(C.c_size_t)]),
+    "rw_rocm_kv_book_truncate": (C.c_int, [C.c_void_p, C.c_int32, C.c_size_t]),
+    "rw_rocm_kv_book_release": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t]),
+    "rw_rocm_kv_book_compact": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_size_t)]),
+    "rw_rocm_kv_book_table": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t]),
+    "rw_rocm_kv_book_len": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(C.c_size_t)]),
+    "rw_rocm_kv_book_info": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t),
+                                       C.POINTER(C.c_size_t)]),
+    "rw_rocm_token_logprobs_workspace_size": (C.c_size_t, [C.c_size_t, C.c_size_t, C.c_size_t]),
+    "rw_rocm_token_logprobs_dev": (C.c_int, [C.c_int, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p,
+                                             C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_size_t, C.c_void_p]),
     "rw_rocm_model_load": (C.c_int, [C.c_char_p, C.c_int, C.POINTER(C.c_void_p)]),
     "rw_rocm_model_free": (None, [C.c_void_p]),
     "rw_rocm_model_hparams": (C.c_int, [C.c_void_p, C.POINTER(C.c_int32)]),
@@ -522,6 +554,196 @@ def logits_topk_dev(logits, rows: int, n_vocab: int, k: int, ids, logprobs, stre
 
 def logits_topk_workspace_size(rows: int, n_vocab: int, k: int) -> int:
     return lib().rw_rocm_logits_topk_workspace_size(rows, n_vocab, k)
+
+
+# ------------------------------------------- keys and values in pages
+
+_TORCH_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
+
+def _dense(a, dtype: str, what: str):
+    """_ptr of a device array, which as a tensor must be dense and of `dtype`."""
+    if hasattr(a, "data_ptr"):
+        if str(a.dtype) != dtype or not a.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous {dtype} tensor")
+        return a.data_ptr()
+    return _ptr(a)
+
+
+def _rows(a, n: int, ld: int | None, what: str, dtypes=("torch.float32",)):
+    """(pointer, row stride) of device rows of n values; a 2-D tensor, which
+    may be a column block of wider rows, brings its stride."""
+    if not hasattr(a, "data_ptr"):
+        return _ptr(a), ld or n
+    if str(a.dtype) not in dtypes or (a.dim() and a.shape[-1] > 1 and a.stride(-1) != 1):
+        raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
+    return a.data_ptr(), ld or (a.stride(0) if a.dim() == 2 and a.shape[0] > 1 else n)
+
+
+class KvPages:
+    """rw_kv_pages over two device tensors: k [n_layer, n_pages, n_head,
+    page_rows, head_size] and v [n_layer, n_pages, n_head, head_size,
+    page_rows], both float32, float16 or bfloat16."""
+
+    def __init__(self, k, v):
+        L, N, H, P, D = k.shape
+        if tuple(v.shape) != (L, N, H, D, P):
+            raise ValueError("v must be [n_layer, n_pages, n_head, head_size, page_rows]")
+        if k.dtype != v.dtype or str(k.dtype) not in _TORCH_DTYPES:
+            raise ValueError("k and v must have one type: float32, float16 or bfloat16")
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("k and v must be contiguous")
+        self.k, self.v = k, v  # keeps the tensors alive
+        self.st = RwKvPages(_TORCH_DTYPES[str(k.dtype)], H, D, P, L, N, k.data_ptr(), v.data_ptr())
+
+    @property
+    def n_values(self) -> int:
+        """Key (or value) elements of one row: n_head * head_size."""
+        return self.st.n_head * self.st.head_size
+
+
+def _table_args(table, seq):
+    """(table, ld_table, n_seqs, seq) of the device entries."""
+    n_seqs, ld = table.shape
+    return _dense(table, "torch.int32", "table"), ld, n_seqs, _dense(seq, "torch.int32", "seq")
+
+
+def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=None, ldk: int | None = None,
+                 ldv: int | None = None, stream: int | None = None) -> None:
+    """Device rows k[r], v[r] into row pos[r] of sequence seq[r] (None: r).
+    table: device int32 [n_seqs, pages per sequence]; pos, seq: device int32."""
+    t, ld, n_seqs, s = _table_args(table, seq)
+    n = pages.n_values
+    check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, n, ldk, "k"), *_rows(v, n, ldv, "v"), rows, t, ld, n_seqs,
+                                     s, _dense(pos, "torch.int32", "pos"), stream))
+
+
+def kv_copy_pages_dev(pages: KvPages, src, dst, stream: int | None = None) -> None:
+    """Pages src[i] -> dst[i] of every layer; src and dst are host ids."""
+    a = np.ascontiguousarray(src, dtype=np.int32)
+    b = np.ascontiguousarray(dst, dtype=np.int32)
+    if a.ndim != 1 or a.shape != b.shape:
+        raise ValueError("src and dst must be two lists of the same length")
+    check(lib().rw_rocm_kv_copy_pages_dev(pages.st, a.ctypes.data, b.ctypes.data, a.size, stream))
+
+
+def paged_attention_workspace_size(pages: KvPages, rows: int, n_head: int, max_len: int) -> int:
+    return lib().rw_rocm_paged_attention_workspace_size(pages.st, rows, n_head, max_len)
+
+
+def paged_attention_dev(pages: KvPages, layer: int, q, rows: int, n_head: int, table, lens, max_len: int, out,
+                        seq=None, ldq: int | None = None, ldo: int | None = None, workspace=None,
+                        workspace_len: int = 0, stream: int | None = None) -> None:
+    """out[r] = attention of the one token q[r] (n_head query heads) over the
+    first lens[r] rows of sequence seq[r] (None: r).  table, lens and seq:
+    device int32, as for kv_write_dev; max_len: the longest of lens, or more."""
+    t, ld, n_seqs, s = _table_args(table, seq)
+    n = n_head * pages.st.head_size
+    check(lib().rw_rocm_paged_attention_dev(pages.st, layer, *_rows(q, n, ldq, "q"), rows, n_head, t, ld, n_seqs, s,
+                                            _dense(lens, "torch.int32", "lens"), max_len, *_rows(out, n, ldo, "out"),
+                                            _ptr(workspace), workspace_len, stream))
+
+
+class KvBook:
+    """rw_kv_book: which sequence holds which pages (host bookkeeping)."""
+
+    def __init__(self, n_pages: int, page_rows: int, max_seqs: int):
+        h = C.c_void_p()
+        check(lib().rw_rocm_kv_book_create(n_pages, page_rows, max_seqs, C.byref(h)))
+        self.handle = h.value
+
+    def add(self, n: int = 1) -> np.ndarray:
+        """n empty sequences' ids."""
+        out = np.empty(n, np.int32)
+        check(lib().rw_rocm_kv_book_add(self.handle, n, out.ctypes.data))
+        return out
+
+    def fork(self, seqs) -> np.ndarray:
+        """New sequences with the rows of `seqs`, sharing their pages."""
+        a = np.ascontiguousarray(seqs, dtype=np.int32)
+        out = np.empty(a.size, np.int32)
+        check(lib().rw_rocm_kv_book_fork(self.handle, a.ctypes.data, a.size, out.ctypes.data))
+        return out
+
+    def extend(self, seqs, more) -> tuple[np.ndarray, np.ndarray]:
+        """more rows (one number, or one per sequence) for `seqs`; the pages
+        to copy before rows are written, for kv_copy_pages_dev."""
+        a = np.ascontiguousarray(seqs, dtype=np.int32)
+        if np.any(np.asarray(more) < 0):
+            raise ValueError("more must not be negative")
+        m = np.ascontiguousarray(np.broadcast_to(np.asarray(more, dtype=np.uintp), a.shape))
+        src, dst = np.empty(a.size, np.int32), np.empty(a.size, np.int32)
+        n = C.c_size_t()
+        check(lib().rw_rocm_kv_book_extend(self.handle, a.ctypes.data, a.size, m.ctypes.data, src.ctypes.data,
+                                           dst.ctypes.data, C.byref(n)))
+        return src[: n.value], dst[: n.value]
+
+    def truncate(self, seq: int, length: int) -> None:
+        check(lib().rw_rocm_kv_book_truncate(self.handle, seq, length))
+
+    def release(self, seqs) -> None:
+        a = np.ascontiguousarray(seqs, dtype=np.int32)
+        check(lib().rw_rocm_kv_book_release(self.handle, a.ctypes.data, a.size))
+
+    def compact(self) -> tuple[np.ndarray, np.ndarray]:
+        """Moves the used pages to the lowest ids; the pages to copy."""
+        used = self.info()[1]
+        src, dst = np.empty(used, np.int32), np.empty(used, np.int32)
+        n = C.c_size_t()
+        check(lib().rw_rocm_kv_book_compact(self.handle, src.ctypes.data, dst.ctypes.data, used, C.byref(n)))
+        return src[: n.value], dst[: n.value]
+
+    def table(self, seqs, width: int) -> np.ndarray:
+        """The page lists of `seqs` as int32 [len(seqs), width]."""
+        a = np.ascontiguousarray(seqs, dtype=np.int32)
+        out = np.empty((a.size, width), np.int32)
+        check(lib().rw_rocm_kv_book_table(self.handle, a.ctypes.data, a.size, out.ctypes.data, width))
+        return out
+
+    def len(self, seq: int) -> int:
+        n = C.c_size_t()
+        check(lib().rw_rocm_kv_book_len(self.handle, seq, C.byref(n)))
+        return n.value
+
+    def info(self) -> tuple[int, int, int]:
+        """(free pages, pages in use, sequences)."""
+        f, u, s = C.c_size_t(), C.c_size_t(), C.c_size_t()
+        check(lib().rw_rocm_kv_book_info(self.handle, C.byref(f), C.byref(u), C.byref(s)))
+        return f.value, u.value, s.value
+
+    def free(self) -> None:
+        if getattr(self, "handle", None):
+            lib().rw_rocm_kv_book_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+# --------------------------------------------------------- token scores
+
+def token_logprobs_workspace_size(rows: int, n_vocab: int, k: int) -> int:
+    return lib().rw_rocm_token_logprobs_workspace_size(rows, n_vocab, k)
+
+
+def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logprobs, entropy=None, k: int = 0,
+                       top_ids=None, top_logprobs=None, ld: int | None = None, dtype: int | None = None, workspace=None,
+                       workspace_len: int = 0, stream: int | None = None) -> None:
+    """Log-probs of tokens [rows, n_tok] (32-bit ids), the entropy and the k
+    largest alternatives of every row of device logits; `dtype` is taken from a
+    logits tensor (F32 for a pointer)."""
+    if dtype is None:
+        dtype = _TORCH_DTYPES.get(str(logits.dtype), -1) if hasattr(logits, "data_ptr") else F32
+    ids = "torch.uint32" if "uint32" in str(getattr(tokens, "dtype", "")) else "torch.int32"
+    tid = "torch.uint32" if "uint32" in str(getattr(top_ids, "dtype", "")) else "torch.int32"
+    check(lib().rw_rocm_token_logprobs_dev(
+        dtype, *_rows(logits, n_vocab, ld, "logits", tuple(_TORCH_DTYPES)), rows, n_vocab, _dense(tokens, ids, "tokens"), n_tok,
+        _dense(logprobs, "torch.float32", "logprobs"), _dense(entropy, "torch.float32", "entropy"), k,
+        _dense(top_ids, tid, "top_ids"), _dense(top_logprobs, "torch.float32", "top_logprobs"), _ptr(workspace),
+        workspace_len, stream))
 
 
 MODEL_PARSE_ONLY = 1

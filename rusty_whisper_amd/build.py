@@ -1,7 +1,8 @@
 """Build recipe for the package's native libraries (run from __graft_entry__.build()).
 
-  librw_rocm.so   hipcc, gfx950 only: csrc/rw_rocm.hip (+ rw_kernels.hpp) and
-                  the host-only model loader csrc/rw_model.cpp
+  librw_rocm.so   hipcc, gfx950 only: csrc/rw_rocm.hip (+ rw_kernels.hpp),
+                  csrc/rw_serve.hip (+ rw_kv.hpp, rw_score.hpp) and the
+                  host-only model loader csrc/rw_model.cpp, side by side
   _rw_quant*.so   g++: the C++ mirror of the reference's quant API
                   (host/rw_quant.cpp) with its pybind11 binding
 
@@ -20,6 +21,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -53,9 +55,18 @@ def _run(cmd: list[str]) -> None:
 
 
 def build_rocm(extra: list[str] | None = None) -> str:
-    srcs = [os.path.join(CSRC, "rw_rocm.hip"), os.path.join(CSRC, "rw_model.cpp")]
+    flags = [*HIP_FLAGS, *(extra or []), f"-I{INCLUDE}", f"-I{CSRC}"]
     tmp = LIB_ROCM + ".tmp"
-    _run([HIPCC, *HIP_FLAGS, *(extra or []), f"-I{INCLUDE}", f"-I{CSRC}", *srcs, "-o", tmp])
+    with tempfile.TemporaryDirectory() as d:
+        objs, jobs = [], []
+        for src in ("rw_rocm.hip", "rw_serve.hip", "rw_model.cpp"):
+            objs.append(os.path.join(d, src + ".o"))
+            cmd = [HIPCC, *[f for f in flags if f != "-shared"], "-c", os.path.join(CSRC, src), "-o", objs[-1]]
+            print("+", " ".join(cmd), flush=True)
+            jobs.append(subprocess.Popen(cmd))
+        if any([job.wait() for job in jobs]):
+            raise RuntimeError("librw_rocm.so: a source does not compile")
+        _run([HIPCC, f"--offload-arch={ARCH}", "-fPIC", "-shared", *objs, "-o", tmp])
     os.replace(tmp, LIB_ROCM)
     return LIB_ROCM
 

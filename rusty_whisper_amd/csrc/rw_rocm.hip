@@ -31,6 +31,7 @@
 #include "rw_attn.hpp"
 #include "rw_kernels.hpp"
 #include "rw_dec.hpp"
+#include "rw_internal.hpp"
 #include "rw_pool.hpp"
 #include "rw_rocm.h"
 
@@ -277,6 +278,18 @@ static int stream_workspace(int device, void *stream, size_t bytes, WsHold &hold
   *out = slot->p;
   return RW_OK;
 }
+
+// (rw_serve.hip)
+int rw_internal_current_device(int *dev) { return current_device(dev); }
+int rw_internal_workspace(int device, void *stream, size_t bytes, void **slot, void **out) {
+  WsHold hold;
+  const int rc = stream_workspace(device, stream, bytes, hold, out);
+  if (rc) return rc;
+  *slot = hold.slot;
+  hold.slot = nullptr;  // held until rw_internal_workspace_release
+  return RW_OK;
+}
+void rw_internal_workspace_release(void *slot) { ws_pool().release((WsPool::Slot *)slot); }
 
 // The workspace of rw_rocm_matmul_t_q_dev_noalloc: a fixed array in device
 // memory that every GPU running this library holds until the process ends
