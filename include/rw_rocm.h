@@ -471,7 +471,7 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
  * those of key/value head h / (n_head / pages->n_head).  n_head is a
  * multiple of pages->n_head; q and out are f32, row strides ldq, ldo in
  * floats, 16-byte aligned; they may not overlap.  len[r] counts the visible rows (the
- * token's own among them, if it was written before) and is cut at max_len
+ * token's own among them, if it was written before) and is cut at max_len, 2^30
  * and at what the table holds; a row with len[r] <= 0 gets zeros.  Several rows
  * may attend to one sequence, with lengths of their own (the tokens of a prompt,
  * drafted tokens).  max_len sizes the launch: give the longest length, or for a

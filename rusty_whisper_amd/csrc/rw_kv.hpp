@@ -88,67 +88,337 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
   if (i < piece) base[id.y * piece + i] = base[id.x * piece + i];
 }
 
-// One wavefront per (row, query head): the softmax's running maximum and sum
-// over 64 keys at a time, a lane per key for the scores, a lane per value for
-// the products.
+// ------------------------------------------------------------- attention
+//
+// One workgroup of PA_WAVES wavefronts per (row, key/value head, 16 of its
+// query heads, chunk of the row's keys).  A wavefront takes every PA_WAVES-th
+// tile of keys (32 of a 2-byte type, 16 of f32: 1 KB of k and of v per 16
+// values of the head) and keeps its own running maximum, sum and 16 x DH
+// output; the wavefronts are joined through LDS at the end, chunks by
+// k_paged_join.
+//
+// Lane 16h + r of a wavefront.  Scores come transposed, S = K q^T, so that a
+// lane holds its query r's scores of keys 8h .. 8h + 7 (f32: 4h .. 4h + 3):
+// just what the second product's left operand wants of lane (h, r), and v,
+// whose rows are innermost, gives the right operand's 8 (4) keys of value
+// 16 i + r as one 16-byte load.  So k and v go from memory to the matrix
+// cores without LDS and without moves between lanes:
+//   2-byte  v_mfma 16x16x32, A = 16 keys: row r of half s is key
+//           8 (r / 4) + 4 s + r % 4, whose scores then lie in lane r / 4's
+//           registers 4 s + r % 4.  The f32 q and p enter as sums of 2 f16
+//           (22 bits) or 3 bf16 (24 bits), a product each.
+//   f32     v_mfma 16x16x4 f32, A = 16 keys in order, exact products.
+// Query columns beyond the group's are zeros.
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int PA_WAVES = 4;
+constexpr float PA_LOG2E = 1.44269504088896340736f;
+// The running maximum m is only raised when a score passes it by PA_SLACK (in
+// powers of two): then and only then the wavefront's lanes exchange their
+// maxima and scale what they hold.  p is kept at 2^PA_LIFT of the maximum's 1:
+// the largest, 2^15, fits f16, and f16's smallest step is 2^-35 of the
+// maximum's weight or less.
+constexpr float PA_SLACK = 5.0f, PA_LIFT = 10.0f;
+
 template <class E>
-__global__ __launch_bounds__(64) void k_paged_attn(PagedView w, const float *__restrict__ q, int64_t ldq, int heads,
-                                                   const int32_t *__restrict__ lens, int max_len, float scale,
-                                                   float *__restrict__ out, int64_t ldo) {
+struct PaTile;  // a tile's product: keys per tile and lane, parts of an f32 operand
+
+template <class E>
+struct PaTile2 {
+  using T = typename E::T;
+  typedef T Op __attribute__((ext_vector_type(8)));
+  static constexpr int KEYS = 32, PER = 8, STEP = 32, SUB = 2;  // STEP: values of the head per k operand
+};
+template <>
+struct PaTile<F16> : PaTile2<F16> {
+  static constexpr int PARTS = 2;
+  static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct PaTile<BF16> : PaTile2<BF16> {
+  static constexpr int PARTS = 3;
+  static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct PaTile<F32> {
+  using T = float;
+  typedef f4 Op;
+  static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1;
+  static __device__ f4 mma(Op a, Op b, f4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// x as a sum of PARTS operands
+template <class E>
+__device__ inline void pa_parts(const float (&x)[PaTile<E>::PER], typename PaTile<E>::Op (&o)[PaTile<E>::PARTS]) {
+#pragma unroll
+  for (int j = 0; j < PaTile<E>::PER; ++j) {
+    float rest = x[j];
+#pragma unroll
+    for (int p = 0; p < PaTile<E>::PARTS; ++p) {
+      const typename E::T t = E::round(rest);
+      o[p][j] = t;
+      rest -= (float)t;  // exact
+    }
+  }
+}
+
+// exp2(x) for x <= 0 or -inf against a maximum that may be -inf itself
+__device__ inline float pa_weight(float m, float top) {
+  return m == -__builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+}
+
+template <class E, int DH>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
+    const void *__restrict__ kp, const void *__restrict__ vp, const float *__restrict__ q, const int32_t *__restrict__ table,
+    const int32_t *__restrict__ seq, const int32_t *__restrict__ lens, float *__restrict__ out, float *__restrict__ part,
+    int kv_heads, int group, int pr, int n_pages, int n_seqs, int64_t ld_table, int64_t ldq, int64_t ldo, int max_len,
+    int chunk) {
+  using M = PaTile<E>;
+  using Op = typename M::Op;
+  using T = typename E::T;
+  constexpr int NC = DH / M::STEP, ND = DH / 16, KEYS = M::KEYS, PER = M::PER, SUB = M::SUB, PARTS = M::PARTS;
+  constexpr int LD = DH + 4;
   constexpr float NEG_INF = -__builtin_huge_valf();
-  __shared__ float sq[128], sp[64];
-  const int r = blockIdx.x / heads, h = blockIdx.x % heads, hk = h / (heads / w.heads), l = threadIdx.x, P = 1 << w.pr;
-  const int32_t *table = paged_row(w, r);
-  const int64_t most = w.ld << w.pr;
-  int n = min(lens[r], max_len);
+  __shared__ float so[PA_WAVES][16][LD], sm[PA_WAVES][16], sl[PA_WAVES][16];
+
+  const int qtiles = (group + 15) / 16;
+  const int qi = blockIdx.x % qtiles, hk = blockIdx.x / qtiles % kv_heads, row = blockIdx.x / qtiles / kv_heads;
+  const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int gq = min(16, group - 16 * qi);  // query heads of this tile
+  const int heads = kv_heads * group, hq = hk * group + 16 * qi;
+  const int sq = seq ? seq[row] : row;
+  const int64_t most = ld_table << pr;
+  int n = min(lens[row], max_len);
   if (n > most) n = (int)most;
-  float *o = out + r * ldo + (int64_t)h * w.dim;
-  if (!table || n <= 0) {
-    for (int d = l; d < w.dim; d += 64) o[d] = 0.0f;
+  if ((unsigned)sq >= (unsigned)n_seqs) n = 0;
+  float *orow = out + row * ldo + (int64_t)hq * DH;
+  if (n <= 0) {
+    if (blockIdx.y == 0)
+      for (int i = threadIdx.x; i < gq * DH; i += 64 * PA_WAVES) orow[i] = 0.0f;
     return;
   }
-  for (int d = l; d < w.dim; d += 64) sq[d] = q[r * ldq + (int64_t)h * w.dim + d] * scale;
-  __syncthreads();
-  const auto *pk = (const typename E::T *)w.k, *pv = (const typename E::T *)w.v;
-  float m = NEG_INF, sum = 0.0f, acc[2] = {0.0f, 0.0f};
-  for (int t0 = 0; t0 < n; t0 += 64) {
-    const int t = t0 + l;
-    float s = NEG_INF;
-    if (t < n) {
-      const int page = table[t >> w.pr];
-      if ((unsigned)page < (unsigned)w.n_pages) {
-        const auto *row = pk + ((((int64_t)page * w.heads + hk) << w.pr) + (t & (P - 1))) * w.dim;
-        s = 0.0f;
-        for (int d = 0; d < w.dim; ++d) s = fmaf(sq[d], E::load(row + d), s);
-      }
+  const int k0 = blockIdx.y * chunk;
+  if (k0 >= n) return;
+  const bool direct = n <= chunk;
+  const int32_t *tab = table + (int64_t)sq * ld_table;
+  const int end = (min(n, k0 + chunk) + KEYS - 1) / KEYS;
+  const int P = 1 << pr;
+
+  // where tile t's pages begin for this head (the two halves of a 32-key tile
+  // lie in two 16-row pages), and which halves hold no rows
+  struct Where {
+    int64_t off0, off1;
+    bool bad0, bad1;
+  };
+  auto where = [&](int t) __attribute__((always_inline)) {
+    Where w;
+    const int i = t * KEYS >> pr;
+    int p0 = tab[i], p1 = p0;
+    if (KEYS > 16 && pr == 4 && t * KEYS + 16 < n) p1 = tab[i + 1];
+    w.bad0 = (unsigned)p0 >= (unsigned)n_pages, w.bad1 = (unsigned)p1 >= (unsigned)n_pages;
+    w.off0 = (((int64_t)(w.bad0 ? 0 : p0) * kv_heads + hk) << pr) * DH;
+    w.off1 = (((int64_t)(w.bad1 ? 0 : p1) * kv_heads + hk) << pr) * DH;
+    return w;
+  };
+  const T *kb = (const T *)kp, *vb = (const T *)vp;
+  Op kf[SUB][NC], vf[ND];
+  auto load_k = [&](int t, const Where &w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const int kk = SUB == 1 ? r : 8 * (r >> 2) + 4 * s + (r & 3);
+      const int slot = KEYS > 16 && pr == 4 ? kk & 15 : (t * KEYS & (P - 1)) + kk;
+      const T *p = kb + (KEYS > 16 && kk >= 16 ? w.off1 : w.off0) + slot * DH + M::PER * h;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) kf[s][c] = *(const Op *)(p + M::STEP * c);
     }
-    float mx = s;
-    for (int x = 1; x < 64; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    const float mn = fmaxf(m, mx);
-    if (mn == NEG_INF) continue;
-    const float f = expf(m - mn), p = expf(s - mn);
-    float ps = p;
-    for (int x = 1; x < 64; x <<= 1) ps += __shfl_xor(ps, x);
-    sum = sum * f + ps;
-    m = mn;
-    __syncthreads();
-    sp[l] = p;
-    __syncthreads();
-    const int top = min(64, n - t0);
-    for (int i = 0; i < 2; ++i) {
-      const int d = l + 64 * i;
-      if (d >= w.dim) break;
-      float a = acc[i] * f;
-      for (int j = 0; j < top; ++j) {
-        if (sp[j] == 0.0f) continue;  // also a page outside the pool
-        const int page = table[(t0 + j) >> w.pr];
-        a = fmaf(sp[j], E::load(pv + ((((int64_t)page * w.heads + hk) * w.dim + d) << w.pr) + ((t0 + j) & (P - 1))), a);
+  };
+  auto load_v = [&](int t, const Where &w) __attribute__((always_inline)) {
+    const int kk = PER * h;
+    const int slot = KEYS > 16 && pr == 4 ? kk & 15 : (t * KEYS & (P - 1)) + kk;
+    const T *p = vb + (KEYS > 16 && kk >= 16 ? w.off1 : w.off0) + (r << pr) + slot;
+#pragma unroll
+    for (int i = 0; i < ND; ++i) vf[i] = *(const Op *)(p + ((16 * i) << pr));
+  };
+
+  int t = k0 / KEYS + wv;
+  Where now{};
+  if (t < end) now = where(t), load_k(t, now);
+
+  // q, in the scores' operand order; f16: each query's values scaled by a
+  // power of two so that the largest lies in [2^14, 2^15), undone in `c`
+  Op qf[PARTS][NC];
+  float c = PA_LOG2E / __builtin_sqrtf((float)DH);
+  {
+    float x[NC][PER], top = 0.0f;
+    const float *p = q + row * ldq + (int64_t)(hq + min(r, gq - 1)) * DH + PER * h;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const f4 y = *(const f4 *)(p + M::STEP * i + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][j + e] = r < gq ? y[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(x[i][j + e]));
       }
-      acc[i] = a;
+    int e = 0;
+    if (sizeof(T) == 2 && PARTS == 2) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+      c = ldexpf(c, e);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      Op o[PARTS];
+      if (PARTS == 2)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) x[i][j] = ldexpf(x[i][j], -e);
+      pa_parts<E>(x[i], o);
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) qf[k][i] = o[k];
     }
   }
-  for (int i = 0; i < 2; ++i)
-    if (l + 64 * i < w.dim) o[l + 64 * i] = sum > 0.0f ? acc[i] / sum : 0.0f;
+
+  f4 o[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = NEG_INF, sum = 0.0f;  // query r's; sum: of this lane's keys
+
+  for (; t < end; t += PA_WAVES) {
+    load_v(t, now);
+    const bool more = t + PA_WAVES < end;
+    Where next{};
+    if (more) next = where(t + PA_WAVES);
+    f4 s[SUB];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) s[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) s[u] = M::mma(kf[u][i], qf[k][i], s[u]);
+    if (more) load_k(t + PA_WAVES, next);
+    float x[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = s[j >> 2][j & 3] * c;
+    // keys behind the length, or in a page outside the pool, have no weight,
+    // and what v holds there (anything) is taken as zero
+    if ((t + 1) * KEYS > n || now.bad0 || now.bad1) {
+      const bool bad = KEYS > 16 && h >= 2 ? now.bad1 : now.bad0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (bad || t * KEYS + PER * h + j >= n) {
+          x[j] = NEG_INF;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) vf[i][j] = (T)0.0f;
+        }
+    }
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) top = fmaxf(top, x[j]);
+    if (__builtin_amdgcn_ballot_w64(top > m + PA_SLACK)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float up = fmaxf(m, top), f = pa_weight(m, up);
+      m = up;
+      sum *= f;
+      f4 fr;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[i] *= fr;
+    }
+    const float base = m == NEG_INF ? 0.0f : m - PA_LIFT;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+      sum += x[j];
+    }
+    Op pf[PARTS];
+    pa_parts<E>(x, pf);
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) o[i] = M::mma(pf[k], vf[i], o[i]);
+    now = next;
+  }
+
+  // the wavefronts' runs: scaled to the largest maximum, summed
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if (h == 0) sm[wv][r] = m, sl[wv][r] = sum;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int qr = 4 * h + i;
+    if (qr >= gq) break;
+    float top = sm[0][qr];
+#pragma unroll
+    for (int k = 1; k < PA_WAVES; ++k) top = fmaxf(top, sm[k][qr]);
+    const float f = pa_weight(sm[wv][qr], top);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) so[wv][qr][16 * d + r] = o[d][i] * f;
+  }
+  __syncthreads();
+  const int64_t runs = (int64_t)(gridDim.x / qtiles / kv_heads) * heads * gridDim.y;
+  for (int i = threadIdx.x; i < gq * DH; i += 64 * PA_WAVES) {
+    const int qr = i / DH, d = i % DH;
+    float top = sm[0][qr], l = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int k = 1; k < PA_WAVES; ++k) top = fmaxf(top, sm[k][qr]);
+#pragma unroll
+    for (int k = 0; k < PA_WAVES; ++k) l += sl[k][qr] * pa_weight(sm[k][qr], top), y += so[k][qr][d];
+    if (direct) {
+      orow[i] = l == 0.0f ? 0.0f : y / l;  // 0: no page of the row is in the pool
+    } else {
+      const int64_t run = ((int64_t)row * heads + hq + qr) * gridDim.y + blockIdx.y;
+      part[run * DH + d] = y;
+      if (d == 0) part[runs * DH + 2 * run] = top, part[runs * DH + 2 * run + 1] = l;
+    }
+  }
+}
+
+// The chunks of one (row, query head): out = sum_z o_z 2^(m_z - m) / sum_z l_z
+// 2^(m_z - m).  A row of one chunk was written by k_paged_attn.  The chunks
+// are summed in a fixed order, every SIDE-th by one side, then the sides.
+template <int DH>
+__global__ __launch_bounds__(256) void k_paged_join(const float *__restrict__ part, const int32_t *__restrict__ seq,
+                                                    const int32_t *__restrict__ lens, int n_seqs, int64_t most,
+                                                    int max_len, int chunk, int nsplit, int heads, int64_t runs,
+                                                    float *__restrict__ out, int64_t ldo) {
+  constexpr int W = DH <= 32 ? 32 : DH <= 64 ? 64 : 128, SIDE = 256 / W;  // a side: W threads, a value each
+  __shared__ float sy[SIDE][DH], sw[SIDE];
+  const int row = blockIdx.x / heads, hq = blockIdx.x % heads;
+  int n = min(lens[row], max_len);
+  if (n > most) n = (int)most;
+  if ((unsigned)(seq ? seq[row] : row) >= (unsigned)n_seqs || n <= chunk) return;
+  const int nz = (n + chunk - 1) / chunk;
+  const int64_t run0 = (int64_t)blockIdx.x * nsplit;
+  const float *ml = part + runs * DH + 2 * run0;
+  float top = -__builtin_huge_valf();
+  for (int z = threadIdx.x & 63; z < nz; z += 64) top = fmaxf(top, ml[2 * z]);
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const int g = threadIdx.x / W, d = threadIdx.x % W;
+  float y = 0.0f, l = 0.0f;
+  for (int z = g; z < nz; z += SIDE) {
+    const float w = pa_weight(ml[2 * z], top);
+    l += ml[2 * z + 1] * w;
+    if (d < DH) y += part[(run0 + z) * DH + d] * w;
+  }
+  if (d < DH) sy[g][d] = y;
+  if (d == 0) sw[g] = l;
+  __syncthreads();
+  if (threadIdx.x < DH) {
+    y = l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SIDE; ++i) y += sy[i][threadIdx.x], l += sw[i];
+    out[row * ldo + (int64_t)hq * DH + threadIdx.x] = l == 0.0f ? 0.0f : y / l;
+  }
 }
 
 #endif  // __HIPCC__

@@ -108,6 +108,106 @@ static PagedView paged_view(const rw_kv_pages *p, size_t layer, const int32_t *t
     else CALL(BF16);                   \
   } while (0)
 
+// ------------------------------------------------------------ attention
+
+static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size_t max_len) {
+  if (n_head < 1 || n_head % p->n_head)
+    return fail(RW_EINVAL, "n_head %d is not a positive multiple of the pages' %d", n_head, p->n_head);
+  if (rows > ((size_t)INT32_MAX - 64) / n_head) return fail(RW_EINVAL, "%zu rows of %d heads", rows, n_head);
+  if (max_len > (size_t)INT32_MAX) return fail(RW_EINVAL, "max_len %zu", max_len);
+  return RW_OK;
+}
+
+// How a launch cuts its rows' keys: chunks of `chunk` keys, `nsplit` of them
+// for the longest row.  `most`, of which the workspace's size is made, is no
+// less than nsplit and never falls with max_len.
+struct PagedPlan {
+  size_t base;  // workgroups per chunk
+  int chunk, nsplit;
+  size_t most;
+  size_t runs;  // partial results
+};
+static PagedPlan paged_plan(const rw_kv_pages *p, size_t rows, int n_head, size_t max_len) {
+  PagedPlan L{};
+  const size_t group = (size_t)n_head / p->n_head;
+  max_len = std::min(max_len, (size_t)1 << 30);
+  L.base = rows * p->n_head * cdiv(group, 16);
+  const size_t few = std::min(cdiv(max_len, 256), std::max((size_t)1, 2048 / L.base));
+  size_t nsplit = std::max(few, cdiv(max_len, 2048));
+  nsplit = std::max((size_t)1, std::min(nsplit, std::max((size_t)1, 16384 / L.base)));
+  L.most = nsplit;
+  L.chunk = (int)(cdiv(std::max(max_len, (size_t)1), nsplit * 128) * 128);
+  L.nsplit = (int)std::max((size_t)1, cdiv(max_len, (size_t)L.chunk));
+  L.runs = rows * n_head * (size_t)L.nsplit;
+  return L;
+}
+static size_t paged_bytes(const PagedPlan &L, size_t rows, int n_head, int head_size) {
+  return L.most > 1 ? rows * n_head * L.most * (head_size + 2) * 4 : 0;
+}
+
+struct PagedCall {
+  PagedView w;
+  const float *q;
+  int64_t ldq;
+  int rows, n_head, max_len;
+  const int32_t *len;
+  float *out;
+  int64_t ldo;
+  float *part;
+};
+
+template <class E, int DH>
+static int launch_paged(const PagedCall &c, const PagedPlan &L, hipStream_t s) {
+  const PagedView &w = c.w;
+  hipLaunchKernelGGL((k_paged_attn<E, DH>), dim3((unsigned)L.base, (unsigned)L.nsplit), dim3(64 * PA_WAVES), 0, s, w.k,
+                     w.v, c.q, w.table, w.seq, c.len, c.out, c.part, w.heads, c.n_head / w.heads, w.pr, w.n_pages,
+                     w.n_seqs, w.ld, c.ldq, c.ldo, c.max_len, L.chunk);
+  SERVE_TRY(launched("k_paged_attn"));
+  if (L.nsplit == 1) return RW_OK;
+  hipLaunchKernelGGL((k_paged_join<DH>), dim3((unsigned)(c.rows * c.n_head)), dim3(256), 0, s, c.part, w.seq, c.len,
+                     w.n_seqs, w.ld << w.pr, c.max_len, L.chunk, L.nsplit, c.n_head, (int64_t)L.runs, c.out, c.ldo);
+  return launched("k_paged_join");
+}
+
+template <class E>
+static int launch_paged_dim(const PagedCall &c, const PagedPlan &L, hipStream_t s) {
+  switch (c.w.dim) {
+    case 32: return launch_paged<E, 32>(c, L, s);
+    case 64: return launch_paged<E, 64>(c, L, s);
+    case 96: return launch_paged<E, 96>(c, L, s);
+    default: return launch_paged<E, 128>(c, L, s);
+  }
+}
+
+// The workspace of a call: the caller's, or this stream's.  A stream that is
+// being captured has to bring one: the library's may be replaced by a later
+// call while the graph still uses it.
+struct CallWorkspace {
+  void *slot = nullptr;
+  CallWorkspace() = default;
+  CallWorkspace(const CallWorkspace &) = delete;
+  CallWorkspace &operator=(const CallWorkspace &) = delete;
+  ~CallWorkspace() {
+    if (slot) rw_internal_workspace_release(slot);
+  }
+  int take(int dev, void *given, size_t len, size_t need, void *stream, void **out) {
+    *out = given;
+    if (need == 0) return RW_OK;
+    if (given) {
+      if (len < need) return fail(RW_EINVAL, "workspace of %zu bytes < %zu needed", len, need);
+      if (!aligned(given, 16)) return fail(RW_EINVAL, "the workspace must be 16-byte aligned");
+      return RW_OK;
+    }
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &st);
+    if (e != hipSuccess) return fail(RW_EHIP, "hipStreamIsCapturing: %s", hipGetErrorString(e));
+    if (st != hipStreamCaptureStatusNone) return fail(RW_EINVAL, "a captured call needs a workspace of %zu bytes", need);
+    return rw_internal_workspace(dev, stream, need, &slot, out);
+  }
+};
+
+// ----------------------------------------------------------------- book
+
 struct rw_kv_book {
   KvBook b;
 };
@@ -201,16 +301,9 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
   return RW_OK;
 }
 
-static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size_t max_len) {
-  if (n_head < 1 || n_head % p->n_head)
-    return fail(RW_EINVAL, "n_head %d is not a positive multiple of the pages' %d", n_head, p->n_head);
-  if (rows > ((size_t)INT32_MAX - 64) / n_head) return fail(RW_EINVAL, "%zu rows of %d heads", rows, n_head);
-  if (max_len > (size_t)INT32_MAX) return fail(RW_EINVAL, "max_len %zu", max_len);
-  return RW_OK;
-}
-
 size_t rw_rocm_paged_attention_workspace_size(const rw_kv_pages *pages, size_t rows, int n_head, size_t max_len) {
-  return 0;
+  if (check_pages(pages) || check_paged_heads(pages, rows, n_head, max_len) || rows == 0) return 0;
+  return paged_bytes(paged_plan(pages, rows, n_head, max_len), rows, n_head, pages->head_size);
 }
 
 int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const float *q, size_t ldq, size_t rows,
@@ -227,14 +320,23 @@ int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const fl
   SERVE_TRY(check_table(table, ld_table, n_seqs, rows, seq, len, "len"));
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
-  const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
-  const float scale = 1.0f / sqrtf((float)pages->head_size);
-#define RW_ATTN(E)                                                                                               \
-  hipLaunchKernelGGL((k_paged_attn<E>), dim3((unsigned)(rows * n_head)), dim3(64), 0, (hipStream_t)stream, w, q, \
-                     (int64_t)ldq, n_head, len, (int)max_len, scale, out, (int64_t)ldo)
-  BY_TYPE(pages->dtype, RW_ATTN);
-#undef RW_ATTN
-  return launched("k_paged_attn");
+  PagedCall c{paged_view(pages, layer, table, ld_table, n_seqs, seq), q, (int64_t)ldq, (int)rows, n_head, 0, len, out,
+              (int64_t)ldo, nullptr};
+  c.max_len = (int)std::min(max_len, std::min((size_t)1 << 30, ld_table * pages->page_rows));
+  const PagedPlan L = paged_plan(pages, rows, n_head, (size_t)c.max_len);
+  // told by max_len alone, so that the size does not depend on the table's width
+  const size_t need = workspace ? rw_rocm_paged_attention_workspace_size(pages, rows, n_head, max_len)
+                                : paged_bytes(L, rows, n_head, pages->head_size);
+  CallWorkspace hold;
+  void *ws = nullptr;
+  SERVE_TRY(hold.take(dev, workspace, workspace_len, need, stream, &ws));
+  c.part = (float *)ws;
+  hipStream_t s = (hipStream_t)stream;
+  switch (pages->dtype) {
+    case RW_F32: return launch_paged_dim<F32>(c, L, s);
+    case RW_F16: return launch_paged_dim<F16>(c, L, s);
+    default: return launch_paged_dim<BF16>(c, L, s);
+  }
 }
 
 int rw_rocm_kv_book_create(size_t n_pages, size_t page_rows, size_t max_seqs, rw_kv_book **out) {
