@@ -8,6 +8,7 @@ fallback: if the library or a gfx950 device is missing, calls raise.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import re
 
@@ -561,23 +562,37 @@ def logits_topk_workspace_size(rows: int, n_vocab: int, k: int) -> int:
 _TORCH_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
 
 
+# a dtype's name: a step's calls look at a dozen arrays, and str() of a dtype takes 0.4 us
+_dtype_name = functools.lru_cache(None)(str)
+
+
 def _dense(a, dtype: str, what: str):
     """_ptr of a device array, which as a tensor must be dense and of `dtype`."""
-    if hasattr(a, "data_ptr"):
-        if str(a.dtype) != dtype or not a.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous {dtype} tensor")
-        return a.data_ptr()
-    return _ptr(a)
+    try:
+        p = a.data_ptr()
+    except AttributeError:
+        return _ptr(a)
+    if _dtype_name(a.dtype) != dtype or not a.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor")
+    return p
 
 
 def _rows(a, n: int, ld: int | None, what: str, dtypes=("torch.float32",)):
     """(pointer, row stride) of device rows of n values; a 2-D tensor, which
     may be a column block of wider rows, brings its stride."""
-    if not hasattr(a, "data_ptr"):
+    try:
+        p = a.data_ptr()
+    except AttributeError:
         return _ptr(a), ld or n
-    if str(a.dtype) not in dtypes or (a.dim() and a.shape[-1] > 1 and a.stride(-1) != 1):
+    st, shape = a.stride(), a.shape
+    if _dtype_name(a.dtype) not in dtypes or (st and st[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
-    return a.data_ptr(), ld or (a.stride(0) if a.dim() == 2 and a.shape[0] > 1 else n)
+    return p, ld or (st[0] if len(st) == 2 and shape[0] > 1 else n)
+
+
+def _host(a: np.ndarray) -> int:
+    """A host array's address (ndarray.ctypes.data in a third of its time)."""
+    return a.__array_interface__["data"][0]
 
 
 class KvPages:
@@ -587,14 +602,15 @@ class KvPages:
 
     def __init__(self, k, v):
         L, N, H, P, D = k.shape
-        if tuple(v.shape) != (L, N, H, D, P):
+        if v.shape != (L, N, H, D, P):
             raise ValueError("v must be [n_layer, n_pages, n_head, head_size, page_rows]")
-        if k.dtype != v.dtype or str(k.dtype) not in _TORCH_DTYPES:
+        dtype = _TORCH_DTYPES.get(_dtype_name(k.dtype))
+        if k.dtype != v.dtype or dtype is None:
             raise ValueError("k and v must have one type: float32, float16 or bfloat16")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("k and v must be contiguous")
         self.k, self.v = k, v  # keeps the tensors alive
-        self.st = RwKvPages(_TORCH_DTYPES[str(k.dtype)], H, D, P, L, N, k.data_ptr(), v.data_ptr())
+        self.st = RwKvPages(dtype, H, D, P, L, N, k.data_ptr(), v.data_ptr())
 
     @property
     def n_values(self) -> int:
@@ -624,7 +640,7 @@ def kv_copy_pages_dev(pages: KvPages, src, dst, stream: int | None = None) -> No
     b = np.ascontiguousarray(dst, dtype=np.int32)
     if a.ndim != 1 or a.shape != b.shape:
         raise ValueError("src and dst must be two lists of the same length")
-    check(lib().rw_rocm_kv_copy_pages_dev(pages.st, a.ctypes.data, b.ctypes.data, a.size, stream))
+    check(lib().rw_rocm_kv_copy_pages_dev(pages.st, _host(a), _host(b), a.size, stream))
 
 
 def paged_attention_workspace_size(pages: KvPages, rows: int, n_head: int, max_len: int) -> int:
@@ -725,6 +741,12 @@ class KvBook:
 
 # --------------------------------------------------------- token scores
 
+def _ids(a, what: str):
+    """_dense of 32-bit ids, signed or not."""
+    unsigned = _dtype_name(getattr(a, "dtype", None)) == "torch.uint32"
+    return _dense(a, "torch.uint32" if unsigned else "torch.int32", what)
+
+
 def token_logprobs_workspace_size(rows: int, n_vocab: int, k: int) -> int:
     return lib().rw_rocm_token_logprobs_workspace_size(rows, n_vocab, k)
 
@@ -736,13 +758,11 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
     largest alternatives of every row of device logits; `dtype` is taken from a
     logits tensor (F32 for a pointer)."""
     if dtype is None:
-        dtype = _TORCH_DTYPES.get(str(logits.dtype), -1) if hasattr(logits, "data_ptr") else F32
-    ids = "torch.uint32" if "uint32" in str(getattr(tokens, "dtype", "")) else "torch.int32"
-    tid = "torch.uint32" if "uint32" in str(getattr(top_ids, "dtype", "")) else "torch.int32"
+        dtype = _TORCH_DTYPES.get(_dtype_name(logits.dtype), -1) if hasattr(logits, "data_ptr") else F32
     check(lib().rw_rocm_token_logprobs_dev(
-        dtype, *_rows(logits, n_vocab, ld, "logits", tuple(_TORCH_DTYPES)), rows, n_vocab, _dense(tokens, ids, "tokens"), n_tok,
+        dtype, *_rows(logits, n_vocab, ld, "logits", tuple(_TORCH_DTYPES)), rows, n_vocab, _ids(tokens, "tokens"), n_tok,
         _dense(logprobs, "torch.float32", "logprobs"), _dense(entropy, "torch.float32", "entropy"), k,
-        _dense(top_ids, tid, "top_ids"), _dense(top_logprobs, "torch.float32", "top_logprobs"), _ptr(workspace),
+        _ids(top_ids, "top_ids"), _dense(top_logprobs, "torch.float32", "top_logprobs"), _ptr(workspace),
         workspace_len, stream))
 
 

@@ -384,39 +384,50 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
 }
 
 // The chunks of one (row, query head): out = sum_z o_z 2^(m_z - m) / sum_z l_z
-// 2^(m_z - m).  A row of one chunk was written by k_paged_attn.  The chunks
-// are summed in a fixed order, every SIDE-th by one side, then the sides.
+// 2^(m_z - m).  A row of one chunk was written by k_paged_attn.  The chunks'
+// weights go to LDS; then SIDE groups of threads, four values each, sum every
+// SIDE-th chunk in order, and the groups' sums are added in order.
+constexpr int PA_MAX_SPLIT = 1024;
 template <int DH>
 __global__ __launch_bounds__(256) void k_paged_join(const float *__restrict__ part, const int32_t *__restrict__ seq,
                                                     const int32_t *__restrict__ lens, int n_seqs, int64_t most,
                                                     int max_len, int chunk, int nsplit, int heads, int64_t runs,
                                                     float *__restrict__ out, int64_t ldo) {
-  constexpr int W = DH <= 32 ? 32 : DH <= 64 ? 64 : 128, SIDE = 256 / W;  // a side: W threads, a value each
-  __shared__ float sy[SIDE][DH], sw[SIDE];
+  constexpr int W = DH <= 32 ? 8 : DH <= 64 ? 16 : 32, SIDE = 256 / W;  // W threads of 4 values
+  __shared__ float sw[PA_MAX_SPLIT], sl[4];
+  __shared__ f4 sy[SIDE][DH / 4];
   const int row = blockIdx.x / heads, hq = blockIdx.x % heads;
   int n = min(lens[row], max_len);
   if (n > most) n = (int)most;
   if ((unsigned)(seq ? seq[row] : row) >= (unsigned)n_seqs || n <= chunk) return;
-  const int nz = (n + chunk - 1) / chunk;
+  const int nz = (n + chunk - 1) / chunk;  // <= nsplit <= PA_MAX_SPLIT
   const int64_t run0 = (int64_t)blockIdx.x * nsplit;
   const float *ml = part + runs * DH + 2 * run0;
-  float top = -__builtin_huge_valf();
+  float top = -__builtin_huge_valf(), l = 0.0f;
   for (int z = threadIdx.x & 63; z < nz; z += 64) top = fmaxf(top, ml[2 * z]);
   for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-  const int g = threadIdx.x / W, d = threadIdx.x % W;
-  float y = 0.0f, l = 0.0f;
-  for (int z = g; z < nz; z += SIDE) {
+  for (int z = threadIdx.x; z < nz; z += 256) {
     const float w = pa_weight(ml[2 * z], top);
+    sw[z] = w;
     l += ml[2 * z + 1] * w;
-    if (d < DH) y += part[(run0 + z) * DH + d] * w;
   }
-  if (d < DH) sy[g][d] = y;
-  if (d == 0) sw[g] = l;
+  for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+  if ((threadIdx.x & 63) == 0) sl[threadIdx.x >> 6] = l;
+  __syncthreads();
+  const int g = threadIdx.x / W, d = threadIdx.x % W;
+  if (d < DH / 4) {
+    f4 y{0.0f, 0.0f, 0.0f, 0.0f};
+    const f4 *o = (const f4 *)(part + run0 * DH) + d;
+#pragma unroll 4
+    for (int z = g; z < nz; z += SIDE) y += o[z * (DH / 4)] * sw[z];
+    sy[g][d] = y;
+  }
   __syncthreads();
   if (threadIdx.x < DH) {
-    y = l = 0.0f;
+    float y = 0.0f;
 #pragma unroll
-    for (int i = 0; i < SIDE; ++i) y += sy[i][threadIdx.x], l += sw[i];
+    for (int i = 0; i < SIDE; ++i) y += ((const float *)sy[i])[threadIdx.x];
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
     out[row * ldo + (int64_t)hq * DH + threadIdx.x] = l == 0.0f ? 0.0f : y / l;
   }
 }

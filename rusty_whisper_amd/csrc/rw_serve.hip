@@ -132,9 +132,13 @@ static PagedPlan paged_plan(const rw_kv_pages *p, size_t rows, int n_head, size_
   const size_t group = (size_t)n_head / p->n_head;
   max_len = std::min(max_len, (size_t)1 << 30);
   L.base = rows * p->n_head * cdiv(group, 16);
-  const size_t few = std::min(cdiv(max_len, 256), std::max((size_t)1, 2048 / L.base));
-  size_t nsplit = std::max(few, cdiv(max_len, 2048));
-  nsplit = std::max((size_t)1, std::min(nsplit, std::max((size_t)1, 16384 / L.base)));
+  const size_t bytes = max_len * 2 * p->head_size * elem_size(p->dtype);
+  size_t nsplit = 1;
+  if (bytes > (size_t)256 << 10) {
+    nsplit = std::min(cdiv(bytes, (size_t)128 << 10), 512 / L.base);
+    if (rows > 1) nsplit = std::max(nsplit, std::min(cdiv(bytes, (size_t)192 << 10), 4096 / L.base));
+    nsplit = std::max((size_t)1, std::min(nsplit, (size_t)PA_MAX_SPLIT));
+  }
   L.most = nsplit;
   L.chunk = (int)(cdiv(std::max(max_len, (size_t)1), nsplit * 128) * 128);
   L.nsplit = (int)std::max((size_t)1, cdiv(max_len, (size_t)L.chunk));
