@@ -444,7 +444,7 @@ size_t rw_rocm_logits_topk_workspace_size(size_t rows, size_t n_vocab, size_t k)
  * the work runs: a captured graph may be replayed with other contents.  The
  * kernels check them: a row whose sequence or position the table does not
  * have is not written, and attends to nothing; a page id outside the pool
- * holds no rows. */
+ * holds no rows.  A call takes up to 2^23 rows (attention: rows times n_head). */
 typedef struct rw_kv_pages {
   int dtype;
   int n_head, head_size, page_rows;
@@ -541,7 +541,8 @@ int rw_rocm_kv_book_info(const rw_kv_book *b, size_t *free_pages, size_t *used_p
  * Logits of -inf (suppressed tokens) have log-prob -inf and add nothing to
  * the entropy.  A row holding NaN or +inf, or only -inf, has NaN log-probs and
  * entropy, and ids 0xFFFFFFFF with NaN for its alternatives.  Every logit is
- * read once; sums are f32 in a fixed order.  n_vocab < 2^31.  The workspace
+ * read once; sums are f32 in a fixed order, and what f32 cannot hold is rounded
+ * as f32 does.  n_vocab < 2^31, rows <= 2^23.  The workspace
  * (NULL: one kept per (device, stream), not for a stream that is being
  * captured) holds rw_rocm_token_logprobs_workspace_size bytes, 16-byte
  * aligned. */

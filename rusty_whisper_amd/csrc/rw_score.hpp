@@ -4,88 +4,341 @@
 // With M = max x, S = sum e^(x - M), T = sum (x - M) e^(x - M):
 //   lp(t) = x_t - M - ln S,   entropy = ln S - T / S
 // (both terms of the entropy are non-negative, so nothing cancels).
+//
+// k_score reads its part of a row once, in steps of 64 x PER logits per
+// wavefront, which stay in registers while the step's maximum, sums and
+// candidates are formed.  A lane keeps M, S and T of its own logits (raised
+// maxima scale S and T); lanes, wavefronts and parts are joined at the end in
+// a fixed order.
+//
+// The alternatives.  A wavefront keeps its k best so far and `thr`, the k-th's
+// logit.  Ids rise with the steps, so a later logit enters only if it is
+// larger than thr, and most steps end with one comparison of the lanes'
+// maxima.  Where at least k lanes' maxima pass thr, the k-th largest of them
+// bounds the k-th best from below: only logits from there on are candidates
+// (on rows in no special order little more than k).  Candidates are collected
+// in the order of their ids behind the k best, and each one's rank is the
+// number of entries before it (larger, or equal with a smaller id).
 #pragma once
 #include "rw_kv.hpp"
 
 namespace rw {
 
-constexpr int SCORE_TOP = 32;  // alternatives per row at most
+constexpr int SCORE_TOP = 32;         // alternatives per row at most
+constexpr int SCORE_MAX_PARTS = 64;   // parts of a row: a lane each in k_score_join
+constexpr uint32_t SCORE_NONE = 0xFFFFFFFFu;
 
 #if defined(__HIPCC__)
 
-__device__ inline float score_max(float v, float *scratch) {
-  for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
-}
-__device__ inline float score_sum(float v, float *scratch) {
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
-}
-__device__ inline int score_imin(int v, int *scratch) {
-  for (int o = 1; o < 64; o <<= 1) v = min(v, __shfl_xor(v, o));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return min(min(scratch[0], scratch[1]), min(scratch[2], scratch[3]));
+struct ScoreOut {
+  const uint32_t *tokens;
+  float *logprobs, *entropy;
+  uint32_t *top_ids;
+  float *top_lp;
+  int64_t n_tok;
+  int k;
+};
+
+// A part's results for k_score_join: M, S, T and its k best (rest: id NONE)
+struct ScorePart {
+  float m, s, t;
+  int pad;
+};
+
+struct ScoreStats {
+  float m, s, t;
+};
+// the sums of both, to the larger maximum (-inf where there is no logit; NaN sums stay)
+__device__ inline ScoreStats score_join(const ScoreStats &a, const ScoreStats &b) {
+  constexpr float NEG_INF = -__builtin_huge_valf();
+  ScoreStats c{fmaxf(a.m, b.m), 0.0f, 0.0f};
+  const float da = a.m == NEG_INF ? 0.0f : a.m - c.m, db = b.m == NEG_INF ? 0.0f : b.m - c.m;
+  // a difference beyond f32's range weighs nothing (0 instead of -inf x 0)
+  const float fa = __builtin_amdgcn_exp2f(da * PA_LOG2E), fb = __builtin_amdgcn_exp2f(db * PA_LOG2E);
+  c.s = a.s * fa + b.s * fb;
+  c.t = (a.t + fmaxf(da, -200.0f) * a.s) * fa + (b.t + fmaxf(db, -200.0f) * b.s) * fb;
+  return c;
 }
 
-// One workgroup per row, which reads the row for the maximum, for the sums
-// and once per alternative.
+template <int CTRL, int ROWS = 0xf>
+__device__ inline float score_dpp(float v) {
+  const int i = __float_as_int(v);
+  return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, ROWS, 0xf, false));
+}
+// the wavefront's largest value, in every lane
+__device__ inline float score_wave_max(float v) {
+  v = fmaxf(v, score_dpp<0x111>(v));  // row_shr 1, 2, 4, 8
+  v = fmaxf(v, score_dpp<0x112>(v));
+  v = fmaxf(v, score_dpp<0x114>(v));
+  v = fmaxf(v, score_dpp<0x118>(v));
+  v = fmaxf(v, score_dpp<0x142, 0xa>(v));  // row_bcast 15 into rows 1 and 3
+  v = fmaxf(v, score_dpp<0x143, 0xc>(v));  // row_bcast 31 into rows 2 and 3
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ inline float score_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
+
+// LDS that one wavefront's lanes write and read: its operations keep their order
+__device__ inline void score_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// entry (v, i) comes before (w, j)
+__device__ inline bool score_before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+
+// log-probs, entropy and alternatives of a row from its sums and its k best
+// (LDS; id NONE where there are fewer), by one workgroup
 template <class E>
-__global__ __launch_bounds__(256) void k_score_row(const typename E::T *__restrict__ logits, int64_t ld, int n,
-                                                   const uint32_t *__restrict__ tokens, int64_t n_tok,
-                                                   float *__restrict__ logprobs, float *__restrict__ entropy, int k,
-                                                   uint32_t *__restrict__ top_ids, float *__restrict__ top_lp) {
+__device__ inline void score_finish(const typename E::T *x, int n, int64_t row, const ScoreStats &st, const float *bv,
+                                    const int *bi, const ScoreOut &o) {
+  const float nan = __builtin_nanf("");
+  // NaN sums: a NaN or +inf among the logits; M = -inf: nothing else in the row
+  const bool bad = !(st.s > 0.0f) || st.m == -__builtin_huge_valf();
+  const float ls = logf(st.s);
+  if (threadIdx.x == 0 && o.entropy) o.entropy[row] = bad ? nan : ls - st.t / st.s;
+  if ((int)threadIdx.x < o.k) {
+    const int id = bi[threadIdx.x];
+    o.top_ids[row * o.k + threadIdx.x] = bad ? SCORE_NONE : (uint32_t)id;
+    o.top_lp[row * o.k + threadIdx.x] = bad ? nan : id == (int)SCORE_NONE ? -__builtin_huge_valf() : (bv[threadIdx.x] - st.m) - ls;
+  }
+  for (int64_t i = threadIdx.x; i < o.n_tok; i += 256) {
+    const uint32_t id = o.tokens[row * o.n_tok + i];
+    float lp = nan;
+    if (id == SCORE_NONE) lp = 0.0f;
+    else if (id < (uint32_t)n && !bad) lp = (E::load(x + id) - st.m) - ls;
+    o.logprobs[row * o.n_tok + i] = lp;
+  }
+}
+
+// NJ: 16-byte loads per lane and step.  blockIdx.x = row * parts + part.
+template <class E, int NJ>
+__global__ __launch_bounds__(256) void k_score(const typename E::T *__restrict__ logits, int64_t ld, int n, int parts,
+                                               int64_t part_len, ScoreOut o, ScorePart *__restrict__ ps,
+                                               float *__restrict__ pv, int *__restrict__ pi) {
+  using T = typename E::T;
   constexpr float NEG_INF = -__builtin_huge_valf();
-  __shared__ float sf[4];
-  __shared__ int si[4];
+  constexpr int V = 16 / sizeof(T), PER = NJ * V, CAP = SCORE_TOP + 64 * V;
+  typedef T Vec __attribute__((ext_vector_type(V)));
+  __shared__ float ev[4][CAP];  // per wavefront: its k best, then candidates
+  __shared__ int ei[4][CAP];
+  __shared__ ScoreStats ss[4];
+  __shared__ float bv[SCORE_TOP];
+  __shared__ int bi[SCORE_TOP], en[4];
+  const int64_t row = blockIdx.x / parts;
+  const int pt = blockIdx.x % parts, k = o.k;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T *x = logits + row * ld;
+  // places count from the 16-byte boundary at or before the row's start
+  const int skip = (int)(((uintptr_t)x & 15) / sizeof(T));
+  const int64_t u1 = min((int64_t)n + skip, (int64_t)(pt + 1) * part_len);
+
+  ScoreStats st{NEG_INF, 0.0f, 0.0f};
+  float thr = NEG_INF;
+  int cnt = 0;  // entries of ev / ei
+  float *wv_v = ev[wv];
+  int *wv_i = ei[wv];
+
+  // the k first of the cnt entries to the front, in order
+  auto keep = [&]() __attribute__((always_inline)) {
+    score_wave_sync();
+    if (cnt <= 64) {
+      const float v = lane < cnt ? wv_v[lane] : NEG_INF;
+      const int id = lane < cnt ? wv_i[lane] : INT32_MAX;
+      int rank = lane < cnt ? 0 : 64;
+      for (int e = 0; e < cnt; ++e)
+        rank += score_before(score_lane(v, e), __builtin_amdgcn_readlane(id, e), v, id);
+      score_wave_sync();
+      if (rank < k) wv_v[rank] = v, wv_i[rank] = id;
+    } else {
+      // many equal logits: k rounds, each entry looked at by one lane
+      float pv0 = __builtin_huge_valf();
+      int pi0 = -1;
+      float kv = NEG_INF;
+      int ki = INT32_MAX;
+      for (int r = 0; r < k; ++r) {
+        float v = NEG_INF;
+        int id = INT32_MAX;
+        for (int e = lane; e < cnt; e += 64)
+          if (score_before(pv0, pi0, wv_v[e], wv_i[e]) && score_before(wv_v[e], wv_i[e], v, id)) v = wv_v[e], id = wv_i[e];
+        pv0 = score_wave_max(v);
+        int mi = v == pv0 ? id : INT32_MAX;
+        for (int s = 1; s < 64; s <<= 1) mi = min(mi, __shfl_xor(mi, s));
+        pi0 = mi;
+        if (lane == r) kv = pv0, ki = pi0;
+      }
+      score_wave_sync();
+      if (lane < k) wv_v[lane] = kv, wv_i[lane] = ki;
+    }
+    cnt = min(cnt, k);
+    score_wave_sync();
+    if (cnt == k) thr = wv_v[k - 1];
+  };
+
+  for (int64_t u = (int64_t)pt * part_len + wv * 64 * PER; u < u1; u += 256 * PER) {
+    // e0: this lane's first id of the step (its j-th load has ids e0 + 64 V j .. + V - 1)
+    const int64_t w0 = u - skip, e0 = w0 + lane * V;
+    float y[PER];
+    if (w0 >= 0 && w0 + 64 * PER <= n) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const Vec q = *(const Vec *)(x + e0 + 64 * V * j);
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[j * V + i] = (float)q[i];
+      }
+    } else {  // a step that the row does not fill
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int64_t e = e0 + 64 * V * j + i;
+          y[j * V + i] = e >= 0 && e < n ? E::load(x + e) : NEG_INF;
+        }
+    }
+    float mx = y[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) mx = fmaxf(mx, y[j]);
+    {
+      const ScoreStats none{mx, 0.0f, 0.0f};
+      if (mx > st.m) st = score_join(st, none);
+      const float m0 = st.m == NEG_INF ? 0.0f : st.m;
+      float s = 0.0f, t = 0.0f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float d = y[j] - m0, e = __builtin_amdgcn_exp2f(d * PA_LOG2E);
+        s += e;
+        t = fmaf(fmaxf(d, -200.0f), e, t);
+      }
+      st.s += s, st.t += t;
+    }
+    if (k == 0) continue;
+    const uint64_t pass = __builtin_amdgcn_ballot_w64(mx > thr);
+    if (!pass) continue;
+    float low = NEG_INF;  // candidates are >= low
+    if (__builtin_popcountll(pass) >= k) {
+      int rank = 0;
+#pragma unroll 8
+      for (int e = 0; e < 64; ++e) {
+        const float w = score_lane(mx, e);
+        rank += w > mx || (w == mx && e < lane);
+      }
+      low = score_lane(mx, __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == k - 1)));
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) c += y[j * V + i] > thr && y[j * V + i] >= low;
+      if (!__builtin_amdgcn_ballot_w64(c > 0)) continue;
+      int before = c;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const int w = __shfl_up(before, s);
+        if (lane >= s) before += w;
+      }
+      const int total = __builtin_amdgcn_readlane(before, 63);
+      if (cnt + total > CAP) {
+        keep();  // to k entries: total <= 64 V fits behind them
+        c = 0;   // thr has risen
+#pragma unroll
+        for (int i = 0; i < V; ++i) c += y[j * V + i] > thr && y[j * V + i] >= low;
+        before = c;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+          const int w = __shfl_up(before, s);
+          if (lane >= s) before += w;
+        }
+      }
+      int at = cnt + before - c;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (y[j * V + i] > thr && y[j * V + i] >= low) wv_v[at] = y[j * V + i], wv_i[at] = (int)(e0 + 64 * V * j + i), ++at;
+      cnt += __builtin_amdgcn_readlane(before, 63);
+    }
+    if (cnt > k || thr == NEG_INF) keep();
+  }
+
+  // lanes, then wavefronts
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const ScoreStats w{__shfl_xor(st.m, s), __shfl_xor(st.s, s), __shfl_xor(st.t, s)};
+    st = score_join(st, w);
+  }
+  if (lane == 0) ss[wv] = st, en[wv] = cnt;
+  if (threadIdx.x < SCORE_TOP) bv[threadIdx.x] = NEG_INF, bi[threadIdx.x] = (int)SCORE_NONE;
+  __syncthreads();
+  st = score_join(score_join(ss[0], ss[1]), score_join(ss[2], ss[3]));
+  if ((int)threadIdx.x < 4 * k) {
+    const int a = threadIdx.x / k, b = threadIdx.x % k;
+    if (b < en[a]) {
+      const float v = ev[a][b];
+      const int id = ei[a][b];
+      int rank = b;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (c != a)
+          for (int e = 0; e < en[c]; ++e) rank += score_before(ev[c][e], ei[c][e], v, id);
+      if (rank < k) bv[rank] = v, bi[rank] = id;
+    }
+  }
+  __syncthreads();
+  if (parts == 1) {
+    score_finish<E>(x, n, row, st, bv, bi, o);
+  } else {
+    if (threadIdx.x == 0) ps[blockIdx.x] = ScorePart{st.m, st.s, st.t, 0};
+    if ((int)threadIdx.x < k) {
+      pv[(int64_t)blockIdx.x * k + threadIdx.x] = bv[threadIdx.x];
+      pi[(int64_t)blockIdx.x * k + threadIdx.x] = bi[threadIdx.x];
+    }
+  }
+}
+
+// The parts of a row: sums in order, and the k best by taking the best head
+// of the parts' lists k times (a lane a list).
+template <class E>
+__global__ __launch_bounds__(256) void k_score_join(const typename E::T *__restrict__ logits, int64_t ld, int n, int parts,
+                                                    ScoreOut o, const ScorePart *__restrict__ ps,
+                                                    const float *__restrict__ pv, const int *__restrict__ pi) {
+  constexpr float NEG_INF = -__builtin_huge_valf();
+  __shared__ float lv[SCORE_MAX_PARTS * SCORE_TOP], bv[SCORE_TOP];
+  __shared__ int li[SCORE_MAX_PARTS * SCORE_TOP], bi[SCORE_TOP];
   const int64_t row = blockIdx.x;
-  const int t = threadIdx.x;
-  const typename E::T *x = logits + row * ld;
-  float m = NEG_INF;
-  for (int i = t; i < n; i += 256) m = fmaxf(m, E::load(x + i));
-  m = score_max(m, sf);
-  float s = 0.0f, u = 0.0f;
-  for (int i = t; i < n; i += 256) {
-    const float d = E::load(x + i) - m, e = expf(d);
-    s += e;
-    if (e != 0.0f) u += d * e;  // also NaN
+  const int k = o.k, lane = threadIdx.x & 63;
+  for (int e = threadIdx.x; e < parts * k; e += 256) lv[e] = pv[row * parts * k + e], li[e] = pi[row * parts * k + e];
+  ScoreStats st{NEG_INF, 0.0f, 0.0f};
+  if (lane < parts) {
+    const ScorePart p = ps[row * parts + lane];
+    st = ScoreStats{p.m, p.s, p.t};
   }
-  s = score_sum(s, sf);
-  u = score_sum(u, sf);
-  const float ls = logf(s);
-  const bool bad = !(s > 0.0f);  // NaN: a NaN or +inf among the logits, or only -inf
-  if (t == 0 && entropy) entropy[row] = bad ? __builtin_nanf("") : ls - u / s;
-  for (int64_t i = t; i < n_tok; i += 256) {
-    const uint32_t id = tokens[row * n_tok + i];
-    float lp = __builtin_nanf("");
-    if (id == 0xFFFFFFFFu) lp = 0.0f;
-    else if (id < (uint32_t)n && !bad) lp = (E::load(x + id) - m) - ls;
-    logprobs[row * n_tok + i] = lp;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const ScoreStats w{__shfl_xor(st.m, s), __shfl_xor(st.s, s), __shfl_xor(st.t, s)};
+    st = score_join(st, w);
   }
-  float pv = __builtin_huge_valf();
-  int pi = -1;
-  for (int j = 0; j < k; ++j) {
-    float bv = NEG_INF;
-    int bi = INT32_MAX;
-    for (int i = t; i < n && !bad; i += 256) {
-      const float v = E::load(x + i);
-      if ((v < pv || (v == pv && i > pi)) && v > bv) bv = v, bi = i;
+  __syncthreads();
+  if (threadIdx.x < 64 && k) {
+    int at = 0;
+    float v = lane < parts ? lv[lane * k] : NEG_INF;
+    int id = lane < parts ? li[lane * k] : (int)SCORE_NONE;
+    for (int r = 0; r < k; ++r) {
+      // (a list's rest holds -inf and NONE: it never wins against an entry, and
+      // where no entry is left the winner's place gets just that)
+      const float top = score_wave_max(v);
+      uint64_t who = __builtin_amdgcn_ballot_w64(v == top);
+      if (__builtin_popcountll(who) > 1) {
+        int mi = v == top ? id : INT32_MAX;
+        for (int s = 1; s < 64; s <<= 1) mi = min(mi, __shfl_xor(mi, s));
+        who = __builtin_amdgcn_ballot_w64(v == top && id == mi);
+      }
+      if (lane == __builtin_ctzll(who)) {
+        bv[r] = v, bi[r] = id;
+        ++at;
+        v = lane < parts && at < k ? lv[lane * k + at] : NEG_INF;
+        id = lane < parts && at < k ? li[lane * k + at] : (int)SCORE_NONE;
+      }
     }
-    const float mv = score_max(bv, sf);
-    const int mi = score_imin(bv == mv ? bi : INT32_MAX, si);
-    if (t == 0) {
-      top_ids[row * k + j] = mi == INT32_MAX ? 0xFFFFFFFFu : (uint32_t)mi;
-      top_lp[row * k + j] = bad ? __builtin_nanf("") : mi == INT32_MAX ? NEG_INF : (mv - m) - ls;
-    }
-    pv = mv, pi = mi;
   }
+  __syncthreads();
+  score_finish<E>(logits + row * ld, n, row, st, bv, bi, o);
 }
 
 #endif  // __HIPCC__

@@ -41,6 +41,10 @@ static int launched(const char *what) {
 static size_t cdiv(size_t a, size_t b) { return (a + b - 1) / b; }
 static bool aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
 
+// rows (times heads) of one call: a workgroup of 256 threads each stays below
+// the 2^32 threads a launch may have
+constexpr size_t MOST_ROWS = (size_t)1 << 23;
+
 static int elem_size(int dtype) { return dtype == RW_F32 ? 4 : dtype == RW_F16 || dtype == RW_BF16 ? 2 : 0; }
 
 // ------------------------------------------------------------- checks
@@ -113,7 +117,7 @@ static PagedView paged_view(const rw_kv_pages *p, size_t layer, const int32_t *t
 static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size_t max_len) {
   if (n_head < 1 || n_head % p->n_head)
     return fail(RW_EINVAL, "n_head %d is not a positive multiple of the pages' %d", n_head, p->n_head);
-  if (rows > ((size_t)INT32_MAX - 64) / n_head) return fail(RW_EINVAL, "%zu rows of %d heads", rows, n_head);
+  if (rows > MOST_ROWS / n_head) return fail(RW_EINVAL, "%zu rows of %d heads", rows, n_head);
   if (max_len > (size_t)INT32_MAX) return fail(RW_EINVAL, "max_len %zu", max_len);
   return RW_OK;
 }
@@ -210,6 +214,59 @@ struct CallWorkspace {
   }
 };
 
+// ------------------------------------------------------------- scores
+
+// Parts of a row of logits, one workgroup each.
+struct ScorePlan {
+  int parts;
+  int64_t part_len;
+  bool wide;  // 32 logits per lane and step, else 8
+  size_t off_v, off_i, bytes;
+};
+static ScorePlan score_plan(size_t rows, size_t n_vocab, size_t k) {
+  ScorePlan L{};
+  const size_t places = n_vocab + 7;  // a row may begin up to 7 elements past a 16-byte boundary
+  size_t parts = std::max((size_t)1, std::min({(size_t)1024 / rows, cdiv(places, 2048), (size_t)SCORE_MAX_PARTS}));
+  L.wide = places / parts > 4096;
+  const size_t step = L.wide ? 8192 : 2048;
+  L.part_len = (int64_t)(cdiv(places, parts * step) * step);
+  L.parts = (int)cdiv(places, (size_t)L.part_len);
+  if (L.parts > 1) {
+    const size_t n = rows * L.parts;
+    L.off_v = n * sizeof(ScorePart);
+    L.off_i = L.off_v + cdiv(n * k * 4, 16) * 16;
+    L.bytes = L.off_i + cdiv(n * k * 4, 16) * 16;
+  }
+  return L;
+}
+
+struct ScoreCall {
+  const void *logits;
+  int64_t ld;
+  int n;
+  size_t rows;
+  ScoreOut o;
+  char *ws;
+};
+
+template <class E>
+static int launch_score(const ScoreCall &c, const ScorePlan &L, hipStream_t s) {
+  const auto *x = (const typename E::T *)c.logits;
+  ScorePart *ps = (ScorePart *)c.ws;
+  float *pv = (float *)(c.ws + L.off_v);
+  int *pi = (int *)(c.ws + L.off_i);
+  constexpr int V = 16 / sizeof(typename E::T);
+  const dim3 grid((unsigned)(c.rows * L.parts));
+  if (L.wide)
+    hipLaunchKernelGGL((k_score<E, 32 / V>), grid, dim3(256), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
+  else
+    hipLaunchKernelGGL((k_score<E, 8 / V>), grid, dim3(256), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
+  SERVE_TRY(launched("k_score"));
+  if (L.parts == 1) return RW_OK;
+  hipLaunchKernelGGL((k_score_join<E>), dim3((unsigned)c.rows), dim3(256), 0, s, x, c.ld, c.n, L.parts, c.o, ps, pv, pi);
+  return launched("k_score_join");
+}
+
 // ----------------------------------------------------------------- book
 
 struct rw_kv_book {
@@ -250,7 +307,7 @@ int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k,
   SERVE_TRY(check_pages(pages));
   if (layer >= pages->n_layer) return fail(RW_EINVAL, "layer %zu of %zu", layer, pages->n_layer);
   if (rows == 0) return RW_OK;
-  if (rows > (size_t)INT32_MAX) return fail(RW_EINVAL, "rows = %zu", rows);
+  if (rows > MOST_ROWS) return fail(RW_EINVAL, "rows = %zu: at most %zu", rows, MOST_ROWS);
   const size_t n = (size_t)pages->n_head * pages->head_size;
   SERVE_TRY(check_rows(k, ldk, n, "k"));
   SERVE_TRY(check_rows(v, ldv, n, "v"));
@@ -420,7 +477,10 @@ int rw_rocm_kv_book_info(const rw_kv_book *b, size_t *free_pages, size_t *used_p
   return RW_OK;
 }
 
-size_t rw_rocm_token_logprobs_workspace_size(size_t rows, size_t n_vocab, size_t k) { return 0; }
+size_t rw_rocm_token_logprobs_workspace_size(size_t rows, size_t n_vocab, size_t k) {
+  if (rows == 0 || rows > MOST_ROWS || n_vocab == 0 || n_vocab > (size_t)INT32_MAX || k > (size_t)SCORE_TOP) return 0;
+  return score_plan(rows, n_vocab, k).bytes;
+}
 
 int rw_rocm_token_logprobs_dev(int dtype, const void *logits, size_t ld, size_t rows, size_t n_vocab,
                                const uint32_t *tokens, size_t n_tok, float *logprobs, float *entropy, size_t k,
@@ -429,7 +489,7 @@ int rw_rocm_token_logprobs_dev(int dtype, const void *logits, size_t ld, size_t 
   if (!elem_size(dtype)) return fail(RW_EINVAL, "unsupported dtype %d (RW_F32, RW_F16 or RW_BF16)", dtype);
   if (k > (size_t)SCORE_TOP) return fail(RW_EINVAL, "k = %zu: at most %d", k, SCORE_TOP);
   if (n_vocab < 1 || n_vocab > (size_t)INT32_MAX) return fail(RW_EINVAL, "n_vocab = %zu: between 1 and 2^31 - 1", n_vocab);
-  if (rows > (size_t)INT32_MAX || n_tok > (size_t)INT32_MAX) return fail(RW_EINVAL, "rows = %zu, n_tok = %zu", rows, n_tok);
+  if (rows > MOST_ROWS || n_tok > (size_t)INT32_MAX) return fail(RW_EINVAL, "rows = %zu, n_tok = %zu", rows, n_tok);
   if (rows == 0) return RW_OK;
   if (!logits || !aligned(logits, elem_size(dtype))) return fail(RW_EINVAL, "logits is NULL or not aligned");
   if (ld < n_vocab || ld > ((size_t)1 << 40)) return fail(RW_EINVAL, "logits: row stride %zu for rows of %zu", ld, n_vocab);
@@ -439,12 +499,18 @@ int rw_rocm_token_logprobs_dev(int dtype, const void *logits, size_t ld, size_t 
     return fail(RW_EINVAL, "tokens and results must be 4-byte aligned");
   int dev;
   SERVE_TRY(call_device(logits, "logits", &dev));
-#define RW_SCORE(E)                                                                                                  \
-  hipLaunchKernelGGL((k_score_row<E>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, (const E::T *)logits, \
-                     (int64_t)ld, (int)n_vocab, tokens, (int64_t)n_tok, logprobs, entropy, (int)k, top_ids, top_logprobs)
-  BY_TYPE(dtype, RW_SCORE);
-#undef RW_SCORE
-  return launched("k_score_row");
+  const ScorePlan L = score_plan(rows, n_vocab, k);
+  CallWorkspace hold;
+  void *ws = nullptr;
+  SERVE_TRY(hold.take(dev, workspace, workspace_len, L.bytes, stream, &ws));
+  const ScoreCall c{logits, (int64_t)ld, (int)n_vocab, rows,
+                    ScoreOut{tokens, logprobs, entropy, top_ids, top_logprobs, (int64_t)n_tok, (int)k}, (char *)ws};
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case RW_F32: return launch_score<F32>(c, L, s);
+    case RW_F16: return launch_score<F16>(c, L, s);
+    default: return launch_score<BF16>(c, L, s);
+  }
 }
 
 }  // extern "C"
