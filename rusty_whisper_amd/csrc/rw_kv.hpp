@@ -52,23 +52,58 @@ __device__ inline const int32_t *paged_row(const PagedView &w, int r) {
   return (unsigned)s < (unsigned)w.n_seqs ? w.table + (int64_t)s * w.ld : nullptr;
 }
 
-// One value of one row per thread: k and v rounded to the pool's type.
-template <class E>
+// R rows x KV_TILE / R values of k and of v per workgroup, 8 values of each per
+// thread.  k's go straight to their rows; v's cross through LDS, so that
+// neighbouring lanes have neighbouring rows, which are neighbours in a page
+// where the rows are a prompt's.
+constexpr int KV_TILE = 2048;
+template <class E, int R>
 __global__ __launch_bounds__(256) void k_kv_write(PagedView w, const float *__restrict__ k, int64_t ldk,
                                                   const float *__restrict__ v, int64_t ldv, int rows,
-                                                  const int32_t *__restrict__ pos) {
-  const int r = blockIdx.x, n = w.heads * w.dim, P = 1 << w.pr;
-  const int32_t *table = paged_row(w, r);
-  const int p = pos[r];
-  if (!table || p < 0 || (p >> w.pr) >= w.ld) return;
-  const int page = table[p >> w.pr], slot = p & (P - 1);
-  if ((unsigned)page >= (unsigned)w.n_pages) return;
-  const int64_t base = (int64_t)page * n << w.pr;
-  auto *pk = (typename E::T *)w.k + base, *pv = (typename E::T *)w.v + base;
-  for (int c = threadIdx.x; c < n; c += 256) {
+                                                  const int32_t *__restrict__ pos, int col_tiles) {
+  using T = typename E::T;
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  typedef T Out __attribute__((ext_vector_type(8)));
+  constexpr int C = KV_TILE / R, LD = R + 2;
+  __shared__ T sv[C][LD];
+  __shared__ int64_t page0[R];  // where the row's page begins, -1: no place
+  __shared__ int slot[R];
+  const int n = w.heads * w.dim, P = 1 << w.pr, t = threadIdx.x;
+  const int r0 = blockIdx.x / col_tiles * R, c0 = blockIdx.x % col_tiles * C;
+  if (t < R) {
+    int64_t at = -1;
+    if (r0 + t < rows) {
+      const int32_t *table = paged_row(w, r0 + t);
+      const int p = pos[r0 + t];
+      if (table && p >= 0 && (p >> w.pr) < w.ld) {
+        const int page = table[p >> w.pr];
+        if ((unsigned)page < (unsigned)w.n_pages) at = (int64_t)page * n << w.pr;
+        slot[t] = p & (P - 1);
+      }
+    }
+    page0[t] = at;
+  }
+  const int i = t / (C / 8), c = c0 + t % (C / 8) * 8;
+  const bool in = r0 + i < rows && c < n;
+  Out ok;
+  if (in) {
+    const float *a = k + (int64_t)(r0 + i) * ldk + c, *b = v + (int64_t)(r0 + i) * ldv + c;
+    const f4 a0 = *(const f4 *)a, a1 = *(const f4 *)(a + 4), b0 = *(const f4 *)b, b1 = *(const f4 *)(b + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ok[j] = E::round(j < 4 ? a0[j] : a1[j - 4]);
+      sv[c - c0 + j][i] = E::round(j < 4 ? b0[j] : b1[j - 4]);
+    }
+  }
+  __syncthreads();
+  if (in && page0[i] >= 0) {
     const int h = c / w.dim, d = c % w.dim;
-    pk[(((int64_t)h << w.pr) + slot) * w.dim + d] = E::round(k[r * ldk + c]);
-    pv[((int64_t)c << w.pr) + slot] = E::round(v[r * ldv + c]);
+    *(Out *)((T *)w.k + page0[i] + (((int64_t)h << w.pr) + slot[i]) * w.dim + d) = ok;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int e = j * 256 + t, row = e % R, col = e / R;
+    if (c0 + col < n && page0[row] >= 0) ((T *)w.v)[page0[row] + ((int64_t)(c0 + col) << w.pr) + slot[row]] = sv[col][row];
   }
 }
 

@@ -11,14 +11,14 @@
 // maxima scale S and T); lanes, wavefronts and parts are joined at the end in
 // a fixed order.
 //
-// The alternatives.  A wavefront keeps its k best so far and `thr`, the k-th's
-// logit.  Ids rise with the steps, so a later logit enters only if it is
-// larger than thr, and most steps end with one comparison of the lanes'
-// maxima.  Where at least k lanes' maxima pass thr, the k-th largest of them
-// bounds the k-th best from below: only logits from there on are candidates
-// (on rows in no special order little more than k).  Candidates are collected
-// in the order of their ids behind the k best, and each one's rank is the
-// number of entries before it (larger, or equal with a smaller id).
+// The alternatives.  A wavefront keeps its k best so far; a later logit, whose
+// id is larger, enters only if it is larger than the k-th of them, and most
+// steps end with one comparison of the lanes' maxima.  Where many lanes'
+// maxima pass, k of the maxima bound the k-th best from below (the smallest
+// of at least k groups' largest; for k > 16 the k-th largest itself), so that
+// on rows in no special order a few dozen candidates are left.  They are
+// collected behind the k best, and each one's rank is the number of entries
+// before it (larger, or equal with a smaller id).
 #pragma once
 #include "rw_kv.hpp"
 
@@ -26,6 +26,7 @@ namespace rw {
 
 constexpr int SCORE_TOP = 32;         // alternatives per row at most
 constexpr int SCORE_MAX_PARTS = 64;   // parts of a row: a lane each in k_score_join
+constexpr int SCORE_LINE = 128;       // bytes that the loads of a step are aligned to
 constexpr uint32_t SCORE_NONE = 0xFFFFFFFFu;
 
 #if defined(__HIPCC__)
@@ -77,6 +78,50 @@ __device__ inline float score_wave_max(float v) {
 }
 __device__ inline float score_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
+__device__ inline float score_wave_sum(float v) {
+  auto add = [&](int ctrl_value) __attribute__((always_inline)) { v += __int_as_float(ctrl_value); };
+  // (lanes without a source add 0)
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x111, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x112, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x114, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x118, 0xf, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x142, 0xa, 0xf, false));
+  add(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x143, 0xc, 0xf, false));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+// the lanes' sums of a wavefront
+__device__ inline ScoreStats score_wave_join(const ScoreStats &st) {
+  const ScoreStats a = score_join(st, ScoreStats{score_wave_max(st.m), 0.0f, 0.0f});
+  return ScoreStats{a.m, score_wave_sum(a.s), score_wave_sum(a.t)};
+}
+
+// A lower bound of the k-th largest of the wavefront's values: the largest of
+// each group of 64 / 2^ceil(log2 k) lanes, the smallest of those (k <= 16).
+template <int CTRL>
+__device__ inline float score_dpp_all(float v) {  // every lane has a source
+  const int i = __float_as_int(v);
+  return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+}
+__device__ inline float score_bound(float v, int k) {
+  float w = fmaxf(v, score_dpp_all<0xB1>(v));  // pairs
+  w = fmaxf(w, score_dpp_all<0x4E>(w));        // fours
+  float o = score_dpp_all<0x141>(w);           // mirrored within 8
+  w = k <= 8 ? fmaxf(w, o) : fminf(w, o);
+  o = score_dpp_all<0x140>(w);                 // mirrored within 16
+  w = k <= 4 ? fmaxf(w, o) : fminf(w, o);
+  float r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = score_lane(w, 16 * i);
+  if (k <= 1) return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+  if (k <= 2) return fminf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+  return fminf(fminf(r[0], r[1]), fminf(r[2], r[3]));
+}
+// the smallest value above x (x = +inf: NaN, which nothing reaches)
+__device__ inline float score_next(float x) {
+  const int b = __float_as_int(x + 0.0f);
+  return x == 0.0f ? __int_as_float(1) : __int_as_float(b + (b < 0 ? -1 : 1));
+}
+
 // LDS that one wavefront's lanes write and read: its operations keep their order
 __device__ inline void score_wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -101,7 +146,7 @@ __device__ inline void score_finish(const typename E::T *x, int n, int64_t row, 
     o.top_ids[row * o.k + threadIdx.x] = bad ? SCORE_NONE : (uint32_t)id;
     o.top_lp[row * o.k + threadIdx.x] = bad ? nan : id == (int)SCORE_NONE ? -__builtin_huge_valf() : (bv[threadIdx.x] - st.m) - ls;
   }
-  for (int64_t i = threadIdx.x; i < o.n_tok; i += 256) {
+  for (int64_t i = threadIdx.x; i < o.n_tok; i += blockDim.x) {
     const uint32_t id = o.tokens[row * o.n_tok + i];
     float lp = nan;
     if (id == SCORE_NONE) lp = 0.0f;
@@ -110,90 +155,120 @@ __device__ inline void score_finish(const typename E::T *x, int n, int64_t row, 
   }
 }
 
-// NJ: 16-byte loads per lane and step.  blockIdx.x = row * parts + part.
-template <class E, int NJ>
-__global__ __launch_bounds__(256) void k_score(const typename E::T *__restrict__ logits, int64_t ld, int n, int parts,
+// NJ: 16-byte loads per lane and step; NW: wavefronts.  blockIdx.x = row * parts + part.
+template <class E, int NJ, int NW>
+__global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restrict__ logits, int64_t ld, int n, int parts,
                                                int64_t part_len, ScoreOut o, ScorePart *__restrict__ ps,
                                                float *__restrict__ pv, int *__restrict__ pi) {
   using T = typename E::T;
   constexpr float NEG_INF = -__builtin_huge_valf();
-  constexpr int V = 16 / sizeof(T), PER = NJ * V, CAP = SCORE_TOP + 64 * V;
+  constexpr int V = 16 / sizeof(T), PER = NJ * V, CAP = SCORE_TOP + 64 + 64 * V;
   typedef T Vec __attribute__((ext_vector_type(V)));
-  __shared__ float ev[4][CAP];  // per wavefront: its k best, then candidates
-  __shared__ int ei[4][CAP];
-  __shared__ ScoreStats ss[4];
+  __shared__ float ev[NW][CAP];  // per wavefront
+  __shared__ int ei[NW][CAP];
+  __shared__ ScoreStats ss[NW];
   __shared__ float bv[SCORE_TOP];
-  __shared__ int bi[SCORE_TOP], en[4];
+  __shared__ int bi[SCORE_TOP];
   const int64_t row = blockIdx.x / parts;
   const int pt = blockIdx.x % parts, k = o.k;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T *x = logits + row * ld;
-  // places count from the 16-byte boundary at or before the row's start
-  const int skip = (int)(((uintptr_t)x & 15) / sizeof(T));
+  // places count from the cache line in which the row starts
+  const int skip = (int)(((uintptr_t)x & (SCORE_LINE - 1)) / sizeof(T));
   const int64_t u1 = min((int64_t)n + skip, (int64_t)(pt + 1) * part_len);
 
   ScoreStats st{NEG_INF, 0.0f, 0.0f};
-  float thr = NEG_INF;
-  int cnt = 0;  // entries of ev / ei
-  float *wv_v = ev[wv];
+  float lo = score_next(NEG_INF);  // the smallest logit that may enter
+  int best = 0;                    // entries of the k best; lane r holds the r-th
+  float lv = NEG_INF;
+  int li = (int)SCORE_NONE;
+  float *wv_v = ev[wv];            // candidates
   int *wv_i = ei[wv];
+  int cnt = 0;
 
-  // the k first of the cnt entries to the front, in order
+  // the candidates into the k best
   auto keep = [&]() __attribute__((always_inline)) {
     score_wave_sync();
-    if (cnt <= 64) {
+    if (best == k && cnt <= k + 2) {
+      // few: each is put in its place (15 instructions; ranking takes 9 for each of best + cnt)
       const float v = lane < cnt ? wv_v[lane] : NEG_INF;
-      const int id = lane < cnt ? wv_i[lane] : INT32_MAX;
-      int rank = lane < cnt ? 0 : 64;
-      for (int e = 0; e < cnt; ++e)
-        rank += score_before(score_lane(v, e), __builtin_amdgcn_readlane(id, e), v, id);
-      score_wave_sync();
-      if (rank < k) wv_v[rank] = v, wv_i[rank] = id;
-    } else {
-      // many equal logits: k rounds, each entry looked at by one lane
-      float pv0 = __builtin_huge_valf();
-      int pi0 = -1;
-      float kv = NEG_INF;
-      int ki = INT32_MAX;
-      for (int r = 0; r < k; ++r) {
-        float v = NEG_INF;
-        int id = INT32_MAX;
-        for (int e = lane; e < cnt; e += 64)
-          if (score_before(pv0, pi0, wv_v[e], wv_i[e]) && score_before(wv_v[e], wv_i[e], v, id)) v = wv_v[e], id = wv_i[e];
-        pv0 = score_wave_max(v);
-        int mi = v == pv0 ? id : INT32_MAX;
-        for (int s = 1; s < 64; s <<= 1) mi = min(mi, __shfl_xor(mi, s));
-        pi0 = mi;
-        if (lane == r) kv = pv0, ki = pi0;
+      const int id = lane < cnt ? wv_i[lane] : 0;
+      for (int e = 0; e < cnt; ++e) {
+        const float cv = score_lane(v, e);
+        const int ci = __builtin_amdgcn_readlane(id, e);
+        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < k && score_before(lv, li, cv, ci)));
+        const float up = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(lv), 0x138, 0xf, 0xf, false));  // from lane - 1
+        const int upi = __builtin_amdgcn_update_dpp(0, li, 0x138, 0xf, 0xf, false);
+        lv = lane < at ? lv : lane == at ? cv : up;
+        li = lane < at ? li : lane == at ? ci : upi;
       }
+    } else {
+      // behind the k best (there is room for k entries in front), then ranked
+      if (lane < best) wv_v[cnt + lane] = lv, wv_i[cnt + lane] = li;
+      cnt += best;
       score_wave_sync();
-      if (lane < k) wv_v[lane] = kv, wv_i[lane] = ki;
+      if (cnt <= 64) {
+        const float v = lane < cnt ? wv_v[lane] : NEG_INF;
+        const int id = lane < cnt ? wv_i[lane] : INT32_MAX;
+        int rank = lane < cnt ? 0 : 64;
+        for (int e = 0; e < cnt; ++e) rank += score_before(score_lane(v, e), __builtin_amdgcn_readlane(id, e), v, id);
+        score_wave_sync();
+        if (rank < k) wv_v[rank] = v, wv_i[rank] = id;
+        score_wave_sync();
+        best = min(cnt, k);
+        lv = lane < best ? wv_v[lane] : NEG_INF;
+        li = lane < best ? wv_i[lane] : (int)SCORE_NONE;
+      } else {
+        // many equal logits: k rounds, each entry looked at by one lane
+        float pv0 = __builtin_huge_valf();
+        int pi0 = -1;
+        float kv = NEG_INF;
+        int ki = (int)SCORE_NONE;
+        for (int r = 0; r < k; ++r) {
+          float v = NEG_INF;
+          int id = INT32_MAX;
+          for (int e = lane; e < cnt; e += 64)
+            if (score_before(pv0, pi0, wv_v[e], wv_i[e]) && score_before(wv_v[e], wv_i[e], v, id)) v = wv_v[e], id = wv_i[e];
+          pv0 = score_wave_max(v);
+          int mi = v == pv0 ? id : INT32_MAX;
+          for (int s = 1; s < 64; s <<= 1) mi = min(mi, __shfl_xor(mi, s));
+          pi0 = mi;
+          if (lane == r) kv = pv0, ki = pi0;
+        }
+        best = k;  // cnt > 64 >= k
+        lv = kv, li = ki;
+      }
     }
-    cnt = min(cnt, k);
+    cnt = 0;
     score_wave_sync();
-    if (cnt == k) thr = wv_v[k - 1];
+    if (best == k) lo = score_next(score_lane(lv, k - 1));
   };
 
-  for (int64_t u = (int64_t)pt * part_len + wv * 64 * PER; u < u1; u += 256 * PER) {
-    // e0: this lane's first id of the step (its j-th load has ids e0 + 64 V j .. + V - 1)
+  // the step at place u: this lane's j-th load has the ids u - skip + (64 j + lane) V ..
+  auto load = [&](int64_t u, Vec(&q)[NJ]) __attribute__((always_inline)) {
     const int64_t w0 = u - skip, e0 = w0 + lane * V;
-    float y[PER];
     if (w0 >= 0 && w0 + 64 * PER <= n) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const Vec q = *(const Vec *)(x + e0 + 64 * V * j);
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[j * V + i] = (float)q[i];
-      }
+      for (int j = 0; j < NJ; ++j) q[j] = *(const Vec *)(x + e0 + 64 * V * j);
     } else {  // a step that the row does not fill
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int64_t e = e0 + 64 * V * j + i;
-          y[j * V + i] = e >= 0 && e < n ? E::load(x + e) : NEG_INF;
+          q[j][i] = e >= 0 && e < n ? x[e] : (T)NEG_INF;
         }
     }
+  };
+  Vec ahead[NJ];  // the next step, on its way while this one is worked on
+  int64_t u = (int64_t)pt * part_len + wv * 64 * PER;
+  if (u < u1) load(u, ahead);
+  for (; u < u1; u += 64 * NW * PER) {
+    const int64_t e0 = u - skip + lane * V;
+    float y[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) y[j] = (float)ahead[j / V][j % V];
+    if (u + 64 * NW * PER < u1) load(u + 64 * NW * PER, ahead);
     float mx = y[0];
 #pragma unroll
     for (int j = 1; j < PER; ++j) mx = fmaxf(mx, y[j]);
@@ -211,76 +286,71 @@ __global__ __launch_bounds__(256) void k_score(const typename E::T *__restrict__
       st.s += s, st.t += t;
     }
     if (k == 0) continue;
-    const uint64_t pass = __builtin_amdgcn_ballot_w64(mx > thr);
+    const uint64_t pass = __builtin_amdgcn_ballot_w64(mx >= lo);
     if (!pass) continue;
-    float low = NEG_INF;  // candidates are >= low
-    if (__builtin_popcountll(pass) >= k) {
-      int rank = 0;
+    float least = lo;
+    if (__builtin_popcountll(pass) > max(k, 8)) {
+      if (k <= 16) {
+        least = fmaxf(lo, score_bound(mx, k));
+      } else {
+        int rank = 0;
 #pragma unroll 8
-      for (int e = 0; e < 64; ++e) {
-        const float w = score_lane(mx, e);
-        rank += w > mx || (w == mx && e < lane);
+        for (int e = 0; e < 64; ++e) {
+          const float w = score_lane(mx, e);
+          rank += w > mx || (w == mx && e < lane);
+        }
+        const uint64_t kth = __builtin_amdgcn_ballot_w64(rank == k - 1 && mx == mx);
+        if (kth) least = fmaxf(lo, score_lane(mx, __builtin_ctzll(kth)));
       }
-      low = score_lane(mx, __builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == k - 1)));
     }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      int c = 0;
+      float mj = y[j * V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) c += y[j * V + i] > thr && y[j * V + i] >= low;
-      if (!__builtin_amdgcn_ballot_w64(c > 0)) continue;
-      int before = c;
-#pragma unroll
-      for (int s = 1; s < 64; s <<= 1) {
-        const int w = __shfl_up(before, s);
-        if (lane >= s) before += w;
+      for (int i = 1; i < V; ++i) mj = fmaxf(mj, y[j * V + i]);
+      if (!__builtin_amdgcn_ballot_w64(mj >= least)) continue;
+      if (cnt > CAP - 64 * V - SCORE_TOP) {  // equal logits in great number
+        keep();
+        least = fmaxf(least, lo);
       }
-      const int total = __builtin_amdgcn_readlane(before, 63);
-      if (cnt + total > CAP) {
-        keep();  // to k entries: total <= 64 V fits behind them
-        c = 0;   // thr has risen
 #pragma unroll
-        for (int i = 0; i < V; ++i) c += y[j * V + i] > thr && y[j * V + i] >= low;
-        before = c;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-          const int w = __shfl_up(before, s);
-          if (lane >= s) before += w;
+      for (int i = 0; i < V; ++i) {
+        const uint64_t in = __builtin_amdgcn_ballot_w64(y[j * V + i] >= least);
+        if (!in) continue;
+        if (y[j * V + i] >= least) {
+          const int at = cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+          wv_v[at] = y[j * V + i], wv_i[at] = (int)(e0 + 64 * V * j + i);
         }
+        cnt += __builtin_popcountll(in);
       }
-      int at = cnt + before - c;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (y[j * V + i] > thr && y[j * V + i] >= low) wv_v[at] = y[j * V + i], wv_i[at] = (int)(e0 + 64 * V * j + i), ++at;
-      cnt += __builtin_amdgcn_readlane(before, 63);
     }
-    if (cnt > k || thr == NEG_INF) keep();
+    if (cnt) keep();
   }
 
   // lanes, then wavefronts
+  st = score_wave_join(st);
+  if (NW == 1) {
+    if (lane < SCORE_TOP) bv[lane] = lv, bi[lane] = li;
+    score_wave_sync();
+  } else {
+    if (threadIdx.x < SCORE_TOP) bv[threadIdx.x] = NEG_INF, bi[threadIdx.x] = (int)SCORE_NONE;
+    if (lane == 0) ss[wv] = st;
+    if (lane < SCORE_TOP) ev[wv][lane] = lv, ei[wv][lane] = li;
+    __syncthreads();
+    st = score_join(ss[0], ss[NW - 1]);
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const ScoreStats w{__shfl_xor(st.m, s), __shfl_xor(st.s, s), __shfl_xor(st.t, s)};
-    st = score_join(st, w);
-  }
-  if (lane == 0) ss[wv] = st, en[wv] = cnt;
-  if (threadIdx.x < SCORE_TOP) bv[threadIdx.x] = NEG_INF, bi[threadIdx.x] = (int)SCORE_NONE;
-  __syncthreads();
-  st = score_join(score_join(ss[0], ss[1]), score_join(ss[2], ss[3]));
-  if ((int)threadIdx.x < 4 * k) {
-    const int a = threadIdx.x / k, b = threadIdx.x % k;
-    if (b < en[a]) {
-      const float v = ev[a][b];
-      const int id = ei[a][b];
-      int rank = b;
+    for (int c = 1; c < NW - 1; ++c) st = score_join(st, ss[c]);
+    if (lane < k) {
+      int rank = lane;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c != a)
-          for (int e = 0; e < en[c]; ++e) rank += score_before(ev[c][e], ei[c][e], v, id);
-      if (rank < k) bv[rank] = v, bi[rank] = id;
+      for (int c = 0; c < NW; ++c)
+        if (c != wv)
+#pragma unroll 8
+          for (int e = 0; e < k; ++e) rank += score_before(ev[c][e], ei[c][e], lv, li);
+      if (li != (int)SCORE_NONE && rank < k) bv[rank] = lv, bi[rank] = li;
     }
+    __syncthreads();
   }
-  __syncthreads();
   if (parts == 1) {
     score_finish<E>(x, n, row, st, bv, bi, o);
   } else {
@@ -309,11 +379,7 @@ __global__ __launch_bounds__(256) void k_score_join(const typename E::T *__restr
     const ScorePart p = ps[row * parts + lane];
     st = ScoreStats{p.m, p.s, p.t};
   }
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const ScoreStats w{__shfl_xor(st.m, s), __shfl_xor(st.s, s), __shfl_xor(st.t, s)};
-    st = score_join(st, w);
-  }
+  st = score_wave_join(st);
   __syncthreads();
   if (threadIdx.x < 64 && k) {
     int at = 0;

@@ -220,15 +220,15 @@ struct CallWorkspace {
 struct ScorePlan {
   int parts;
   int64_t part_len;
-  bool wide;  // 32 logits per lane and step, else 8
+  bool wide;  // two wavefronts per part, else one
   size_t off_v, off_i, bytes;
 };
 static ScorePlan score_plan(size_t rows, size_t n_vocab, size_t k) {
   ScorePlan L{};
-  const size_t places = n_vocab + 7;  // a row may begin up to 7 elements past a 16-byte boundary
-  size_t parts = std::max((size_t)1, std::min({(size_t)1024 / rows, cdiv(places, 2048), (size_t)SCORE_MAX_PARTS}));
+  const size_t places = n_vocab + SCORE_LINE / 2 - 1;  // a row may begin anywhere in its first cache line
+  const size_t parts = std::max((size_t)1, std::min({(size_t)2048 / rows, cdiv(places, 1024), (size_t)SCORE_MAX_PARTS}));
   L.wide = places / parts > 4096;
-  const size_t step = L.wide ? 8192 : 2048;
+  const size_t step = L.wide ? 4096 : 1024;
   L.part_len = (int64_t)(cdiv(places, parts * step) * step);
   L.parts = (int)cdiv(places, (size_t)L.part_len);
   if (L.parts > 1) {
@@ -258,9 +258,9 @@ static int launch_score(const ScoreCall &c, const ScorePlan &L, hipStream_t s) {
   constexpr int V = 16 / sizeof(typename E::T);
   const dim3 grid((unsigned)(c.rows * L.parts));
   if (L.wide)
-    hipLaunchKernelGGL((k_score<E, 32 / V>), grid, dim3(256), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
+    hipLaunchKernelGGL((k_score<E, 4, 2>), grid, dim3(128), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
   else
-    hipLaunchKernelGGL((k_score<E, 8 / V>), grid, dim3(256), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
+    hipLaunchKernelGGL((k_score<E, 16 / V, 1>), grid, dim3(64), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
   SERVE_TRY(launched("k_score"));
   if (L.parts == 1) return RW_OK;
   hipLaunchKernelGGL((k_score_join<E>), dim3((unsigned)c.rows), dim3(256), 0, s, x, c.ld, c.n, L.parts, c.o, ps, pv, pi);
@@ -315,9 +315,19 @@ int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k,
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
   const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
-#define RW_WRITE(E)                                                                                              \
-  hipLaunchKernelGGL((k_kv_write<E>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v, \
-                     (int64_t)ldv, (int)rows, pos)
+  // few rows go to places of their own and want workgroups; many rows fill pages
+  const bool many = rows > 256;
+  const int r = many ? 64 : 8;
+  const unsigned row_tiles = (unsigned)cdiv(rows, r), col_tiles = (unsigned)cdiv(n, KV_TILE / r);
+#define RW_WRITE(E)                                                                                                    \
+  do {                                                                                                                 \
+    if (many)                                                                                                          \
+      hipLaunchKernelGGL((k_kv_write<E, 64>), dim3(row_tiles * col_tiles), dim3(256), 0, (hipStream_t)stream, w, k,    \
+                         (int64_t)ldk, v, (int64_t)ldv, (int)rows, pos, (int)col_tiles);                               \
+    else                                                                                                               \
+      hipLaunchKernelGGL((k_kv_write<E, 8>), dim3(row_tiles * col_tiles), dim3(256), 0, (hipStream_t)stream, w, k,     \
+                         (int64_t)ldk, v, (int64_t)ldv, (int)rows, pos, (int)col_tiles);                               \
+  } while (0)
   BY_TYPE(pages->dtype, RW_WRITE);
 #undef RW_WRITE
   return launched("k_kv_write");
