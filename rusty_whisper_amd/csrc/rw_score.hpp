@@ -11,14 +11,14 @@
 // maxima scale S and T); lanes, wavefronts and parts are joined at the end in
 // a fixed order.
 //
-// The alternatives.  A wavefront keeps its k best so far; a later logit, whose
-// id is larger, enters only if it is larger than the k-th of them, and most
-// steps end with one comparison of the lanes' maxima.  Where many lanes'
-// maxima pass, k of the maxima bound the k-th best from below (the smallest
-// of at least k groups' largest; for k > 16 the k-th largest itself), so that
-// on rows in no special order a few dozen candidates are left.  They are
-// collected behind the k best, and each one's rank is the number of entries
-// before it (larger, or equal with a smaller id).
+// The alternatives.  A wavefront keeps its k best so far, one per lane; a later
+// logit, whose id is larger, enters only if it is larger than the k-th of them,
+// and most steps end with one comparison of the lanes' maxima.  Where many lanes'
+// maxima pass, a lower bound of their k-th largest is one of the k-th best, and
+// on rows in no special order little more than k logits reach it.  These are
+// collected in LDS; a few are put in place one by one, more of them ranked: an
+// entry's rank is the number of entries before it (larger, or equal with a
+// smaller id).
 #pragma once
 #include "rw_kv.hpp"
 
@@ -95,26 +95,37 @@ __device__ inline ScoreStats score_wave_join(const ScoreStats &st) {
   return ScoreStats{a.m, score_wave_sum(a.s), score_wave_sum(a.t)};
 }
 
-// A lower bound of the k-th largest of the wavefront's values: the largest of
-// each group of 64 / 2^ceil(log2 k) lanes, the smallest of those (k <= 16).
 template <int CTRL>
 __device__ inline float score_dpp_all(float v) {  // every lane has a source
   const int i = __float_as_int(v);
   return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
 }
+// A lower bound of the k-th largest of the wavefront's values (k <= 32), with
+// at most k + 3 of them from it on where six halvings get that far: from the
+// largest of each group of 64 / 2^ceil(log2 k) lanes, the smallest of those, up.
 __device__ inline float score_bound(float v, int k) {
   float w = fmaxf(v, score_dpp_all<0xB1>(v));  // pairs
-  w = fmaxf(w, score_dpp_all<0x4E>(w));        // fours
-  float o = score_dpp_all<0x141>(w);           // mirrored within 8
+  float o = score_dpp_all<0x4E>(w);            // fours
+  float top = fmaxf(w, o);
+  w = k <= 16 ? top : fminf(w, o);
+  o = score_dpp_all<0x141>(w);  // mirrored within 8
   w = k <= 8 ? fmaxf(w, o) : fminf(w, o);
-  o = score_dpp_all<0x140>(w);                 // mirrored within 16
+  o = score_dpp_all<0x140>(w);  // mirrored within 16
   w = k <= 4 ? fmaxf(w, o) : fminf(w, o);
   float r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = score_lane(w, 16 * i);
   if (k <= 1) return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
-  if (k <= 2) return fminf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
-  return fminf(fminf(r[0], r[1]), fminf(r[2], r[3]));
+  float low = k <= 2 ? fminf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) : fminf(fminf(r[0], r[1]), fminf(r[2], r[3]));
+  float high = score_wave_max(v);
+  for (int i = 0; i < 6; ++i) {
+    const float mid = 0.5f * low + 0.5f * high;
+    const int from = __builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= mid));
+    if (from >= k) low = mid;
+    else high = mid;
+    if (from >= k && from <= k + 3) break;
+  }
+  return low;
 }
 // the smallest value above x (x = +inf: NaN, which nothing reaches)
 __device__ inline float score_next(float x) {
@@ -289,20 +300,7 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
     const uint64_t pass = __builtin_amdgcn_ballot_w64(mx >= lo);
     if (!pass) continue;
     float least = lo;
-    if (__builtin_popcountll(pass) > max(k, 8)) {
-      if (k <= 16) {
-        least = fmaxf(lo, score_bound(mx, k));
-      } else {
-        int rank = 0;
-#pragma unroll 8
-        for (int e = 0; e < 64; ++e) {
-          const float w = score_lane(mx, e);
-          rank += w > mx || (w == mx && e < lane);
-        }
-        const uint64_t kth = __builtin_amdgcn_ballot_w64(rank == k - 1 && mx == mx);
-        if (kth) least = fmaxf(lo, score_lane(mx, __builtin_ctzll(kth)));
-      }
-    }
+    if (__builtin_popcountll(pass) > k + 3) least = fmaxf(lo, score_bound(mx, k));
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float mj = y[j * V];
