@@ -566,18 +566,21 @@ _TORCH_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": B
 _dtype_name = functools.lru_cache(None)(str)
 
 
-def _dense(a, dtype: str, what: str):
-    """_ptr of a device array, which as a tensor must be dense and of `dtype`."""
+def _dense(a, dtype: str, what: str, device: int | None):
+    """_ptr of a device array, which as a tensor must be dense, of `dtype` and
+    on the `device` of the call's first tensor (None: that was a pointer)."""
     try:
         p = a.data_ptr()
     except AttributeError:
         return _ptr(a)
     if _dtype_name(a.dtype) != dtype or not a.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor")
+    if device is not None and a.get_device() != device:
+        raise ValueError(f"{what} is on another device")
     return p
 
 
-def _rows(a, n: int, ld: int | None, what: str, dtypes=("torch.float32",)):
+def _rows(a, n: int, ld: int | None, what: str, device: int | None, dtypes=("torch.float32",)):
     """(pointer, row stride) of device rows of n values; a 2-D tensor, which
     may be a column block of wider rows, brings its stride."""
     try:
@@ -587,6 +590,8 @@ def _rows(a, n: int, ld: int | None, what: str, dtypes=("torch.float32",)):
     st, shape = a.stride(), a.shape
     if _dtype_name(a.dtype) not in dtypes or (st and st[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
+    if device is not None and a.get_device() != device:
+        raise ValueError(f"{what} is on another device")
     return p, ld or (st[0] if len(st) == 2 and shape[0] > 1 else n)
 
 
@@ -610,6 +615,9 @@ class KvPages:
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("k and v must be contiguous")
         self.k, self.v = k, v  # keeps the tensors alive
+        self.device = k.get_device()
+        if v.get_device() != self.device:
+            raise ValueError("k and v are on different devices")
         self.st = RwKvPages(dtype, H, D, P, L, N, k.data_ptr(), v.data_ptr())
 
     @property
@@ -618,20 +626,21 @@ class KvPages:
         return self.st.n_head * self.st.head_size
 
 
-def _table_args(table, seq):
+def _table_args(table, seq, device: int):
     """(table, ld_table, n_seqs, seq) of the device entries."""
     n_seqs, ld = table.shape
-    return _dense(table, "torch.int32", "table"), ld, n_seqs, _dense(seq, "torch.int32", "seq")
+    return _dense(table, "torch.int32", "table", device), ld, n_seqs, _dense(seq, "torch.int32", "seq", device)
 
 
 def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=None, ldk: int | None = None,
                  ldv: int | None = None, stream: int | None = None) -> None:
     """Device rows k[r], v[r] into row pos[r] of sequence seq[r] (None: r).
     table: device int32 [n_seqs, pages per sequence]; pos, seq: device int32."""
-    t, ld, n_seqs, s = _table_args(table, seq)
+    d = pages.device
+    t, ld, n_seqs, s = _table_args(table, seq, d)
     n = pages.n_values
-    check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, n, ldk, "k"), *_rows(v, n, ldv, "v"), rows, t, ld, n_seqs,
-                                     s, _dense(pos, "torch.int32", "pos"), stream))
+    check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, n, ldk, "k", d), *_rows(v, n, ldv, "v", d), rows, t, ld,
+                                     n_seqs, s, _dense(pos, "torch.int32", "pos", d), stream))
 
 
 def kv_copy_pages_dev(pages: KvPages, src, dst, stream: int | None = None) -> None:
@@ -653,11 +662,12 @@ def paged_attention_dev(pages: KvPages, layer: int, q, rows: int, n_head: int, t
     """out[r] = attention of the one token q[r] (n_head query heads) over the
     first lens[r] rows of sequence seq[r] (None: r).  table, lens and seq:
     device int32, as for kv_write_dev; max_len: the longest of lens, or more."""
-    t, ld, n_seqs, s = _table_args(table, seq)
+    d = pages.device
+    t, ld, n_seqs, s = _table_args(table, seq, d)
     n = n_head * pages.st.head_size
-    check(lib().rw_rocm_paged_attention_dev(pages.st, layer, *_rows(q, n, ldq, "q"), rows, n_head, t, ld, n_seqs, s,
-                                            _dense(lens, "torch.int32", "lens"), max_len, *_rows(out, n, ldo, "out"),
-                                            _ptr(workspace), workspace_len, stream))
+    check(lib().rw_rocm_paged_attention_dev(pages.st, layer, *_rows(q, n, ldq, "q", d), rows, n_head, t, ld, n_seqs, s,
+                                            _dense(lens, "torch.int32", "lens", d), max_len,
+                                            *_rows(out, n, ldo, "out", d), _ptr(workspace), workspace_len, stream))
 
 
 class KvBook:
@@ -741,10 +751,10 @@ class KvBook:
 
 # --------------------------------------------------------- token scores
 
-def _ids(a, what: str):
+def _ids(a, what: str, device: int | None):
     """_dense of 32-bit ids, signed or not."""
     unsigned = _dtype_name(getattr(a, "dtype", None)) == "torch.uint32"
-    return _dense(a, "torch.uint32" if unsigned else "torch.int32", what)
+    return _dense(a, "torch.uint32" if unsigned else "torch.int32", what, device)
 
 
 def token_logprobs_workspace_size(rows: int, n_vocab: int, k: int) -> int:
@@ -757,13 +767,16 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
     """Log-probs of tokens [rows, n_tok] (32-bit ids), the entropy and the k
     largest alternatives of every row of device logits; `dtype` is taken from a
     logits tensor (F32 for a pointer)."""
-    if dtype is None:
-        dtype = _TORCH_DTYPES.get(_dtype_name(logits.dtype), -1) if hasattr(logits, "data_ptr") else F32
+    d = None
+    if hasattr(logits, "data_ptr"):
+        d = logits.get_device()
+        if dtype is None:
+            dtype = _TORCH_DTYPES.get(_dtype_name(logits.dtype), -1)
     check(lib().rw_rocm_token_logprobs_dev(
-        dtype, *_rows(logits, n_vocab, ld, "logits", tuple(_TORCH_DTYPES)), rows, n_vocab, _ids(tokens, "tokens"), n_tok,
-        _dense(logprobs, "torch.float32", "logprobs"), _dense(entropy, "torch.float32", "entropy"), k,
-        _ids(top_ids, "top_ids"), _dense(top_logprobs, "torch.float32", "top_logprobs"), _ptr(workspace),
-        workspace_len, stream))
+        F32 if dtype is None else dtype, *_rows(logits, n_vocab, ld, "logits", d, tuple(_TORCH_DTYPES)), rows, n_vocab,
+        _ids(tokens, "tokens", d), n_tok, _dense(logprobs, "torch.float32", "logprobs", d),
+        _dense(entropy, "torch.float32", "entropy", d), k, _ids(top_ids, "top_ids", d),
+        _dense(top_logprobs, "torch.float32", "top_logprobs", d), _ptr(workspace), workspace_len, stream))
 
 
 MODEL_PARSE_ONLY = 1

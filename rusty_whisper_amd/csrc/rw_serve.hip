@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <new>
+#include <stdexcept>
 #include <vector>
 
 #include "rw_internal.hpp"

@@ -224,6 +224,109 @@ def test_workspace_stream_and_bounds():
             run(P, q, table, lens, 3000, workspace=ws, workspace_len=need - 1)
 
 
+def test_more_chunks_than_one_launch_keeps():
+    """A length whose chunks would be more than the most there are, beside a
+    short row of the same launch."""
+    page, dim, n = 256, 128, 200_000
+    n_pages = -(-n // page) + 1
+    P = A.KvPages(*pool("f32", 1, n_pages, 1, page, dim, seed=18))
+    table = tables([n, 5], page, n_pages, seed=18)
+    q = torch.randn(2, dim, device="cuda")
+    compare(run(P, q, table, [n, 5], n), P, q, table, [n, 5], sigma=1.0)
+
+
+def test_capacity_far_above_the_lengths():
+    """max_len as a graph's program gives it: the table's capacity."""
+    page, dim, heads, lens = 16, 64, 3, [0, 1, 500, 33]
+    P = A.KvPages(*pool("bf16", 1, 64, heads, page, dim, seed=19))
+    table = tables(lens, page, 64, seed=19, width=20_000)
+    q = torch.randn(4, heads * dim, device="cuda")
+    compare(run(P, q, table, lens, 20_000 * page), P, q, table, lens, sigma=1.0)
+
+
+def test_a_captured_call_brings_its_workspace():
+    page, dim, heads = 64, 64, 1
+    P = A.KvPages(*pool("f16", 1, 64, heads, page, dim, seed=20))
+    q, out = torch.randn(1, dim, device="cuda"), torch.empty(1, dim, device="cuda")
+    table, lens = i32(np.arange(64)[None]), i32([4096])
+    assert A.paged_attention_workspace_size(P, 1, 1, 4096) > 0
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out.zero_()
+        with pytest.raises(A.RwError, match="captured call needs a workspace"):
+            A.paged_attention_dev(P, 0, q, 1, 1, table, lens, 4096, out, stream=torch.cuda.current_stream().cuda_stream)
+
+
+def test_two_graphs_on_one_workspace_and_eager_calls_between():
+    page, dim, heads = 64, 64, 2
+    P = A.KvPages(*pool("f16", 1, 130, heads, page, dim, seed=21))
+    q = [torch.randn(2, heads * dim, device="cuda") for _ in range(2)]
+    out = [torch.empty_like(x) for x in q]
+    lens = [[4100, 9], [70, 3000]]
+    table = [tables(n, page, 130, seed=i, width=65) for i, n in enumerate(lens)]
+    dev = [(i32(t), i32(n)) for t, n in zip(table, lens)]
+    need = A.paged_attention_workspace_size(P, 2, heads, 65 * page)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    graphs = []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            A.paged_attention_dev(P, 0, q[i], 2, heads, dev[i][0], dev[i][1], 65 * page, out[i], workspace=ws,
+                                  workspace_len=need, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        for i in (0, 1, 1, 0):
+            q[i].normal_()
+            graphs[i].replay()
+            big = torch.randn(8, heads * dim, device="cuda")  # the library's own workspace grows meanwhile
+            run(P, big, np.repeat(table[0][:1], 8, 0), [4100] * 8, 4100)
+            torch.cuda.synchronize()
+            compare(out[i], P, q[i], table[i], lens[i], sigma=1.0)
+
+
+def test_threads_on_streams_of_their_own():
+    """Calls at once, each thread with its stream's own workspace."""
+    import threading
+
+    page, dim, heads, n = 64, 64, 2, 5000
+    P = A.KvPages(*pool("bf16", 1, 80, heads, page, dim, seed=22))
+    table = tables([n], page, 80, seed=22)
+    td, ld = i32(table), i32([n])
+    qs = [torch.randn(1, heads * dim, device="cuda") for _ in range(4)]
+    outs = [torch.empty_like(x) for x in qs]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(i):
+        try:
+            A.init(0)
+            s = torch.cuda.Stream()
+            for _ in range(50):
+                A.paged_attention_dev(P, 0, qs[i], 1, heads, td, ld, n, outs[i], stream=s.cuda_stream)
+            s.synchronize()
+        except Exception as e:  # reported by the main thread
+            errors.append(e)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in ts], [t.join() for t in ts]
+    assert not errors
+    for q, out in zip(qs, outs):
+        compare(out, P, q, table, [n], sigma=1.0)
+
+
+def test_tensors_elsewhere_are_refused():
+    P = A.KvPages(*pool("f32", 1, 2, 1, 16, 32, seed=23))
+    q, out, t, n = torch.zeros(1, 32, device="cuda"), torch.empty(1, 32, device="cuda"), i32([[0]]), i32([1])
+    for i in range(4):
+        args = [q, t, n, out]
+        args[i] = args[i].cpu()
+        with pytest.raises(ValueError, match="another device"):
+            A.paged_attention_dev(P, 0, args[0], 1, 1, args[1], args[2], 1, args[3])
+    with pytest.raises(ValueError, match="another device"):
+        A.kv_write_dev(P, 0, q.cpu(), q, 1, t, n)
+    with pytest.raises(ValueError, match="different devices"):
+        A.KvPages(P.k, P.v.cpu())
+
+
 def test_captured_and_replayed_with_other_contents():
     """Lengths, sequences and table change between replays; eager calls of the
     library run between them."""
@@ -257,7 +360,7 @@ def test_captured_and_replayed_with_other_contents():
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("heads,dim,page", [(1, 32, 16), (3, 64, 32), (2, 96, 256), (5, 128, 64)])
-@pytest.mark.parametrize("new,past", [(1, 0), (1, 31), (45, 9), (64, 64), (7, 250)])
+@pytest.mark.parametrize("new,past", [(1, 0), (1, 31), (45, 9), (64, 64), (7, 250), (86, 3), (101, 130)])
 def test_write(dtype, heads, dim, page, new, past):
     seqs, n = 3, heads * dim
     width = -(-(past + new) // page)

@@ -89,14 +89,31 @@ def test_sizes(dtype, n, k):
     check(logits, tokens, k, *score(logits, tokens, k))
 
 
-@pytest.mark.parametrize("rows", [1, 2, 5, 33, 448, 1500])
-@pytest.mark.parametrize("n,k", [(257, 5), (5003, 16), (51866, 5)])
+@pytest.mark.parametrize("rows,n,k", [(r, n, k) for r in (1, 2, 5, 33, 300) for n, k in ((257, 5), (5003, 16), (51866, 5))]
+                         + [(1500, 257, 5), (1500, 5003, 16), (2100, 3000, 32)])
 def test_rows(rows, n, k):
-    if rows * n > 448 * 51866:
-        pytest.skip("covered by fewer rows")
     logits = torch.randn(rows, n, device="cuda") * 2
     tokens = np.random.default_rng(rows).integers(0, n, (rows, 1))
     check(logits, tokens, k, *score(logits, tokens, k))
+
+
+def test_a_vocabulary_of_millions():
+    """More than 64 steps per part, 64 parts."""
+    n, k = 3_000_001, 32
+    logits = torch.randn(2, n, device="cuda") * 2
+    tokens = [[0, n - 1], [n // 2, n]]
+    check(logits, tokens, k, *score(logits, tokens, k))
+
+
+def test_a_captured_call_brings_its_workspace():
+    x = torch.randn(1, 51866, device="cuda")
+    t, lp = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.empty(1, 1, device="cuda")
+    assert A.token_logprobs_workspace_size(1, 51866, 0) > 0
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        lp.zero_()
+        with pytest.raises(A.RwError, match="captured call needs a workspace"):
+            A.token_logprobs_dev(x, 1, 51866, t, 1, lp, stream=torch.cuda.current_stream().cuda_stream)
 
 
 @pytest.mark.parametrize("n_tok", [0, 1, 2, 99, 1000])
