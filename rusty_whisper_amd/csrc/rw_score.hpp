@@ -100,14 +100,15 @@ __device__ inline float score_dpp_all(float v) {  // every lane has a source
   const int i = __float_as_int(v);
   return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
 }
-// A lower bound of the k-th largest of the wavefront's values (k <= 32), with
-// at most k + 3 of them from it on where six halvings get that far: from the
-// largest of each group of 64 / 2^ceil(log2 k) lanes, the smallest of those, up.
-__device__ inline float score_bound(float v, int k) {
+// A lower bound of the k-th largest of the wavefront's values, more than k of
+// which are at least `lo` (k <= 32): the smallest of at least k groups' largest
+// (groups of 64 / 2^ceil(log2 k) lanes), or of the values from lo on, moved up
+// by halving while k values lie above; the k-th largest itself where that stops
+// far below it (values of very unlike size, such as masks of the type's lowest).
+__device__ inline float score_bound(float v, int k, float lo) {
   float w = fmaxf(v, score_dpp_all<0xB1>(v));  // pairs
   float o = score_dpp_all<0x4E>(w);            // fours
-  float top = fmaxf(w, o);
-  w = k <= 16 ? top : fminf(w, o);
+  w = k <= 16 ? fmaxf(w, o) : fminf(w, o);
   o = score_dpp_all<0x141>(w);  // mirrored within 8
   w = k <= 8 ? fmaxf(w, o) : fminf(w, o);
   o = score_dpp_all<0x140>(w);  // mirrored within 16
@@ -117,15 +118,34 @@ __device__ inline float score_bound(float v, int k) {
   for (int i = 0; i < 4; ++i) r[i] = score_lane(w, 16 * i);
   if (k <= 1) return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
   float low = k <= 2 ? fminf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) : fminf(fminf(r[0], r[1]), fminf(r[2], r[3]));
+  if (!(low >= lo)) low = -score_wave_max(v >= lo ? -v : -__builtin_huge_valf());
   float high = score_wave_max(v);
-  for (int i = 0; i < 6; ++i) {
+  int from = 64;
+  for (int i = 0; i < 6 && from > k + 3; ++i) {
     const float mid = 0.5f * low + 0.5f * high;
-    const int from = __builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= mid));
-    if (from >= k) low = mid;
+    const int c = __builtin_popcountll(__builtin_amdgcn_ballot_w64(v >= mid));
+    if (c >= k) low = mid, from = c;
     else high = mid;
-    if (from >= k && from <= k + 3) break;
+  }
+  if (from > k + 16) {
+    const int lane = threadIdx.x & 63;
+    int rank = 0;
+#pragma unroll 8
+    for (int e = 0; e < 64; ++e) {
+      const float x = score_lane(v, e);
+      rank += x > v || (x == v && e < lane);
+    }
+    const uint64_t kth = __builtin_amdgcn_ballot_w64(rank == k - 1 && v == v);
+    if (kth) low = score_lane(v, __builtin_ctzll(kth));
   }
   return low;
+}
+// the smallest id among the lanes of `who` (at least one)
+__device__ inline int score_first_id(uint64_t who, int id) {
+  if (__builtin_popcountll(who) == 1) return __builtin_amdgcn_readlane(id, __builtin_ctzll(who));
+  int m = who >> (threadIdx.x & 63) & 1 ? id : INT32_MAX;
+  for (int s = 1; s < 64; s <<= 1) m = min(m, __shfl_xor(m, s));
+  return __builtin_amdgcn_readfirstlane(m);
 }
 // the smallest value above x (x = +inf: NaN, which nothing reaches)
 __device__ inline float score_next(float x) {
@@ -241,9 +261,7 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
           for (int e = lane; e < cnt; e += 64)
             if (score_before(pv0, pi0, wv_v[e], wv_i[e]) && score_before(wv_v[e], wv_i[e], v, id)) v = wv_v[e], id = wv_i[e];
           pv0 = score_wave_max(v);
-          int mi = v == pv0 ? id : INT32_MAX;
-          for (int s = 1; s < 64; s <<= 1) mi = min(mi, __shfl_xor(mi, s));
-          pi0 = mi;
+          pi0 = score_first_id(__builtin_amdgcn_ballot_w64(v == pv0), id);
           if (lane == r) kv = pv0, ki = pi0;
         }
         best = k;  // cnt > 64 >= k
@@ -300,7 +318,7 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
     const uint64_t pass = __builtin_amdgcn_ballot_w64(mx >= lo);
     if (!pass) continue;
     float least = lo;
-    if (__builtin_popcountll(pass) > k + 3) least = fmaxf(lo, score_bound(mx, k));
+    if (__builtin_popcountll(pass) > k + 3) least = fmaxf(lo, score_bound(mx, k, lo));
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float mj = y[j * V];
@@ -387,13 +405,8 @@ __global__ __launch_bounds__(256) void k_score_join(const typename E::T *__restr
       // (a list's rest holds -inf and NONE: it never wins against an entry, and
       // where no entry is left the winner's place gets just that)
       const float top = score_wave_max(v);
-      uint64_t who = __builtin_amdgcn_ballot_w64(v == top);
-      if (__builtin_popcountll(who) > 1) {
-        int mi = v == top ? id : INT32_MAX;
-        for (int s = 1; s < 64; s <<= 1) mi = min(mi, __shfl_xor(mi, s));
-        who = __builtin_amdgcn_ballot_w64(v == top && id == mi);
-      }
-      if (lane == __builtin_ctzll(who)) {
+      const int first = score_first_id(__builtin_amdgcn_ballot_w64(v == top), id);
+      if (lane == __builtin_ctzll(__builtin_amdgcn_ballot_w64(v == top && id == first))) {
         bv[r] = v, bi[r] = id;
         ++at;
         v = lane < parts && at < k ? lv[lane * k + at] : NEG_INF;

@@ -184,6 +184,20 @@ def test_suppressed_and_lowest(dtype, n):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("mask", ["-inf", "lowest"])
+@pytest.mark.parametrize("rows", [1, 600])
+def test_masks_that_leave_a_range(dtype, mask, rows):
+    """As after a rule on timestamps: a few hundred neighbouring ids are left."""
+    n, t = 51866, DTYPES[dtype]
+    x = torch.full((rows, n), -float("inf") if mask == "-inf" else torch.finfo(t).min, dtype=t, device="cuda")
+    at = torch.arange(rows, device="cuda") * 61 % (n - 700)
+    x.scatter_(1, at[:, None] + torch.arange(700, device="cuda"), torch.randn(rows, 700, device="cuda").to(t))
+    tokens = np.stack([at.cpu().numpy() + 3, np.zeros(rows, np.int64)], 1)
+    for k in (5, 32):
+        check(x, tokens, k, *score(x, tokens, k))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("n", [33, 4100, 51866])
 def test_rows_without_a_distribution(dtype, n):
     inf = float("inf")
