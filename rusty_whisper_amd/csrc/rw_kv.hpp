@@ -222,8 +222,8 @@ template <class E, int DH>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     const void *__restrict__ kp, const void *__restrict__ vp, const float *__restrict__ q, const int32_t *__restrict__ table,
     const int32_t *__restrict__ seq, const int32_t *__restrict__ lens, float *__restrict__ out, float *__restrict__ part,
-    int kv_heads, int group, int pr, int n_pages, int n_seqs, int64_t ld_table, int64_t ldq, int64_t ldo, int max_len,
-    int chunk) {
+    int rows, int kv_heads, int group, int pr, int n_pages, int n_seqs, int64_t ld_table, int64_t ldq, int64_t ldo,
+    int max_len, int chunk) {
   using M = PaTile<E>;
   using Op = typename M::Op;
   using T = typename E::T;
@@ -232,8 +232,12 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
   constexpr float NEG_INF = -__builtin_huge_valf();
   __shared__ float so[PA_WAVES][16][LD], sm[PA_WAVES][16], sl[PA_WAVES][16];
 
+  // (row, key/value head) items; the query tiles of one item run eight
+  // workgroups apart, on one XCD, whose L2 the second reads k and v from
   const int qtiles = (group + 15) / 16;
-  const int qi = blockIdx.x % qtiles, hk = blockIdx.x / qtiles % kv_heads, row = blockIdx.x / qtiles / kv_heads;
+  const int qi = blockIdx.x / 8 % qtiles, item = blockIdx.x / (8 * qtiles) * 8 + blockIdx.x % 8;
+  const int hk = item % kv_heads, row = item / kv_heads;
+  if (row >= rows) return;
   const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int gq = min(16, group - 16 * qi);  // query heads of this tile
   const int heads = kv_heads * group, hq = hk * group + 16 * qi;
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     for (int d = 0; d < ND; ++d) so[wv][qr][16 * d + r] = o[d][i] * f;
   }
   __syncthreads();
-  const int64_t runs = (int64_t)(gridDim.x / qtiles / kv_heads) * heads * gridDim.y;
+  const int64_t runs = (int64_t)rows * heads * gridDim.y;
   for (int i = threadIdx.x; i < gq * DH; i += 64 * PA_WAVES) {
     const int qr = i / DH, d = i % DH;
     float top = sm[0][qr], l = 0.0f, y = 0.0f;

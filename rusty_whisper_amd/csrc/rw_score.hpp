@@ -26,6 +26,7 @@ namespace rw {
 
 constexpr int SCORE_TOP = 32;         // alternatives per row at most
 constexpr int SCORE_MAX_PARTS = 64;   // parts of a row: a lane each in k_score_join
+constexpr int SCORE_HEADS = 8;        // alternatives up to which k_score_join compares heads
 constexpr int SCORE_LINE = 128;       // bytes that the loads of a step are aligned to
 constexpr uint32_t SCORE_NONE = 0xFFFFFFFFu;
 
@@ -162,6 +163,55 @@ __device__ inline void score_wave_sync() {
 // entry (v, i) comes before (w, j)
 __device__ inline bool score_before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
+// The k best entries of a wavefront: lane r < n holds the r-th, the others -inf
+// and NONE (which come before no entry).
+struct ScoreBest {
+  float v = -__builtin_huge_valf();
+  int id = (int)SCORE_NONE;
+  int n = 0;
+
+  // Takes in the entries (w, i) of lanes 0 .. c - 1 (the others: -inf); sv, si:
+  // k places of LDS.
+  __device__ inline void take(float w, int i, int c, int k, float *sv, int *si) {
+    const int lane = threadIdx.x & 63;
+    if (n == k && c <= 4 + k * 3 / 8) {
+      // few: each in its place, 15 instructions that wait for each other
+      for (int e = 0; e < c; ++e) {
+        const float cv = score_lane(w, e);
+        const int ci = __builtin_amdgcn_readlane(i, e);
+        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(score_before(v, id, cv, ci)));
+        // the entries from `at` on move up one lane (0x138: from lane - 1)
+        const float up = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x138, 0xf, 0xf, false));
+        const int upi = __builtin_amdgcn_update_dpp(0, id, 0x138, 0xf, 0xf, false);
+        v = lane < at ? v : lane == at ? cv : up;
+        id = lane < at ? id : lane == at ? ci : upi;
+        if (lane >= k) v = -__builtin_huge_valf(), id = (int)SCORE_NONE;
+      }
+      return;
+    }
+    // the old and the new ones are ranked together, eight at a time
+    int rank = 0, rold = lane;
+    for (int e = 0; e < n; e += 8)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rank += score_before(score_lane(v, e + j), __builtin_amdgcn_readlane(id, e + j), w, i);
+    for (int e = 0; e < c; e += 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rank += score_before(score_lane(w, e + j), __builtin_amdgcn_readlane(i, e + j), w, i);
+      if (n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rold += score_before(score_lane(w, e + j), __builtin_amdgcn_readlane(i, e + j), v, id);
+    }
+    score_wave_sync();
+    if (lane < c && rank < k) sv[rank] = w, si[rank] = i;
+    if (lane < n && rold < k) sv[rold] = v, si[rold] = id;
+    score_wave_sync();
+    n = min(k, n + c);
+    v = lane < n ? sv[lane] : -__builtin_huge_valf();
+    id = lane < n ? si[lane] : (int)SCORE_NONE;
+    score_wave_sync();
+  }
+};
+
 // log-probs, entropy and alternatives of a row from its sums and its k best
 // (LDS; id NONE where there are fewer), by one workgroup
 template <class E>
@@ -193,10 +243,10 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
                                                float *__restrict__ pv, int *__restrict__ pi) {
   using T = typename E::T;
   constexpr float NEG_INF = -__builtin_huge_valf();
-  constexpr int V = 16 / sizeof(T), PER = NJ * V, CAP = SCORE_TOP + 64 + 64 * V;
+  constexpr int V = 16 / sizeof(T), PER = NJ * V, CAP = 64 + 64 * V;
   typedef T Vec __attribute__((ext_vector_type(V)));
-  __shared__ float ev[NW][CAP];  // per wavefront
-  __shared__ int ei[NW][CAP];
+  __shared__ float ev[NW][CAP + SCORE_TOP];  // per wavefront
+  __shared__ int ei[NW][CAP + SCORE_TOP];
   __shared__ ScoreStats ss[NW];
   __shared__ float bv[SCORE_TOP];
   __shared__ int bi[SCORE_TOP];
@@ -210,67 +260,23 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
 
   ScoreStats st{NEG_INF, 0.0f, 0.0f};
   float lo = score_next(NEG_INF);  // the smallest logit that may enter
-  int best = 0;                    // entries of the k best; lane r holds the r-th
-  float lv = NEG_INF;
-  int li = (int)SCORE_NONE;
-  float *wv_v = ev[wv];            // candidates
-  int *wv_i = ei[wv];
+  ScoreBest best;
+  float *wv_v = ev[wv], *sv = ev[wv] + CAP;  // candidates; the places that `take` wants
+  int *wv_i = ei[wv], *si = ei[wv] + CAP;
   int cnt = 0;
 
-  // the candidates into the k best
   auto keep = [&]() __attribute__((always_inline)) {
     score_wave_sync();
-    if (best == k && cnt <= k + 2) {
-      // few: each is put in its place (15 instructions; ranking takes 9 for each of best + cnt)
-      const float v = lane < cnt ? wv_v[lane] : NEG_INF;
-      const int id = lane < cnt ? wv_i[lane] : 0;
-      for (int e = 0; e < cnt; ++e) {
-        const float cv = score_lane(v, e);
-        const int ci = __builtin_amdgcn_readlane(id, e);
-        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < k && score_before(lv, li, cv, ci)));
-        const float up = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(lv), 0x138, 0xf, 0xf, false));  // from lane - 1
-        const int upi = __builtin_amdgcn_update_dpp(0, li, 0x138, 0xf, 0xf, false);
-        lv = lane < at ? lv : lane == at ? cv : up;
-        li = lane < at ? li : lane == at ? ci : upi;
-      }
-    } else {
-      // behind the k best (there is room for k entries in front), then ranked
-      if (lane < best) wv_v[cnt + lane] = lv, wv_i[cnt + lane] = li;
-      cnt += best;
-      score_wave_sync();
-      if (cnt <= 64) {
-        const float v = lane < cnt ? wv_v[lane] : NEG_INF;
-        const int id = lane < cnt ? wv_i[lane] : INT32_MAX;
-        int rank = lane < cnt ? 0 : 64;
-        for (int e = 0; e < cnt; ++e) rank += score_before(score_lane(v, e), __builtin_amdgcn_readlane(id, e), v, id);
-        score_wave_sync();
-        if (rank < k) wv_v[rank] = v, wv_i[rank] = id;
-        score_wave_sync();
-        best = min(cnt, k);
-        lv = lane < best ? wv_v[lane] : NEG_INF;
-        li = lane < best ? wv_i[lane] : (int)SCORE_NONE;
-      } else {
-        // many equal logits: k rounds, each entry looked at by one lane
-        float pv0 = __builtin_huge_valf();
-        int pi0 = -1;
-        float kv = NEG_INF;
-        int ki = (int)SCORE_NONE;
-        for (int r = 0; r < k; ++r) {
-          float v = NEG_INF;
-          int id = INT32_MAX;
-          for (int e = lane; e < cnt; e += 64)
-            if (score_before(pv0, pi0, wv_v[e], wv_i[e]) && score_before(wv_v[e], wv_i[e], v, id)) v = wv_v[e], id = wv_i[e];
-          pv0 = score_wave_max(v);
-          pi0 = score_first_id(__builtin_amdgcn_ballot_w64(v == pv0), id);
-          if (lane == r) kv = pv0, ki = pi0;
-        }
-        best = k;  // cnt > 64 >= k
-        lv = kv, li = ki;
-      }
+    for (int at = 0; at < cnt; at += 64) {
+      const float v = at + lane < cnt ? wv_v[at + lane] : NEG_INF;
+      const int id = at + lane < cnt ? wv_i[at + lane] : INT32_MAX;
+      // (of many equal logits the first ones may leave none to take in)
+      if (best.n < k || __builtin_amdgcn_ballot_w64(score_before(v, id, score_lane(best.v, k - 1), __builtin_amdgcn_readlane(best.id, k - 1))))
+        best.take(v, id, min(64, cnt - at), k, sv, si);
     }
     cnt = 0;
     score_wave_sync();
-    if (best == k) lo = score_next(score_lane(lv, k - 1));
+    if (best.n == k) lo = score_next(score_lane(best.v, k - 1));
   };
 
   // the step at place u: this lane's j-th load has the ids u - skip + (64 j + lane) V ..
@@ -325,7 +331,7 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
 #pragma unroll
       for (int i = 1; i < V; ++i) mj = fmaxf(mj, y[j * V + i]);
       if (!__builtin_amdgcn_ballot_w64(mj >= least)) continue;
-      if (cnt > CAP - 64 * V - SCORE_TOP) {  // equal logits in great number
+      if (cnt > CAP - 64 * V) {  // equal logits in great number
         keep();
         least = fmaxf(least, lo);
       }
@@ -346,12 +352,12 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
   // lanes, then wavefronts
   st = score_wave_join(st);
   if (NW == 1) {
-    if (lane < SCORE_TOP) bv[lane] = lv, bi[lane] = li;
+    if (lane < SCORE_TOP) bv[lane] = best.v, bi[lane] = best.id;
     score_wave_sync();
   } else {
     if (threadIdx.x < SCORE_TOP) bv[threadIdx.x] = NEG_INF, bi[threadIdx.x] = (int)SCORE_NONE;
     if (lane == 0) ss[wv] = st;
-    if (lane < SCORE_TOP) ev[wv][lane] = lv, ei[wv][lane] = li;
+    if (lane < SCORE_TOP) ev[wv][lane] = best.v, ei[wv][lane] = best.id;
     __syncthreads();
     st = score_join(ss[0], ss[NW - 1]);
 #pragma unroll
@@ -362,8 +368,8 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
       for (int c = 0; c < NW; ++c)
         if (c != wv)
 #pragma unroll 8
-          for (int e = 0; e < k; ++e) rank += score_before(ev[c][e], ei[c][e], lv, li);
-      if (li != (int)SCORE_NONE && rank < k) bv[rank] = lv, bi[rank] = li;
+          for (int e = 0; e < k; ++e) rank += score_before(ev[c][e], ei[c][e], best.v, best.id);
+      if (lane < best.n && rank < k) bv[rank] = best.v, bi[rank] = best.id;
     }
     __syncthreads();
   }
@@ -378,18 +384,29 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
   }
 }
 
-// The parts of a row: sums in order, and the k best by taking the best head
-// of the parts' lists k times (a lane a list).
-template <class E>
+// The parts of a row: sums in order, and the k best of the parts' lists.
+// K = 1 (few alternatives): the best of the lists' heads, a lane a list, k
+// times.  Else by halving the number of lists: of two lists of K places, one
+// read backwards, the better entry of each place is one of the K best, and
+// log2 K exchanges put these in order again, 64 / K pairs of lists per
+// wavefront and turn.  (51 lists of 5: 3.5 us against 5.0; of 16: 6.3 and 6.4;
+// of 32: 11.0 and 9.9; 341 rows of 6 lists of 10: 5.1 and 4.2.)
+template <class E, int K>
 __global__ __launch_bounds__(256) void k_score_join(const typename E::T *__restrict__ logits, int64_t ld, int n, int parts,
                                                     ScoreOut o, const ScorePart *__restrict__ ps,
                                                     const float *__restrict__ pv, const int *__restrict__ pi) {
   constexpr float NEG_INF = -__builtin_huge_valf();
-  __shared__ float lv[SCORE_MAX_PARTS * SCORE_TOP], bv[SCORE_TOP];
-  __shared__ int li[SCORE_MAX_PARTS * SCORE_TOP], bi[SCORE_TOP];
+  constexpr int LIST = K == 1 ? SCORE_HEADS : K;
+  __shared__ float lv[SCORE_MAX_PARTS * LIST], bv[SCORE_HEADS];
+  __shared__ int li[SCORE_MAX_PARTS * LIST], bi[SCORE_HEADS];
   const int64_t row = blockIdx.x;
   const int k = o.k, lane = threadIdx.x & 63;
-  for (int e = threadIdx.x; e < parts * k; e += 256) lv[e] = pv[row * parts * k + e], li[e] = pi[row * parts * k + e];
+  for (int e = threadIdx.x; e < parts * LIST; e += 256) {
+    const int p = e / LIST, r = e % LIST;
+    const bool in = r < k;
+    lv[e] = in ? pv[(row * parts + p) * k + r] : NEG_INF;
+    li[e] = in ? pi[(row * parts + p) * k + r] : (int)SCORE_NONE;
+  }
   ScoreStats st{NEG_INF, 0.0f, 0.0f};
   if (lane < parts) {
     const ScorePart p = ps[row * parts + lane];
@@ -397,25 +414,52 @@ __global__ __launch_bounds__(256) void k_score_join(const typename E::T *__restr
   }
   st = score_wave_join(st);
   __syncthreads();
-  if (threadIdx.x < 64 && k) {
-    int at = 0;
-    float v = lane < parts ? lv[lane * k] : NEG_INF;
-    int id = lane < parts ? li[lane * k] : (int)SCORE_NONE;
-    for (int r = 0; r < k; ++r) {
-      // (a list's rest holds -inf and NONE: it never wins against an entry, and
-      // where no entry is left the winner's place gets just that)
-      const float top = score_wave_max(v);
-      const int first = score_first_id(__builtin_amdgcn_ballot_w64(v == top), id);
-      if (lane == __builtin_ctzll(__builtin_amdgcn_ballot_w64(v == top && id == first))) {
-        bv[r] = v, bi[r] = id;
-        ++at;
-        v = lane < parts && at < k ? lv[lane * k + at] : NEG_INF;
-        id = lane < parts && at < k ? li[lane * k + at] : (int)SCORE_NONE;
+  if (K == 1) {
+    if (threadIdx.x < 64 && k) {
+      int at = 0;
+      float v = lane < parts ? lv[lane * LIST] : NEG_INF;
+      int id = lane < parts ? li[lane * LIST] : (int)SCORE_NONE;
+      for (int r = 0; r < k; ++r) {
+        // (where no entry is left, all heads are -inf and NONE: one of them is written)
+        const float top = score_wave_max(v);
+        const int first = score_first_id(__builtin_amdgcn_ballot_w64(v == top), id);
+        if (lane == __builtin_ctzll(__builtin_amdgcn_ballot_w64(v == top && id == first))) {
+          bv[r] = v, bi[r] = id;
+          ++at;
+          v = lane < parts && at < k ? lv[lane * LIST + at] : NEG_INF;
+          id = lane < parts && at < k ? li[lane * LIST + at] : (int)SCORE_NONE;
+        }
       }
     }
+    __syncthreads();
+    score_finish<E>(logits + row * ld, n, row, st, bv, bi, o);
+    return;
   }
-  __syncthreads();
-  score_finish<E>(logits + row * ld, n, row, st, bv, bi, o);
+  // lists p and p + half become list p
+  for (int lists = parts; lists > 1; lists = (lists + 1) / 2) {
+    const int half = (lists + 1) / 2;
+    for (int p0 = 0; p0 < half; p0 += 256 / K) {
+      const int p = p0 + threadIdx.x / K, r = threadIdx.x % K;
+      float v = NEG_INF;
+      int id = (int)SCORE_NONE;
+      if (p + half < lists) {
+        v = lv[p * K + r], id = li[p * K + r];
+        const float w = lv[(p + half) * K + K - 1 - r];
+        const int i = li[(p + half) * K + K - 1 - r];
+        if (score_before(w, i, v, id)) v = w, id = i;
+#pragma unroll
+        for (int x = K / 2; x; x >>= 1) {
+          // the lower lane of a pair keeps the better one (lanes of one list take this branch together)
+          const float y = __shfl_xor(v, x);
+          const int j = __shfl_xor(id, x);
+          if (score_before(y, j, v, id) == !(r & x) && (y != v || j != id)) v = y, id = j;
+        }
+        lv[p * K + r] = v, li[p * K + r] = id;
+      }
+    }
+    __syncthreads();
+  }
+  score_finish<E>(logits + row * ld, n, row, st, lv, li, o);
 }
 
 #endif  // __HIPCC__

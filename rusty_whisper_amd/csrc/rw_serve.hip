@@ -168,9 +168,11 @@ struct PagedCall {
 template <class E, int DH>
 static int launch_paged(const PagedCall &c, const PagedPlan &L, hipStream_t s) {
   const PagedView &w = c.w;
-  hipLaunchKernelGGL((k_paged_attn<E, DH>), dim3((unsigned)L.base, (unsigned)L.nsplit), dim3(64 * PA_WAVES), 0, s, w.k,
-                     w.v, c.q, w.table, w.seq, c.len, c.out, c.part, w.heads, c.n_head / w.heads, w.pr, w.n_pages,
-                     w.n_seqs, w.ld, c.ldq, c.ldo, c.max_len, L.chunk);
+  const int group = c.n_head / w.heads;
+  const size_t items = (size_t)c.rows * w.heads;
+  const dim3 grid((unsigned)(cdiv(items, 8) * 8 * cdiv(group, 16)), (unsigned)L.nsplit);
+  hipLaunchKernelGGL((k_paged_attn<E, DH>), grid, dim3(64 * PA_WAVES), 0, s, w.k, w.v, c.q, w.table, w.seq, c.len, c.out,
+                     c.part, c.rows, w.heads, group, w.pr, w.n_pages, w.n_seqs, w.ld, c.ldq, c.ldo, c.max_len, L.chunk);
   SERVE_TRY(launched("k_paged_attn"));
   if (L.nsplit == 1) return RW_OK;
   hipLaunchKernelGGL((k_paged_join<DH>), dim3((unsigned)(c.rows * c.n_head)), dim3(256), 0, s, c.part, w.seq, c.len,
@@ -264,7 +266,12 @@ static int launch_score(const ScoreCall &c, const ScorePlan &L, hipStream_t s) {
     hipLaunchKernelGGL((k_score<E, 16 / V, 1>), grid, dim3(64), 0, s, x, c.ld, c.n, L.parts, L.part_len, c.o, ps, pv, pi);
   SERVE_TRY(launched("k_score"));
   if (L.parts == 1) return RW_OK;
-  hipLaunchKernelGGL((k_score_join<E>), dim3((unsigned)c.rows), dim3(256), 0, s, x, c.ld, c.n, L.parts, c.o, ps, pv, pi);
+#define RW_JOIN(K)                                                                                                   \
+  hipLaunchKernelGGL((k_score_join<E, K>), dim3((unsigned)c.rows), dim3(256), 0, s, x, c.ld, c.n, L.parts, c.o, ps, pv, pi)
+  if (c.o.k <= SCORE_HEADS) RW_JOIN(1);
+  else if (c.o.k <= 16) RW_JOIN(16);
+  else RW_JOIN(32);
+#undef RW_JOIN
   return launched("k_score_join");
 }
 
