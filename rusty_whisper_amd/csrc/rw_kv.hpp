@@ -126,7 +126,8 @@ struct KvPairs {
 };
 
 // 16-byte pieces of page id[y], layer z / 2 of k (z even) or v; a page has
-// `piece` of them per layer.
+// `piece` of them per layer.  700 pages of 1.57 MB over 24 layers: 430 us, 5.1
+// TB/s read and written, a large copy's rate.
 __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t piece, int64_t n_pages, KvPairs pairs) {
   uint4 *base = (blockIdx.z & 1 ? v : k) + (int64_t)(blockIdx.z >> 1) * n_pages * piece;
   const int2 id = pairs.id[blockIdx.y];
@@ -154,7 +155,17 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
 //           registers 4 s + r % 4.  The f32 q and p enter as sums of 2 f16
 //           (22 bits) or 3 bf16 (24 bits), a product each.
 //   f32     v_mfma 16x16x4 f32, A = 16 keys in order, exact products.
-// Query columns beyond the group's are zeros.
+// Query columns beyond the group's are zeros (a matrix instruction costs the
+// same with 1 or 16 queries, and the matrix cores are a fifth busy at most).
+//
+// Bound by reading k and v once, which at 5.4 TB/s also the score kernel's
+// plain reads do not pass: 131071 f16 keys of 8 heads of 128, 537 MB, 96 us +
+// 5 for the join (counters: 545 MB read, each line once).  61 rows of up to
+// 8190 bf16 keys, 767 MB, 152 + 5 us: the rest is the tail of unlike rows.
+// Measured and left: 8 wavefronts per workgroup (same: one CU draws about 50
+// GB/s either way), 3 wavefronts per SIMD (same; bf16 spills), non-temporal
+// loads (99 -> 113 us: half lines that the next wavefront's tile needs are
+// gone), two or four neighbouring tiles per wavefront (98 -> 111).
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 

@@ -19,6 +19,12 @@
 // collected in LDS; a few are put in place one by one, more of them ranked: an
 // entry's rank is the number of entries before it (larger, or equal with a
 // smaller id).
+//
+// Bound by reading the logits: 1792 rows of 51866 f32, 372 MB, 68 us without
+// alternatives (5.4 TB/s), 71 with 5, 80 with 16, 98 with 32; f16 45 and 58
+// (4.1 TB/s: the exponentials and the conversion begin to show).  Rows whose
+// logits rise with their ids take longest (every step replaces the k best: 205
+// us with 5).  One row: latency, 4.4 us with 5 alternatives and 3.8 for the join.
 #pragma once
 #include "rw_kv.hpp"
 

@@ -126,6 +126,17 @@ static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size
 // How a launch cuts its rows' keys: chunks of `chunk` keys, `nsplit` of them
 // for the longest row.  `most`, of which the workspace's size is made, is no
 // less than nsplit and never falls with max_len.
+//   Up to 256 KB of k and v per row and head: one chunk.  A CU draws 50 GB/s,
+// so 256 KB take it 5 us, and the join's launch takes 3 to 5 (448 f16 keys of
+// 64: 6.2 us, in two chunks 5.4 + 2.9; 1024 keys of 128, 512 KB: 15.1 against
+// 7.4 + 4 in four).
+//   Longer: chunks of 128 KB or more, up to 512 workgroups, two per CU (more of
+// them only cost: 131071 keys over 8 heads in 512 workgroups 96 us + join 5.0,
+// in 1024 98 + 5.6, in 2048 104 + 6).
+//   Several rows are seldom of one length, and a long one must not be left to
+// itself at the end: up to 4096 workgroups, in chunks of 192 KB or more (48
+// ragged rows of 20 heads: 64.4 us; chunks of 256 KB 66.9, of 384 KB 73.8, of
+// 128 KB 64.6; 11 rows of 10468 keys: 69.7, and 75.6 with 128 KB).
 struct PagedPlan {
   size_t base;  // workgroups per chunk
   int chunk, nsplit;
@@ -219,7 +230,12 @@ struct CallWorkspace {
 
 // ------------------------------------------------------------- scores
 
-// Parts of a row of logits, one workgroup each.
+// Parts of a row of logits, one workgroup each: about 2048 workgroups where rows
+// are few, no part below 1024 logits.  Short parts take one wavefront, which has
+// no lists to join with another's (one row of 51866, 5 alternatives: 4.4 us and
+// 3.8 for the join; 26 parts of four wavefronts 6.5 and 3.6, one workgroup of
+// 16 wavefronts 25).  Long ones take two (1792 rows with 16 alternatives 80 us,
+// with four wavefronts, each with k best of its own, 89).
 struct ScorePlan {
   int parts;
   int64_t part_len;
