@@ -454,7 +454,7 @@ typedef struct rw_kv_pages {
 
 /* Rows k[r], v[r] (f32 [rows, n_head * head_size], row strides ldk, ldv in
  * floats, 16-byte aligned) become row pos[r] of sequence seq[r] in `layer`,
- * rounded once to the pool's type.  Where two rows of a call have the same
+ * rounded once to the pool's type (to infinity beyond its range).  Where two rows of a call have the same
  * place, the place holds values of either. */
 int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k, size_t ldk, const float *v, size_t ldv,
                          size_t rows, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,

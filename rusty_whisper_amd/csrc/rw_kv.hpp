@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
 //           (22 bits) or 3 bf16 (24 bits), a product each.
 //   f32     v_mfma 16x16x4 f32, A = 16 keys in order, exact products.
 // Query columns beyond the group's are zeros (a matrix instruction costs the
-// same with 1 or 16 queries, and the matrix cores are a fifth busy at most).
+// same with 1 or 16 queries, and the matrix cores are a quarter busy at most).
 //
 // Bound by reading k and v once, which at 5.4 TB/s also the score kernel's
 // plain reads do not pass: 131071 f16 keys of 8 heads of 128, 537 MB, 96 us +
@@ -173,10 +173,11 @@ constexpr int PA_WAVES = 4;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 // The running maximum m is only raised when a score passes it by PA_SLACK (in
 // powers of two): then and only then the wavefront's lanes exchange their
-// maxima and scale what they hold.  p is kept at 2^PA_LIFT of the maximum's 1:
-// the largest, 2^15, fits f16, and f16's smallest step is 2^-35 of the
-// maximum's weight or less.
-constexpr float PA_SLACK = 5.0f, PA_LIFT = 10.0f;
+// maxima and scale what they hold.  The maximum's p is kept at 2^LIFT: for f16
+// 2^10, so that the largest p, 2^15, fits and f16's smallest step is 2^-35 of
+// the maximum's weight or less; else 2^-30, so that sums of 2^25 values near
+// f32's largest stay in range (and values down to 2^-72 keep their bits).
+constexpr float PA_SLACK = 5.0f;
 
 template <class E>
 struct PaTile;  // a tile's product: keys per tile and lane, parts of an f32 operand
@@ -190,11 +191,13 @@ struct PaTile2 {
 template <>
 struct PaTile<F16> : PaTile2<F16> {
   static constexpr int PARTS = 2;
+  static constexpr float LIFT = 10.0f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct PaTile<BF16> : PaTile2<BF16> {
   static constexpr int PARTS = 3;
+  static constexpr float LIFT = -30.0f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -202,6 +205,7 @@ struct PaTile<F32> {
   using T = float;
   typedef f4 Op;
   static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1;
+  static constexpr float LIFT = -30.0f;
   static __device__ f4 mma(Op a, Op b, f4 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] *= fr;
     }
-    const float base = m == NEG_INF ? 0.0f : m - PA_LIFT;
+    const float base = m == NEG_INF ? 0.0f : m - M::LIFT;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       x[j] = __builtin_amdgcn_exp2f(x[j] - base);

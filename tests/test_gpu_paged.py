@@ -96,6 +96,23 @@ def test_query_magnitudes(dtype, scale):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("size", ["largest", "small"])
+def test_values_at_the_ends_of_the_range(dtype, size):
+    """Weighted means of values near the type's largest are finite; small ones
+    (down to 2^-60; f16's down to 2^-10, where it still has all its bits) keep
+    their precision."""
+    page, dim, heads, lens = 64, 64, 2, [1, 33, 3000]
+    k, v = pool(dtype, 1, 64, heads, page, dim, seed=24)
+    big = torch.finfo(v.dtype).max if size == "largest" else 2.0**-60 if dtype != "f16" else 2.0**-10
+    v.uniform_(0.5, 1.0)
+    v.copy_((v.double() * big).to(v.dtype))
+    table = tables(lens, page, 64, seed=24)
+    P = A.KvPages(k, v)
+    q = torch.randn(3, heads * dim, device="cuda")
+    compare(run(P, q, table, lens, 3000), P, q, table, lens, sigma=1.0)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_rising_scores_and_small_weights(dtype):
     """Each block of keys outweighs those before it; then one key far above
     4000 others whose weights add up."""
