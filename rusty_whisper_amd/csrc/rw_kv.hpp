@@ -30,6 +30,9 @@ struct PagedView {
 
 #if defined(__HIPCC__)
 
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// the pool's (and the logits') types: a conversion rounds to nearest even
 struct F32 {
   using T = float;
   static __device__ float load(const T *p) { return *p; }
@@ -52,30 +55,29 @@ __device__ inline const int32_t *paged_row(const PagedView &w, int r) {
   return (unsigned)s < (unsigned)w.n_seqs ? w.table + (int64_t)s * w.ld : nullptr;
 }
 
-// R rows x C values of k and of v per workgroup, 8 values of a row at a time.
-// k's go straight to their rows; v's cross through LDS, so that neighbouring
-// lanes have neighbouring rows, which are neighbours in a page where the rows
-// are a prompt's.  Workgroups of one XCD (every eighth) take tiles that follow
-// each other, whose parts of a cache line then meet in one L2 (24 prompts of
-// 1500 rows, 1280 bf16 values: 112 us, the 4.9 TB/s of a large copy; tiles of
-// 64 x 64 119, of 64 x 32 126, and 135 without the order).
-template <class E, int R, int C>
+// KV_ROWS rows x KV_COLS values of k and of v per workgroup, 8 values of a row
+// per thread.  k's go straight to their rows; v's cross through LDS, so that
+// neighbouring lanes have neighbouring rows, which are neighbours in a page
+// where the rows are a prompt's.  Workgroups of one XCD (every eighth) take
+// tiles that follow each other, whose parts of a cache line then meet in one L2.
+// 24 prompts of 1500 rows, 1280 bf16 values: 112 us, the 4.9 TB/s of a large
+// copy (tiles of 64 x 64 119, of 64 x 32 126, and 135 without the order); 64 rows
+// of a step 5.0 us (tiles of 8 x 256 the same).
+constexpr int KV_ROWS = 32, KV_COLS = 64;
+template <class E>
 __global__ __launch_bounds__(256) void k_kv_write(PagedView w, const float *__restrict__ k, int64_t ldk,
                                                   const float *__restrict__ v, int64_t ldv, int rows,
                                                   const int32_t *__restrict__ pos, int col_tiles, int tiles) {
   using T = typename E::T;
-  typedef float f4 __attribute__((ext_vector_type(4)));
   typedef T Out __attribute__((ext_vector_type(8)));
-  constexpr int LD = R + 2, REPS = R * C / 2048;
-  static_assert(REPS * 2048 == R * C, "whole passes of 256 threads");
-  __shared__ T sv[C][LD];
-  __shared__ int64_t page0[R];  // where the row's page begins, -1: no place
-  __shared__ int slot[R];
+  __shared__ T sv[KV_COLS][KV_ROWS + 2];
+  __shared__ int64_t page0[KV_ROWS];  // where the row's page begins, -1: no place
+  __shared__ int slot[KV_ROWS];
   const int tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);  // gridDim.x: a multiple of 8
   if (tile >= tiles) return;
   const int n = w.heads * w.dim, P = 1 << w.pr, t = threadIdx.x;
-  const int r0 = tile / col_tiles * R, c0 = tile % col_tiles * C;
-  if (t < R) {
+  const int r0 = tile / col_tiles * KV_ROWS, c0 = tile % col_tiles * KV_COLS;
+  if (t < KV_ROWS) {
     int64_t at = -1;
     if (r0 + t < rows) {
       const int32_t *table = paged_row(w, r0 + t);
@@ -88,32 +90,26 @@ __global__ __launch_bounds__(256) void k_kv_write(PagedView w, const float *__re
     }
     page0[t] = at;
   }
-  Out ok[REPS];
+  const int i = t / (KV_COLS / 8), c = c0 + t % (KV_COLS / 8) * 8;
+  const bool in = r0 + i < rows && c < n;
+  Out ok;
+  if (in) {
+    const float *a = k + (int64_t)(r0 + i) * ldk + c, *b = v + (int64_t)(r0 + i) * ldv + c;
+    const f4 a0 = *(const f4 *)a, a1 = *(const f4 *)(a + 4), b0 = *(const f4 *)b, b1 = *(const f4 *)(b + 4);
 #pragma unroll
-  for (int q = 0; q < REPS; ++q) {
-    const int i = (q * 256 + t) / (C / 8), c = c0 + t % (C / 8) * 8;
-    if (r0 + i < rows && c < n) {
-      const float *a = k + (int64_t)(r0 + i) * ldk + c, *b = v + (int64_t)(r0 + i) * ldv + c;
-      const f4 a0 = *(const f4 *)a, a1 = *(const f4 *)(a + 4), b0 = *(const f4 *)b, b1 = *(const f4 *)(b + 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ok[q][j] = E::round(j < 4 ? a0[j] : a1[j - 4]);
-        sv[c - c0 + j][i] = E::round(j < 4 ? b0[j] : b1[j - 4]);
-      }
+    for (int j = 0; j < 8; ++j) {
+      ok[j] = E::round(j < 4 ? a0[j] : a1[j - 4]);
+      sv[c - c0 + j][i] = E::round(j < 4 ? b0[j] : b1[j - 4]);
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int q = 0; q < REPS; ++q) {
-    const int i = (q * 256 + t) / (C / 8), c = c0 + t % (C / 8) * 8;
-    if (r0 + i < rows && c < n && page0[i] >= 0) {
-      const int h = c / w.dim, d = c % w.dim;
-      *(Out *)((T *)w.k + page0[i] + (((int64_t)h << w.pr) + slot[i]) * w.dim + d) = ok[q];
-    }
+  if (in && page0[i] >= 0) {
+    const int h = c / w.dim, d = c % w.dim;
+    *(Out *)((T *)w.k + page0[i] + (((int64_t)h << w.pr) + slot[i]) * w.dim + d) = ok;
   }
 #pragma unroll
-  for (int j = 0; j < 8 * REPS; ++j) {
-    const int e = j * 256 + t, row = e % R, col = e / R;
+  for (int j = 0; j < KV_ROWS * KV_COLS / 256; ++j) {
+    const int e = j * 256 + t, row = e % KV_ROWS, col = e / KV_ROWS;
     if (c0 + col < n && page0[row] >= 0) ((T *)w.v)[page0[row] + ((int64_t)(c0 + col) << w.pr) + slot[row]] = sv[col][row];
   }
 }
@@ -166,8 +162,6 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
 // GB/s either way), 3 wavefronts per SIMD (same; bf16 spills), non-temporal
 // loads (99 -> 113 us: half lines that the next wavefront's tile needs are
 // gone), two or four neighbouring tiles per wavefront (98 -> 111).
-
-typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int PA_WAVES = 4;
 constexpr float PA_LOG2E = 1.44269504088896340736f;

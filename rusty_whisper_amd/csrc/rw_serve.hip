@@ -339,21 +339,12 @@ int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k,
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
   const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
-  // few rows go to places of their own and want workgroups; many rows fill pages
-  const bool many = rows > 256;
-  const size_t tiles = cdiv(rows, many ? 32 : 8) * cdiv(n, many ? 64 : 256);
+  const size_t tiles = cdiv(rows, KV_ROWS) * cdiv(n, KV_COLS);
   if (tiles > MOST_ROWS) return fail(RW_EINVAL, "%zu rows of %zu values", rows, n);
-  const int col_tiles = (int)cdiv(n, many ? 64 : 256);
   const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
 #define RW_WRITE(E)                                                                                                \
-  do {                                                                                                             \
-    if (many)                                                                                                      \
-      hipLaunchKernelGGL((k_kv_write<E, 32, 64>), grid, dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v,  \
-                         (int64_t)ldv, (int)rows, pos, col_tiles, (int)tiles);                                     \
-    else                                                                                                           \
-      hipLaunchKernelGGL((k_kv_write<E, 8, 256>), grid, dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v,  \
-                         (int64_t)ldv, (int)rows, pos, col_tiles, (int)tiles);                                     \
-  } while (0)
+  hipLaunchKernelGGL((k_kv_write<E>), grid, dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v, (int64_t)ldv, \
+                     (int)rows, pos, (int)cdiv(n, KV_COLS), (int)tiles)
   BY_TYPE(pages->dtype, RW_WRITE);
 #undef RW_WRITE
   return launched("k_kv_write");
