@@ -134,9 +134,13 @@ static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size
 // them only cost: 131071 keys over 8 heads in 512 workgroups 96 us + join 5.0,
 // in 1024 98 + 5.6, in 2048 104 + 6).
 //   Several rows are seldom of one length, and a long one must not be left to
-// itself at the end: up to 4096 workgroups, in chunks of 192 KB or more (48
-// ragged rows of 20 heads: 64.4 us; chunks of 256 KB 66.9, of 384 KB 73.8, of
-// 128 KB 64.6; 11 rows of 10468 keys: 69.7, and 75.6 with 128 KB).
+// itself at the end: up to 256 workgroups per row and 4096 in all, in chunks of
+// 192 KB or more (48 ragged rows of 20 heads: 64.4 us; chunks of 256 KB 66.9, of
+// 384 KB 73.8, of 128 KB 64.6; 11 rows of 10468 keys: 69.7, and 75.6 with 128 KB;
+// four rows of 32768 keys, 8 heads: 99 us, ragged 81, and with up to 4096 111 and
+// 88).  Equal shares of all rows' keys for 512 resident workgroups, found from
+// the lengths on the device, measured 171 us where this takes 157 (61 ragged
+// rows, 8 heads).
 struct PagedPlan {
   size_t base;  // workgroups per chunk
   int chunk, nsplit;
@@ -152,7 +156,8 @@ static PagedPlan paged_plan(const rw_kv_pages *p, size_t rows, int n_head, size_
   size_t nsplit = 1;
   if (bytes > (size_t)256 << 10) {
     nsplit = std::min(cdiv(bytes, (size_t)128 << 10), 512 / L.base);
-    if (rows > 1) nsplit = std::max(nsplit, std::min(cdiv(bytes, (size_t)192 << 10), 4096 / L.base));
+    if (rows > 1)
+      nsplit = std::max(nsplit, std::min(cdiv(bytes, (size_t)192 << 10), std::min((size_t)4096, 256 * rows) / L.base));
     nsplit = std::max((size_t)1, std::min(nsplit, (size_t)PA_MAX_SPLIT));
   }
   L.most = nsplit;
