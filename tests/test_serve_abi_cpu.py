@@ -145,3 +145,21 @@ def test_tensors_of_another_type_are_refused():
         A.paged_attention_dev(p, 0, f[0, 0, 0].half(), 1, 1, i, i[0], 5, f[0, 0, 0])
     with pytest.raises(ValueError, match="tokens"):
         A.token_logprobs_dev(f[0, 0, 0], 16, 32, i.long(), 1, f)
+
+
+def test_workspace_of_a_longer_call_is_no_smaller():
+    """A caller sizes its workspace by the longest length it will see."""
+    import random
+
+    rng = random.Random(4)
+    L = A.lib()
+    for _ in range(300):
+        p = pages(dtype=rng.choice((A.F32, A.F16, A.BF16)), n_head=rng.choice((1, 3, 8, 20)),
+                  head_size=rng.choice((32, 64, 96, 128)))
+        rows, heads = rng.choice((1, 2, 7, 61, 300, 5000)), p.n_head * rng.choice((1, 4, 17))
+        lens = sorted(int(2 ** rng.uniform(0, 31)) for _ in range(12))
+        sizes = [L.rw_rocm_paged_attention_workspace_size(p, rows, heads, n) for n in lens]
+        assert sizes == sorted(sizes), (rows, heads, lens, sizes)
+    for rows, n in ((1, 51866), (5, 51866), (2100, 51866), (3, 2**31 - 1)):
+        sizes = [L.rw_rocm_token_logprobs_workspace_size(rows, n, k) for k in range(33)]
+        assert sizes == sorted(sizes)
