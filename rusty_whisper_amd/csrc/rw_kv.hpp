@@ -167,7 +167,7 @@ constexpr int PA_WAVES = 4;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 // The running maximum m is only raised when a score passes it by PA_SLACK (in
 // powers of two): then and only then the wavefront's lanes exchange their
-// maxima and scale what they hold.  The maximum's p is kept at 2^LIFT: for f16
+// maxima and scale what they hold.  The maximum's p is kept at LIFT: for f16
 // 2^10, so that the largest p, 2^15, fits and f16's smallest step is 2^-35 of
 // the maximum's weight or less; else 2^-30, so that sums of 2^25 values near
 // f32's largest stay in range (and values down to 2^-72 keep their bits).
@@ -185,13 +185,13 @@ struct PaTile2 {
 template <>
 struct PaTile<F16> : PaTile2<F16> {
   static constexpr int PARTS = 2;
-  static constexpr float LIFT = 10.0f;
+  static constexpr float LIFT = 0x1p10f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct PaTile<BF16> : PaTile2<BF16> {
   static constexpr int PARTS = 3;
-  static constexpr float LIFT = -30.0f;
+  static constexpr float LIFT = 0x1p-30f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -199,7 +199,7 @@ struct PaTile<F32> {
   using T = float;
   typedef f4 Op;
   static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1;
-  static constexpr float LIFT = -30.0f;
+  static constexpr float LIFT = 0x1p-30f;
   static __device__ f4 mma(Op a, Op b, f4 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -392,10 +392,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] *= fr;
     }
-    const float base = m == NEG_INF ? 0.0f : m - M::LIFT;
+    const float base = m == NEG_INF ? 0.0f : m;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+      // (x - m keeps all its bits where p is large; LIFT in the exponent cost some)
+      x[j] = __builtin_amdgcn_exp2f(x[j] - base) * M::LIFT;
       sum += x[j];
     }
     Op pf[PARTS];
