@@ -454,8 +454,8 @@ typedef struct rw_kv_pages {
 
 /* Rows k[r], v[r] (f32 [rows, n_head * head_size], row strides ldk, ldv in
  * floats, 16-byte aligned) become row pos[r] of sequence seq[r] in `layer`,
- * rounded once to the pool's type (to infinity beyond its range).  Where two rows of a call have the same
- * place, the place holds values of either. */
+ * rounded once to the pool's type (to infinity beyond its range).  Where two
+ * rows of a call have the same place, the place holds values of either. */
 int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k, size_t ldk, const float *v, size_t ldv,
                          size_t rows, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,
                          const int32_t *pos, void *stream);
@@ -470,14 +470,15 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
  * sqrt(head_size)) V over rows 0 .. len[r] - 1 of sequence seq[r], K and V
  * those of key/value head h / (n_head / pages->n_head).  n_head is a
  * multiple of pages->n_head; q and out are f32, row strides ldq, ldo in
- * floats, 16-byte aligned; they may not overlap.  len[r] counts the visible rows (the
- * token's own among them, if it was written before) and is cut at max_len, 2^30
- * and at what the table holds; a row with len[r] <= 0 gets zeros.  Several rows
- * may attend to one sequence, with lengths of their own (the tokens of a prompt,
- * drafted tokens).  max_len sizes the launch: give the longest length, or for a
- * graph the longest that replays will see.  Scores, softmax and sums are f32,
- * products f32-equivalent for every type of pool.  The rows seen and q must
- * be finite; what the pool holds behind a sequence's length is not looked at.
+ * floats, 16-byte aligned; they may not overlap.  len[r] counts the visible
+ * rows (the token's own among them, if it was written before) and is cut at
+ * max_len, at 2^30 and at what the table holds; a row with len[r] <= 0, or that
+ * sees no row of the pool, gets zeros.  Several rows may attend to one sequence,
+ * with lengths of their own (the tokens of a prompt, drafted tokens).  max_len
+ * sizes the launch: give the longest length, or for a graph the longest that
+ * replays will see.  Scores, softmax and sums are f32, products f32-equivalent
+ * for every type of pool.  The rows seen and q must be finite; what the pool
+ * holds behind a sequence's length has no effect.
  * The workspace (NULL: one kept per (device, stream), not for a stream that
  * is being captured) holds rw_rocm_paged_attention_workspace_size bytes, 16-byte
  * aligned; 0 for arguments the call would refuse. */
@@ -529,8 +530,8 @@ int rw_rocm_kv_book_info(const rw_kv_book *b, size_t *free_pages, size_t *used_p
  * of logits [rows, n_vocab] (device, dtype RW_F32, RW_F16 or RW_BF16, row
  * stride ld in elements): log_softmax as src/transcribe.rs:482-486 has it, for
  * what rw_rocm_logits_topk_dev does not give -- a transcript's average
- * log-prob, the no-speech probability, the
- * language tokens' probabilities, an entropy threshold.
+ * log-prob, the no-speech probability, the language tokens' probabilities, an
+ * entropy threshold.
  *   logprobs[rows, n_tok]  of tokens[rows, n_tok] (ids on the device); the id
  *                          0xFFFFFFFF ("no token", padding) gets 0, any other id outside
  *                          the vocabulary NaN.  n_tok = 0: neither is used.

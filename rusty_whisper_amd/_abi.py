@@ -587,12 +587,12 @@ def _rows(a, n: int, ld: int | None, what: str, device: int | None, dtypes=("tor
         p = a.data_ptr()
     except AttributeError:
         return _ptr(a), ld or n
-    st, shape = a.stride(), a.shape
-    if _dtype_name(a.dtype) not in dtypes or (st and st[-1] != 1 and shape[-1] > 1):
+    st = a.stride()
+    if _dtype_name(a.dtype) not in dtypes or (st and st[-1] != 1 and a.shape[-1] > 1):
         raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
-    return p, ld or (st[0] if len(st) == 2 and shape[0] > 1 else n)
+    return p, ld or (st[0] if len(st) == 2 and (st[0] >= n or a.shape[0] > 1) else n)
 
 
 def _host(a: np.ndarray) -> int:
