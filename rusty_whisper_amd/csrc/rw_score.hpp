@@ -11,19 +11,20 @@
 // maxima scale S and T); lanes, wavefronts and parts are joined at the end in
 // a fixed order.
 //
-// The alternatives.  A wavefront keeps its k best so far, one per lane; a later
-// logit, whose id is larger, enters only if it is larger than the k-th of them,
-// and most steps end with one comparison of the lanes' maxima.  Where many lanes'
-// maxima pass, a lower bound of their k-th largest is one of the k-th best, and
-// on rows in no special order little more than k logits reach it.  These are
-// collected in LDS; a few are put in place one by one, more of them ranked: an
-// entry's rank is the number of entries before it (larger, or equal with a
-// smaller id).
+// The alternatives.  `lo` is the smallest logit that may be one of the k best: of
+// the k best so far, kept one per lane, the next above the k-th (later ids are
+// larger, so an equal logit comes too late), or the k-th largest of the lanes'
+// maxima so far, which score_bound finds to within a few.  Most steps end with
+// one comparison; the logits from lo on are collected in LDS, and from time to
+// time (for few alternatives in every step) they are put into the k best: a few
+// one by one, more of them ranked, an entry's rank being the number of entries
+// before it (larger, or equal with a smaller id).  366 rows of 51865 f32 with 20
+// alternatives: 28 us; ranked in every step 35; with 5, every step 22.
 //
 // Bound by reading the logits: 1792 rows of 51866 f32, 372 MB, 68 us without
-// alternatives (5.4 TB/s), 71 with 5, 80 with 16, 98 with 32; f16 45 and 58
+// alternatives (5.4 TB/s), 71 with 5, 77 with 16, 100 with 32; f16 45 and 58
 // (4.1 TB/s: the exponentials and the conversion begin to show).  Rows whose
-// logits rise with their ids take longest (every step replaces the k best: 205
+// logits rise with their ids take longest (every step replaces the k best: 180
 // us with 5).  One row: latency, 4.4 us with 5 alternatives and 3.8 for the join.
 #pragma once
 #include "rw_kv.hpp"
@@ -33,6 +34,7 @@ namespace rw {
 constexpr int SCORE_TOP = 32;         // alternatives per row at most
 constexpr int SCORE_MAX_PARTS = 64;   // parts of a row: a lane each in k_score_join
 constexpr int SCORE_HEADS = 8;        // alternatives up to which k_score_join compares heads
+constexpr int SCORE_EAGER = 8;        // alternatives up to which every step's candidates are ranked at once
 constexpr int SCORE_LINE = 128;       // bytes that the loads of a step are aligned to
 constexpr uint32_t SCORE_NONE = 0xFFFFFFFFu;
 
@@ -265,7 +267,8 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
   const int64_t u1 = min((int64_t)n + skip, (int64_t)(pt + 1) * part_len);
 
   ScoreStats st{NEG_INF, 0.0f, 0.0f};
-  float lo = score_next(NEG_INF);  // the smallest logit that may enter
+  const float all = score_next(NEG_INF);
+  float lo = all;  // the smallest logit that may be one of the k best
   ScoreBest best;
   float *wv_v = ev[wv], *sv = ev[wv] + CAP;  // candidates; the places that `take` wants
   int *wv_i = ei[wv], *si = ei[wv] + CAP;
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
     }
     cnt = 0;
     score_wave_sync();
-    if (best.n == k) lo = score_next(score_lane(best.v, k - 1));
+    if (best.n == k) lo = fmaxf(lo, score_next(score_lane(best.v, k - 1)));
   };
 
   // the step at place u: this lane's j-th load has the ids u - skip + (64 j + lane) V ..
@@ -329,31 +332,30 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
     if (k == 0) continue;
     const uint64_t pass = __builtin_amdgcn_ballot_w64(mx >= lo);
     if (!pass) continue;
-    float least = lo;
-    if (__builtin_popcountll(pass) > k + 3) least = fmaxf(lo, score_bound(mx, k, lo));
+    // the k-th largest of the lanes' maxima so far is one of the k best
+    if (__builtin_popcountll(pass) > (k <= SCORE_EAGER ? k + 3 : 4) && __builtin_popcountll(__builtin_amdgcn_ballot_w64(st.m >= all)) > k)
+      lo = fmaxf(lo, score_bound(st.m, k, all));
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       float mj = y[j * V];
 #pragma unroll
       for (int i = 1; i < V; ++i) mj = fmaxf(mj, y[j * V + i]);
-      if (!__builtin_amdgcn_ballot_w64(mj >= least)) continue;
-      if (cnt > CAP - 64 * V) {  // equal logits in great number
-        keep();
-        least = fmaxf(least, lo);
-      }
+      if (!__builtin_amdgcn_ballot_w64(mj >= lo)) continue;
+      if (cnt > CAP - 64 * V) keep();  // equal logits in great number
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const uint64_t in = __builtin_amdgcn_ballot_w64(y[j * V + i] >= least);
+        const uint64_t in = __builtin_amdgcn_ballot_w64(y[j * V + i] >= lo);
         if (!in) continue;
-        if (y[j * V + i] >= least) {
+        if (y[j * V + i] >= lo) {
           const int at = cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
           wv_v[at] = y[j * V + i], wv_i[at] = (int)(e0 + 64 * V * j + i);
         }
         cnt += __builtin_popcountll(in);
       }
     }
-    if (cnt) keep();
+    if (cnt && (k <= SCORE_EAGER || cnt + best.n > 64)) keep();
   }
+  if (cnt) keep();
 
   // lanes, then wavefronts
   st = score_wave_join(st);

@@ -239,8 +239,8 @@ struct CallWorkspace {
 // are few, no part below 1024 logits.  Short parts take one wavefront, which has
 // no lists to join with another's (one row of 51866, 5 alternatives: 4.4 us and
 // 3.8 for the join; 26 parts of four wavefronts 6.5 and 3.6, one workgroup of
-// 16 wavefronts 25).  Long ones take two (1792 rows with 16 alternatives 80 us,
-// with four wavefronts, each with k best of its own, 89).
+// 16 wavefronts 25).  Long ones take two (1792 rows with 5 alternatives 71 us,
+// with four wavefronts, each with k best of its own, 80).
 struct ScorePlan {
   int parts;
   int64_t part_len;
