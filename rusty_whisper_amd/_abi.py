@@ -580,19 +580,49 @@ def _dense(a, dtype: str, what: str, device: int | None):
     return p
 
 
+def _row_step(a, n: int, what: str) -> int:
+    """Elements from one row of n values to the next.  A row's values are the
+    trailing dimensions of a tensor, which have to be dense, its rows the ones
+    before, which have to lie at one distance: [rows, n], a column block of
+    wider rows (or their first n columns), [rows, n_head, head_size] out of a
+    fused projection.  A contiguous tensor of any other shape is rows one
+    behind the other."""
+    sh, st = a.shape, a.stride()
+    values, d = 1, len(sh)
+    while d and values < n:
+        d -= 1
+        if sh[d] != 1 and st[d] != values:
+            raise ValueError(f"{what}: the values of a row are not contiguous")
+        values *= sh[d]
+    if d == 0 or (values != n and d < len(sh) - 1):
+        if not a.is_contiguous():
+            raise ValueError(f"{what}: not rows of {n} values")
+        return n
+    count, step = 1, n  # the rows of dimensions d .. are `step` apart
+    for i in range(d - 1, -1, -1):
+        if sh[i] == 1:
+            continue
+        if count == 1:
+            step = st[i]
+        elif st[i] != count * step:
+            raise ValueError(f"{what}: rows are not all at one distance")
+        count *= sh[i]
+    return step
+
+
 def _rows(a, n: int, ld: int | None, what: str, device: int | None, dtypes=("torch.float32",)):
-    """(pointer, row stride) of device rows of n values; a 2-D tensor, which
-    may be a column block of wider rows, brings its stride."""
+    """(pointer, row stride) of device rows of n values (a tensor's as _row_step
+    has them, at the stride `ld` where one is given)."""
     try:
         p = a.data_ptr()
     except AttributeError:
         return _ptr(a), ld or n
-    st = a.stride()
-    if _dtype_name(a.dtype) not in dtypes or (st and st[-1] != 1 and a.shape[-1] > 1):
+    if _dtype_name(a.dtype) not in dtypes:
         raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
-    return p, ld or (st[0] if len(st) == 2 and (st[0] >= n or a.shape[0] > 1) else n)
+    step = _row_step(a, n, what)
+    return p, ld or step
 
 
 def _host(a: np.ndarray) -> int:
