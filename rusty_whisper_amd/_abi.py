@@ -566,17 +566,40 @@ _TORCH_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": B
 _dtype_name = functools.lru_cache(None)(str)
 
 
-def _dense(a, dtype: str, what: str, device: int | None):
-    """_ptr of a device array, which as a tensor must be dense, of `dtype` and
-    on the `device` of the call's first tensor (None: that was a pointer)."""
+def _pointer(a, what: str) -> int | None:
+    """A device pointer given as a number (None: NULL)."""
+    if isinstance(a, np.ndarray):
+        raise ValueError(f"{what} is a host array")
+    return _ptr(a)
+
+
+def _dense(a, dtype: str, count: int, what: str, device: int | None):
+    """The pointer of a device array of `count` elements, which as a tensor
+    must be dense, of `dtype`, long enough and on the `device` of the call's
+    first tensor (None: that was a pointer)."""
     try:
         p = a.data_ptr()
     except AttributeError:
-        return _ptr(a)
+        return _pointer(a, what)
     if _dtype_name(a.dtype) != dtype or not a.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
+    if a.numel() < count:
+        raise ValueError(f"{what} has {a.numel()} elements, the call takes {count}")
+    return p
+
+
+def _workspace(a, size: int, device: int | None):
+    """The pointer of a workspace of `size` bytes."""
+    try:
+        p = a.data_ptr()
+    except AttributeError:
+        return _pointer(a, "workspace")
+    if not a.is_contiguous() or a.numel() * a.element_size() < size:
+        raise ValueError(f"workspace is not {size} contiguous bytes")
+    if device is not None and a.get_device() != device:
+        raise ValueError("workspace is on another device")
     return p
 
 
@@ -610,19 +633,25 @@ def _row_step(a, n: int, what: str) -> int:
     return step
 
 
-def _rows(a, n: int, ld: int | None, what: str, device: int | None, dtypes=("torch.float32",)):
-    """(pointer, row stride) of device rows of n values (a tensor's as _row_step
-    has them, at the stride `ld` where one is given)."""
+def _rows(a, rows: int, n: int, ld: int | None, what: str, device: int | None, dtypes=("torch.float32",)):
+    """(pointer, row stride) of `rows` device rows of n values (a tensor's as
+    _row_step has them, at the stride `ld` where one is given)."""
     try:
         p = a.data_ptr()
     except AttributeError:
-        return _ptr(a), ld or n
+        return _pointer(a, what), ld or n
     if _dtype_name(a.dtype) not in dtypes:
         raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
+    sh, st = a.shape, a.stride()
+    if ld is None and len(sh) == 2 and 1 <= rows <= sh[0] != 1 and sh[1] == n and st[1] == 1:
+        return p, st[0]  # (most calls)
     step = _row_step(a, n, what)
-    return p, ld or step
+    step = ld or step
+    if rows > 0 and (rows - 1) * step + n > (1 + sum((x - 1) * y for x, y in zip(sh, st)) if a.numel() else 0):
+        raise ValueError(f"{what} ends before row {rows - 1} of {n} values does")
+    return p, step
 
 
 def _host(a: np.ndarray) -> int:
@@ -656,10 +685,11 @@ class KvPages:
         return self.st.n_head * self.st.head_size
 
 
-def _table_args(table, seq, device: int):
+def _table_args(table, seq, rows: int, device: int):
     """(table, ld_table, n_seqs, seq) of the device entries."""
     n_seqs, ld = table.shape
-    return _dense(table, "torch.int32", "table", device), ld, n_seqs, _dense(seq, "torch.int32", "seq", device)
+    return (_dense(table, "torch.int32", n_seqs * ld, "table", device), ld, n_seqs,
+            _dense(seq, "torch.int32", rows, "seq", device))
 
 
 def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=None, ldk: int | None = None,
@@ -667,10 +697,10 @@ def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=No
     """Device rows k[r], v[r] into row pos[r] of sequence seq[r] (None: r).
     table: device int32 [n_seqs, pages per sequence]; pos, seq: device int32."""
     d = pages.device
-    t, ld, n_seqs, s = _table_args(table, seq, d)
+    t, ld, n_seqs, s = _table_args(table, seq, rows, d)
     n = pages.n_values
-    check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, n, ldk, "k", d), *_rows(v, n, ldv, "v", d), rows, t, ld,
-                                     n_seqs, s, _dense(pos, "torch.int32", "pos", d), stream))
+    check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, rows, n, ldk, "k", d), *_rows(v, rows, n, ldv, "v", d),
+                                     rows, t, ld, n_seqs, s, _dense(pos, "torch.int32", rows, "pos", d), stream))
 
 
 def kv_copy_pages_dev(pages: KvPages, src, dst, stream: int | None = None) -> None:
@@ -693,11 +723,12 @@ def paged_attention_dev(pages: KvPages, layer: int, q, rows: int, n_head: int, t
     first lens[r] rows of sequence seq[r] (None: r).  table, lens and seq:
     device int32, as for kv_write_dev; max_len: the longest of lens, or more."""
     d = pages.device
-    t, ld, n_seqs, s = _table_args(table, seq, d)
+    t, ld, n_seqs, s = _table_args(table, seq, rows, d)
     n = n_head * pages.st.head_size
-    check(lib().rw_rocm_paged_attention_dev(pages.st, layer, *_rows(q, n, ldq, "q", d), rows, n_head, t, ld, n_seqs, s,
-                                            _dense(lens, "torch.int32", "lens", d), max_len,
-                                            *_rows(out, n, ldo, "out", d), _ptr(workspace), workspace_len, stream))
+    check(lib().rw_rocm_paged_attention_dev(pages.st, layer, *_rows(q, rows, n, ldq, "q", d), rows, n_head, t, ld, n_seqs,
+                                            s, _dense(lens, "torch.int32", rows, "lens", d), max_len,
+                                            *_rows(out, rows, n, ldo, "out", d),
+                                            _workspace(workspace, workspace_len, d), workspace_len, stream))
 
 
 class KvBook:
@@ -781,10 +812,10 @@ class KvBook:
 
 # --------------------------------------------------------- token scores
 
-def _ids(a, what: str, device: int | None):
+def _ids(a, count: int, what: str, device: int | None):
     """_dense of 32-bit ids, signed or not."""
     unsigned = _dtype_name(getattr(a, "dtype", None)) == "torch.uint32"
-    return _dense(a, "torch.uint32" if unsigned else "torch.int32", what, device)
+    return _dense(a, "torch.uint32" if unsigned else "torch.int32", count, what, device)
 
 
 def token_logprobs_workspace_size(rows: int, n_vocab: int, k: int) -> int:
@@ -803,10 +834,12 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
         if dtype is None:
             dtype = _TORCH_DTYPES.get(_dtype_name(logits.dtype), -1)
     check(lib().rw_rocm_token_logprobs_dev(
-        F32 if dtype is None else dtype, *_rows(logits, n_vocab, ld, "logits", d, tuple(_TORCH_DTYPES)), rows, n_vocab,
-        _ids(tokens, "tokens", d), n_tok, _dense(logprobs, "torch.float32", "logprobs", d),
-        _dense(entropy, "torch.float32", "entropy", d), k, _ids(top_ids, "top_ids", d),
-        _dense(top_logprobs, "torch.float32", "top_logprobs", d), _ptr(workspace), workspace_len, stream))
+        F32 if dtype is None else dtype, *_rows(logits, rows, n_vocab, ld, "logits", d, tuple(_TORCH_DTYPES)), rows,
+        n_vocab, _ids(tokens, rows * n_tok, "tokens", d), n_tok,
+        _dense(logprobs, "torch.float32", rows * n_tok, "logprobs", d),
+        _dense(entropy, "torch.float32", rows, "entropy", d), k, _ids(top_ids, rows * k, "top_ids", d),
+        _dense(top_logprobs, "torch.float32", rows * k, "top_logprobs", d), _workspace(workspace, workspace_len, d),
+        workspace_len, stream))
 
 
 MODEL_PARSE_ONLY = 1

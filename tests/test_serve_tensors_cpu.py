@@ -1,6 +1,7 @@
 """How the serving entries' Python wrappers take tensors: which element of
 which row a call reads.  On the CPU: pointers and strides are looked at, no
 call is queued."""
+import numpy as np
 import pytest
 import torch
 
@@ -13,7 +14,7 @@ N = H * D
 def places(a, ld=None):
     """Element [row, value] as `_rows` tells the library to read it: offsets
     from the storage's start."""
-    p, step = A._rows(a, N, ld, "q", None)
+    p, step = A._rows(a, ROWS, N, ld, "q", None)
     first = (p - a.untyped_storage().data_ptr()) // 4
     return [[first + r * step + i for i in range(N)] for r in range(ROWS)]
 
@@ -48,10 +49,10 @@ def test_rows_are_the_tensors_own(name):
 
 def test_one_row_and_flat_arrays():
     for a in (numbered(1, N), numbered(N), numbered(H, D), numbered(1, 1, N), numbered(7, 1, N)[3:4]):
-        assert A._rows(a, N, None, "q", None) == (a.data_ptr(), N)
-    assert A._rows(numbered(ROWS * N), N, None, "q", None)[1] == N  # rows one behind the other
-    assert A._rows(numbered(ROWS, N + 9), N, None, "q", None)[1] == N + 9  # the first columns of wider rows
-    assert A._rows(numbered(ROWS, 2 * N), N, 3 * N, "q", None)[1] == 3 * N  # the caller's own stride
+        assert A._rows(a, 1, N, None, "q", None) == (a.data_ptr(), N)
+    assert A._rows(numbered(ROWS * N), ROWS, N, None, "q", None)[1] == N  # rows one behind the other
+    assert A._rows(numbered(ROWS, N + 9), ROWS, N, None, "q", None)[1] == N + 9  # the first columns of wider rows
+    assert A._rows(numbered(ROWS, 2 * N), 4, N, 3 * N, "q", None)[1] == 3 * N  # the caller's own stride
 
 
 @pytest.mark.parametrize("a,needle", [
@@ -67,4 +68,74 @@ def test_one_row_and_flat_arrays():
 @pytest.mark.parametrize("ld", [None, N])
 def test_other_layouts_are_refused(a, needle, ld):
     with pytest.raises(ValueError, match=needle):
-        A._rows(a, N, ld, "q", None)
+        A._rows(a, ROWS, N, ld, "q", None)
+
+
+def i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def pages():
+    return A.KvPages(torch.zeros(1, 5, H, 16, D), torch.zeros(1, 5, H, D, 16))
+
+
+def write(**kw):
+    f = dict(k=torch.zeros(ROWS, N), v=torch.zeros(ROWS, N), table=i32(2, 3), pos=i32(ROWS), seq=i32(ROWS))
+    f.update(kw)
+    A.kv_write_dev(pages(), 0, f["k"], f["v"], ROWS, f["table"], f["pos"], seq=f["seq"], ldk=f.get("ldk"))
+
+
+def attention(**kw):
+    f = dict(q=torch.zeros(ROWS, 2 * N), table=i32(2, 3), lens=i32(ROWS), seq=i32(ROWS), out=torch.zeros(ROWS, 2 * N),
+             workspace=None, workspace_len=0)
+    f.update(kw)
+    A.paged_attention_dev(pages(), 0, f["q"], ROWS, 2 * H, f["table"], f["lens"], 40, f["out"], seq=f["seq"],
+                          workspace=f["workspace"], workspace_len=f["workspace_len"])
+
+
+def scores(**kw):
+    f = dict(logits=torch.zeros(ROWS, 50), tokens=i32(ROWS, 2), logprobs=torch.zeros(ROWS, 2), entropy=torch.zeros(ROWS),
+             ids=i32(ROWS, 3), top=torch.zeros(ROWS, 3), workspace=None, workspace_len=0)
+    f.update(kw)
+    A.token_logprobs_dev(f["logits"], ROWS, 50, f["tokens"], 2, f["logprobs"], entropy=f["entropy"], k=3,
+                         top_ids=f["ids"], top_logprobs=f["top"], workspace=f["workspace"],
+                         workspace_len=f["workspace_len"])
+
+
+SHORT = [(write, dict(k=torch.zeros(ROWS - 1, N)), "k ends"), (write, dict(v=torch.zeros(ROWS * N - 1)), "v ends"),
+         (write, dict(v=torch.zeros(ROWS, 3, H, D)[: ROWS - 1, 1]), "v ends"),
+         (write, dict(ldk=N + 4), "k ends"),
+         (write, dict(k=torch.zeros(0, N)), "k ends"),
+         (write, dict(pos=i32(ROWS - 1)), "pos has 5"), (write, dict(seq=i32(1)), "seq has 1"),
+         (attention, dict(q=torch.zeros(ROWS, N)), "q"), (attention, dict(q=torch.zeros(ROWS - 1, 2 * N)), "q ends"),
+         (attention, dict(out=torch.zeros(ROWS - 1, 2 * N)), "out ends"), (attention, dict(lens=i32(2)), "lens has 2"),
+         (attention, dict(seq=i32(ROWS - 1)), "seq has 5"),
+         (attention, dict(workspace=torch.zeros(1023, dtype=torch.uint8), workspace_len=1024), "workspace"),
+         (attention, dict(workspace=torch.zeros(4, 600, dtype=torch.uint8)[:, :300], workspace_len=1024), "workspace"),
+         (scores, dict(logits=torch.zeros(ROWS - 1, 50)), "logits ends"), (scores, dict(logits=torch.zeros(ROWS, 49)), "logits"),
+         (scores, dict(tokens=i32(ROWS, 1)), "tokens has 6"), (scores, dict(logprobs=torch.zeros(ROWS)), "logprobs has 6"),
+         (scores, dict(entropy=torch.zeros(ROWS - 1)), "entropy has 5"), (scores, dict(ids=i32(ROWS, 2)), "top_ids has 12"),
+         (scores, dict(top=torch.zeros(3)), "top_logprobs has 3"),
+         (scores, dict(workspace=torch.zeros(2), workspace_len=16), "workspace")]
+
+
+@pytest.mark.parametrize("call,bad,needle", SHORT, ids=[f"{c.__name__}-{i}" for i, (c, _, _) in enumerate(SHORT)])
+def test_tensors_that_end_too_early_are_refused(call, bad, needle):
+    with pytest.raises(ValueError, match=needle):
+        call(**bad)
+
+
+@pytest.mark.parametrize("call", [write, attention, scores], ids=lambda c: c.__name__)
+def test_tensors_that_just_suffice_reach_the_library(call):
+    with pytest.raises(A.RwError):  # no device here, or tensors that are not on it
+        call()
+
+
+HOST = [(write, n) for n in ("k", "v", "pos", "seq")] + [(attention, n) for n in ("q", "lens", "seq", "out", "workspace")] + [
+    (scores, n) for n in ("logits", "tokens", "logprobs", "entropy", "ids", "top", "workspace")]
+
+
+@pytest.mark.parametrize("call,name", HOST, ids=[f"{c.__name__}-{n}" for c, n in HOST])
+def test_host_arrays_are_refused(call, name):
+    with pytest.raises(ValueError, match="host array"):
+        call(**{name: np.zeros(4096, np.float32)})
