@@ -8,7 +8,6 @@ fallback: if the library or a gfx950 device is missing, calls raise.
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import os
 import re
 
@@ -559,11 +558,12 @@ def logits_topk_workspace_size(rows: int, n_vocab: int, k: int) -> int:
 
 # ------------------------------------------- keys and values in pages
 
-_TORCH_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
-
-
-# a dtype's name: a step's calls look at a dozen arrays, and str() of a dtype takes 0.4 us
-_dtype_name = functools.lru_cache(None)(str)
+try:  # (a step's calls look at a dozen tensors: types are compared as objects, not by name)
+    from torch import bfloat16 as _BF16, float16 as _F16, float32 as _F32, int32 as _I32, uint32 as _U32
+except ImportError:
+    _BF16 = _F16 = _F32 = _I32 = _U32 = None
+_TORCH_DTYPES = {_F32: F32, _F16: F16, _BF16: BF16}
+_ANY_FLOAT = (_F32, _F16, _BF16)
 
 
 def _pointer(a, what: str) -> int | None:
@@ -573,7 +573,7 @@ def _pointer(a, what: str) -> int | None:
     return _ptr(a)
 
 
-def _dense(a, dtype: str, count: int, what: str, device: int | None):
+def _dense(a, dtype, count: int, what: str, device: int | None):
     """The pointer of a device array of `count` elements, which as a tensor
     must be dense, of `dtype`, long enough and on the `device` of the call's
     first tensor (None: that was a pointer)."""
@@ -581,7 +581,7 @@ def _dense(a, dtype: str, count: int, what: str, device: int | None):
         p = a.data_ptr()
     except AttributeError:
         return _pointer(a, what)
-    if _dtype_name(a.dtype) != dtype or not a.is_contiguous():
+    if a.dtype is not dtype or not a.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
@@ -633,20 +633,20 @@ def _row_step(a, n: int, what: str) -> int:
     return step
 
 
-def _rows(a, rows: int, n: int, ld: int | None, what: str, device: int | None, dtypes=("torch.float32",)):
+def _rows(a, rows: int, n: int, ld: int | None, what: str, device: int | None, dtypes=(_F32,)):
     """(pointer, row stride) of `rows` device rows of n values (a tensor's as
     _row_step has them, at the stride `ld` where one is given)."""
     try:
         p = a.data_ptr()
     except AttributeError:
         return _pointer(a, what), ld or n
-    if _dtype_name(a.dtype) not in dtypes:
-        raise ValueError(f"{what} must be rows of {' or '.join(dtypes)}")
+    if a.dtype not in dtypes:
+        raise ValueError(f"{what} must be rows of {' or '.join(map(str, dtypes))}")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
     sh, st = a.shape, a.stride()
-    if ld is None and len(sh) == 2 and 1 <= rows <= sh[0] != 1 and sh[1] == n and st[1] == 1:
-        return p, st[0]  # (most calls)
+    if ld is None and sh == (rows, n) and st[1] == 1:
+        return p, st[0] if rows > 1 else n  # (most calls)
     step = _row_step(a, n, what)
     step = ld or step
     if rows > 0 and (rows - 1) * step + n > (1 + sum((x - 1) * y for x, y in zip(sh, st)) if a.numel() else 0):
@@ -668,7 +668,7 @@ class KvPages:
         L, N, H, P, D = k.shape
         if v.shape != (L, N, H, D, P):
             raise ValueError("v must be [n_layer, n_pages, n_head, head_size, page_rows]")
-        dtype = _TORCH_DTYPES.get(_dtype_name(k.dtype))
+        dtype = _TORCH_DTYPES.get(k.dtype)
         if k.dtype != v.dtype or dtype is None:
             raise ValueError("k and v must have one type: float32, float16 or bfloat16")
         if not (k.is_contiguous() and v.is_contiguous()):
@@ -688,8 +688,8 @@ class KvPages:
 def _table_args(table, seq, rows: int, device: int):
     """(table, ld_table, n_seqs, seq) of the device entries."""
     n_seqs, ld = table.shape
-    return (_dense(table, "torch.int32", n_seqs * ld, "table", device), ld, n_seqs,
-            _dense(seq, "torch.int32", rows, "seq", device))
+    return (_dense(table, _I32, n_seqs * ld, "table", device), ld, n_seqs,
+            _dense(seq, _I32, rows, "seq", device))
 
 
 def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=None, ldk: int | None = None,
@@ -700,7 +700,7 @@ def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=No
     t, ld, n_seqs, s = _table_args(table, seq, rows, d)
     n = pages.n_values
     check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, rows, n, ldk, "k", d), *_rows(v, rows, n, ldv, "v", d),
-                                     rows, t, ld, n_seqs, s, _dense(pos, "torch.int32", rows, "pos", d), stream))
+                                     rows, t, ld, n_seqs, s, _dense(pos, _I32, rows, "pos", d), stream))
 
 
 def kv_copy_pages_dev(pages: KvPages, src, dst, stream: int | None = None) -> None:
@@ -726,7 +726,7 @@ def paged_attention_dev(pages: KvPages, layer: int, q, rows: int, n_head: int, t
     t, ld, n_seqs, s = _table_args(table, seq, rows, d)
     n = n_head * pages.st.head_size
     check(lib().rw_rocm_paged_attention_dev(pages.st, layer, *_rows(q, rows, n, ldq, "q", d), rows, n_head, t, ld, n_seqs,
-                                            s, _dense(lens, "torch.int32", rows, "lens", d), max_len,
+                                            s, _dense(lens, _I32, rows, "lens", d), max_len,
                                             *_rows(out, rows, n, ldo, "out", d),
                                             _workspace(workspace, workspace_len, d), workspace_len, stream))
 
@@ -814,8 +814,8 @@ class KvBook:
 
 def _ids(a, count: int, what: str, device: int | None):
     """_dense of 32-bit ids, signed or not."""
-    unsigned = _dtype_name(getattr(a, "dtype", None)) == "torch.uint32"
-    return _dense(a, "torch.uint32" if unsigned else "torch.int32", count, what, device)
+    unsigned = a is not None and getattr(a, "dtype", None) is _U32
+    return _dense(a, _U32 if unsigned else _I32, count, what, device)
 
 
 def token_logprobs_workspace_size(rows: int, n_vocab: int, k: int) -> int:
@@ -832,13 +832,13 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
     if hasattr(logits, "data_ptr"):
         d = logits.get_device()
         if dtype is None:
-            dtype = _TORCH_DTYPES.get(_dtype_name(logits.dtype), -1)
+            dtype = _TORCH_DTYPES.get(logits.dtype, -1)
     check(lib().rw_rocm_token_logprobs_dev(
-        F32 if dtype is None else dtype, *_rows(logits, rows, n_vocab, ld, "logits", d, tuple(_TORCH_DTYPES)), rows,
+        F32 if dtype is None else dtype, *_rows(logits, rows, n_vocab, ld, "logits", d, _ANY_FLOAT), rows,
         n_vocab, _ids(tokens, rows * n_tok, "tokens", d), n_tok,
-        _dense(logprobs, "torch.float32", rows * n_tok, "logprobs", d),
-        _dense(entropy, "torch.float32", rows, "entropy", d), k, _ids(top_ids, rows * k, "top_ids", d),
-        _dense(top_logprobs, "torch.float32", rows * k, "top_logprobs", d), _workspace(workspace, workspace_len, d),
+        _dense(logprobs, _F32, rows * n_tok, "logprobs", d),
+        _dense(entropy, _F32, rows, "entropy", d), k, _ids(top_ids, rows * k, "top_ids", d),
+        _dense(top_logprobs, _F32, rows * k, "top_logprobs", d), _workspace(workspace, workspace_len, d),
         workspace_len, stream))
 
 
