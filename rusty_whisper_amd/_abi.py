@@ -831,8 +831,11 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
     d = None
     if hasattr(logits, "data_ptr"):
         d = logits.get_device()
+        own = _TORCH_DTYPES.get(logits.dtype, -1)
         if dtype is None:
-            dtype = _TORCH_DTYPES.get(logits.dtype, -1)
+            dtype = own
+        elif dtype != own:
+            raise ValueError(f"dtype {dtype} for {logits.dtype} logits")
     check(lib().rw_rocm_token_logprobs_dev(
         F32 if dtype is None else dtype, *_rows(logits, rows, n_vocab, ld, "logits", d, _ANY_FLOAT), rows,
         n_vocab, _ids(tokens, rows * n_tok, "tokens", d), n_tok,

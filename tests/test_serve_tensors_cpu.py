@@ -139,3 +139,13 @@ HOST = [(write, n) for n in ("k", "v", "pos", "seq")] + [(attention, n) for n in
 def test_host_arrays_are_refused(call, name):
     with pytest.raises(ValueError, match="host array"):
         call(**{name: np.zeros(4096, np.float32)})
+
+
+def test_a_type_that_is_not_the_logits_own_is_refused():
+    """RW_F32 for f16 logits would read twice their bytes."""
+    for own in (torch.float32, torch.float16, torch.bfloat16):
+        for dtype in (A.F32, A.F16, A.BF16):
+            x, lp = torch.zeros(1, 8, dtype=own), torch.zeros(1, 1)
+            right = A._TORCH_DTYPES[own] == dtype
+            with pytest.raises(A.RwError if right else ValueError, match="" if right else "logits"):
+                A.token_logprobs_dev(x, 1, 8, i32(1, 1), 1, lp, dtype=dtype)
