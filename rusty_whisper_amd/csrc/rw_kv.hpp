@@ -9,6 +9,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #if defined(__HIPCC__)
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -148,8 +150,9 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
 // cores without LDS and without moves between lanes:
 //   2-byte  v_mfma 16x16x32, A = 16 keys: row r of half s is key
 //           8 (r / 4) + 4 s + r % 4, whose scores then lie in lane r / 4's
-//           registers 4 s + r % 4.  The f32 q and p enter as sums of 2 f16
-//           (22 bits) or 3 bf16 (24 bits), a product each.
+//           registers 4 s + r % 4.  The f32 q enters as a sum of 2 f16 (22 bits)
+//           or 3 bf16 (24 bits), a product each; p as 3 bf16 for both types, as
+//           weights need f32's range, and f16's v as 2 bf16 (8 and 3 bits).
 //   f32     v_mfma 16x16x4 f32, A = 16 keys in order, exact products.
 // Query columns beyond the group's are zeros (a matrix instruction costs the
 // same with 1 or 16 queries, and the matrix cores are a quarter busy at most).
@@ -167,14 +170,13 @@ constexpr int PA_WAVES = 4;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 // The running maximum m is only raised when a score passes it by PA_SLACK (in
 // powers of two): then and only then the wavefront's lanes exchange their
-// maxima and scale what they hold.  The maximum's p is kept at LIFT: for f16
-// 2^10, so that the largest p, 2^15, fits and f16's smallest step is 2^-35 of
-// the maximum's weight or less; else 2^-30, so that sums of 2^25 values near
-// f32's largest stay in range (and values down to 2^-72 keep their bits).
+// maxima and scale what they hold.  The maximum's p is kept at LIFT: 2^-30 for
+// bf16 and f32, so that sums of 2^25 values near f32's largest stay in range
+// (and values down to 2^-72 keep their bits).
 constexpr float PA_SLACK = 5.0f;
 
 template <class E>
-struct PaTile;  // a tile's product: keys per tile and lane, parts of an f32 operand
+struct PaTile;  // keys per tile and lane, parts of an f32 operand, the two products
 
 template <class E>
 struct PaTile2 {
@@ -185,7 +187,7 @@ struct PaTile2 {
 template <>
 struct PaTile<F16> : PaTile2<F16> {
   static constexpr int PARTS = 2;
-  static constexpr float LIFT = 0x1p10f;
+  static constexpr float LIFT = 1.0f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -218,6 +220,47 @@ __device__ inline void pa_parts(const float (&x)[PaTile<E>::PER], typename PaTil
       const typename E::T t = E::round(rest);
       o[p][j] = t;
       rest -= (float)t;  // exact
+    }
+  }
+}
+
+// f16 values as sums of two bf16: the 8 leading bits and the 3 others
+__device__ inline void pa_split(PaTile<F16>::Op x, PaTile<BF16>::Op &hi, PaTile<BF16>::Op &lo) {
+  typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+  constexpr uint32_t HIGH = 0xFFFF0000u, HIGHS = 0x07060302u;  // v_perm: the upper halves of two registers
+  U4 a, b;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x0 = (float)x[2 * j], x1 = (float)x[2 * j + 1];
+    const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+    a[j] = __builtin_amdgcn_perm(u1, u0, HIGHS);
+    b[j] = __builtin_amdgcn_perm(__float_as_uint(x1 - __uint_as_float(u1 & HIGH)),
+                                 __float_as_uint(x0 - __uint_as_float(u0 & HIGH)), HIGHS);
+  }
+  hi = __builtin_bit_cast(PaTile<BF16>::Op, a), lo = __builtin_bit_cast(PaTile<BF16>::Op, b);
+}
+
+// o += p v for a tile's weights and 16 ND values.  f16: all six products of the
+// parts, so p v is as exact as in f32 at any size of p.  (In f16 parts, p at 2^10
+// of the maximum, a weight below 2^-13 of the maximum lost bits and one below
+// 2^-35 was nothing, though the sum had it; that took 0.7 to 1.6% less time, and
+// 6.3 us instead of 7.5 for 448 keys of 5 rows.  With the f32 matrix instruction
+// and v converted: 8.5, and 35 us instead of 32.4 for 48 rows of up to 1500 keys.)
+template <class E, int ND>
+__device__ inline void pa_add(const float (&p)[PaTile<E>::PER], const typename PaTile<E>::Op (&v)[ND], f4 (&o)[ND]) {
+  using W = PaTile<std::conditional_t<sizeof(typename E::T) == 2, BF16, E>>;
+  typename W::Op pf[W::PARTS];
+  pa_parts<std::conditional_t<sizeof(typename E::T) == 2, BF16, E>>(p, pf);
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    if constexpr (std::is_same_v<E, F16>) {
+      typename W::Op hi, lo;
+      pa_split(v[i], hi, lo);
+#pragma unroll
+      for (int k = W::PARTS - 1; k >= 0; --k) o[i] = W::mma(pf[k], lo, o[i]), o[i] = W::mma(pf[k], hi, o[i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < W::PARTS; ++k) o[i] = W::mma(pf[k], v[i], o[i]);
     }
   }
 }
@@ -399,12 +442,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
       x[j] = __builtin_amdgcn_exp2f(x[j] - base) * M::LIFT;
       sum += x[j];
     }
-    Op pf[PARTS];
-    pa_parts<E>(x, pf);
-#pragma unroll
-    for (int i = 0; i < ND; ++i)
-#pragma unroll
-      for (int k = 0; k < PARTS; ++k) o[i] = M::mma(pf[k], vf[i], o[i]);
+    pa_add<E>(x, vf, o);
     now = next;
   }
 

@@ -1,0 +1,60 @@
+"""Attention over pages where weights, queries or values are of very unlike
+size: what f32 arithmetic keeps, every type of pool keeps."""
+import numpy as np
+import pytest
+import torch
+
+from _paged import DTYPES, U, attend, gather, i32, pool, tables
+from rusty_whisper_amd import _abi as A
+
+pytestmark = pytest.mark.gpu
+
+PAGE, DIM = 32, 64
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _device():
+    A.init(0)
+    torch.cuda.init()
+
+
+def run(P, q, table, lens, group=1):
+    out = torch.full(q.shape, float("nan"), device="cuda")
+    A.paged_attention_dev(P, 0, q, q.shape[0], P.st.n_head * group, i32(table), i32(lens), int(max(lens)), out)
+    torch.cuda.synchronize()
+    return out.double().cpu().numpy().reshape(q.shape[0], -1, P.st.head_size)
+
+
+# ------------------------------------------------------- small weights
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("gap", [5.0, 14.0, 18.5, 20.0, 24.75, 40.0, 60.0])
+@pytest.mark.parametrize("n", [32, 448, 3000])
+def test_one_key_outweighs_the_others_and_has_no_value(dtype, gap, n):
+    """The result is the others' alone, whose weights are e^-gap of the largest.
+
+    q and k have one value each that is not zero, of 8 bits or fewer, so a score
+    is one exact product.  The exponential's argument, in powers of two, is
+    rounded four times at most (the constant twice, its product, the
+    difference): a weight is off by 4 (|s| + |largest s|) <= 8 (gap + 1) half
+    steps of itself, by 4 for the exponential; sums of n products and of n
+    weights by n each, the rest by 8."""
+    pages = -(-n // PAGE)
+    k, v = pool(dtype, 1, pages, 1, PAGE, DIM, seed=n)
+    rng = np.random.default_rng(n)
+    s = rng.integers(-32, 33, pages * PAGE) / 64.0
+    s[3] = gap
+    k.zero_()
+    k[0, :, 0, :, 0] = torch.from_numpy(s).cuda().reshape(pages, PAGE).to(k.dtype)
+    v[0, 0, 0, :, 3] = 0
+    q = torch.zeros(1, DIM, device="cuda")
+    q[0, 0] = 8.0  # scores are k's first value
+    table = np.arange(pages, dtype=np.int32)[None]
+    P = A.KvPages(k, v)
+    got = run(P, q, table, [n])[0, 0]
+    _, V = gather(k, v, 0, table[0], n)
+    p = np.exp(s[:n] - s[:n].max())
+    p /= p.sum()
+    tol = 2 * (8 * (gap + 1) + 12 + n) * U * (p @ np.abs(V[0]))
+    bad = np.abs(got - p @ V[0]) > tol
+    assert not bad.any(), (np.max(np.abs(got - p @ V[0]) / (p @ np.abs(V[0]))), np.max(tol / (p @ np.abs(V[0]))))
