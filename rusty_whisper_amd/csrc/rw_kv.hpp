@@ -150,9 +150,9 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
 // cores without LDS and without moves between lanes:
 //   2-byte  v_mfma 16x16x32, A = 16 keys: row r of half s is key
 //           8 (r / 4) + 4 s + r % 4, whose scores then lie in lane r / 4's
-//           registers 4 s + r % 4.  The f32 q enters as a sum of 2 f16 (22 bits)
-//           or 3 bf16 (24 bits), a product each; p as 3 bf16 for both types, as
-//           weights need f32's range, and f16's v as 2 bf16 (8 and 3 bits).
+//           registers 4 s + r % 4.  The f32 q enters as 3 parts of the pool's
+//           type, a product each; p as 3 bf16 for both types, as weights need
+//           f32's range, and f16's v as 2 bf16 (8 and 3 bits).
 //   f32     v_mfma 16x16x4 f32, A = 16 keys in order, exact products.
 // Query columns beyond the group's are zeros (a matrix instruction costs the
 // same with 1 or 16 queries, and the matrix cores are a quarter busy at most).
@@ -184,15 +184,21 @@ struct PaTile2 {
   typedef T Op __attribute__((ext_vector_type(8)));
   static constexpr int KEYS = 32, PER = 8, STEP = 32, SUB = 2;  // STEP: values of the head per k operand
 };
+// f16's range is short: each further part of an operand is MOVE times what is left,
+// and the parts' products have sums of their own (SUMS).  So q keeps 24 bits of
+// every value down to 2^-37 of the query's largest, and something of it down to
+// 2^-61.  (Two parts at one scale kept 22 bits down to 2^-18, nothing below 2^-40.)
 template <>
 struct PaTile<F16> : PaTile2<F16> {
-  static constexpr int PARTS = 2;
+  static constexpr int PARTS = 3, SUMS = 3;
+  static constexpr float MOVE = 0x1p11f;
   static constexpr float LIFT = 1.0f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct PaTile<BF16> : PaTile2<BF16> {
-  static constexpr int PARTS = 3;
+  static constexpr int PARTS = 3, SUMS = 1;
+  static constexpr float MOVE = 1.0f;
   static constexpr float LIFT = 0x1p-30f;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -200,7 +206,8 @@ template <>
 struct PaTile<F32> {
   using T = float;
   typedef f4 Op;
-  static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1;
+  static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1, SUMS = 1;
+  static constexpr float MOVE = 1.0f;
   static constexpr float LIFT = 0x1p-30f;
   static __device__ f4 mma(Op a, Op b, f4 c) {
 #pragma unroll
@@ -209,7 +216,7 @@ struct PaTile<F32> {
   }
 };
 
-// x as a sum of PARTS operands
+// x as a sum of PARTS operands, the p-th MOVE^p of its own size
 template <class E>
 __device__ inline void pa_parts(const float (&x)[PaTile<E>::PER], typename PaTile<E>::Op (&o)[PaTile<E>::PARTS]) {
 #pragma unroll
@@ -219,7 +226,7 @@ __device__ inline void pa_parts(const float (&x)[PaTile<E>::PER], typename PaTil
     for (int p = 0; p < PaTile<E>::PARTS; ++p) {
       const typename E::T t = E::round(rest);
       o[p][j] = t;
-      rest -= (float)t;  // exact
+      rest = (rest - (float)t) * PaTile<E>::MOVE;  // exact
     }
   }
 }
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
         for (int e = 0; e < 4; ++e) x[i][j + e] = r < gq ? y[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(x[i][j + e]));
       }
     int e = 0;
-    if (sizeof(T) == 2 && PARTS == 2) {
+    if (std::is_same_v<E, F16>) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
@@ -376,7 +383,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       Op o[PARTS];
-      if (PARTS == 2)
+      if (std::is_same_v<E, F16>)
 #pragma unroll
         for (int j = 0; j < PER; ++j) x[i][j] = ldexpf(x[i][j], -e);
       pa_parts<E>(x[i], o);
@@ -395,19 +402,26 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     const bool more = t + PA_WAVES < end;
     Where next{};
     if (more) next = where(t + PA_WAVES);
-    f4 s[SUB];
+    f4 s[M::SUMS][SUB];
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) s[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < M::SUMS; ++k)
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) s[k][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
       for (int k = 0; k < PARTS; ++k)
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) s[u] = M::mma(kf[u][i], qf[k][i], s[u]);
+        for (int u = 0; u < SUB; ++u) s[k % M::SUMS][u] = M::mma(kf[u][i], qf[k][i], s[k % M::SUMS][u]);
     if (more) load_k(t + PA_WAVES, next);
     float x[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = s[j >> 2][j & 3] * c;
+    for (int j = 0; j < PER; ++j) {
+      x[j] = s[M::SUMS - 1][j >> 2][j & 3];
+#pragma unroll
+      for (int k = M::SUMS - 2; k >= 0; --k) x[j] = fmaf(x[j], 1.0f / M::MOVE, s[k][j >> 2][j & 3]);
+      x[j] *= c;
+    }
     // keys behind the length, or in a page outside the pool, have no weight,
     // and what v holds there (anything) is taken as zero
     if ((t + 1) * KEYS > n || now.bad0 || now.bad1) {

@@ -58,3 +58,27 @@ def test_one_key_outweighs_the_others_and_has_no_value(dtype, gap, n):
     tol = 2 * (8 * (gap + 1) + 12 + n) * U * (p @ np.abs(V[0]))
     bad = np.abs(got - p @ V[0]) > tol
     assert not bad.any(), (np.max(np.abs(got - p @ V[0]) / (p @ np.abs(V[0]))), np.max(tol / (p @ np.abs(V[0]))))
+
+
+# ------------------------------------------- values of unlike size in q
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("power", [0, 14, 22, 30, 36])
+def test_a_large_value_of_q_that_meets_zeros(dtype, group, power):
+    """q's first value is 2^power, all of k's first values are 0: the scores are
+    the other values' (`attend`'s bound takes sum |q k|)."""
+    lens = [1, 33, 700, 3000]
+    n_pages = sum(-(-n // PAGE) for n in lens)
+    k, v = pool(dtype, 1, n_pages, 2, PAGE, DIM, seed=power)
+    k[..., 0] = 0
+    q = torch.randn(4, 2 * group, DIM, device="cuda") * 2
+    q[..., 0] = 2.0**power
+    q = q.reshape(4, -1)
+    table = tables(lens, PAGE, n_pages, seed=power)
+    P = A.KvPages(k, v)
+    got = run(P, q, table, lens, group)
+    for r, n in enumerate(lens):
+        want, tol = attend(q[r].double().cpu().numpy().reshape(-1, DIM), *gather(k, v, 0, table[r, : -(-n // PAGE)], n))
+        bad = np.abs(got[r] - want) > tol
+        assert not bad.any(), (r, np.max(np.abs(got[r] - want)), np.max(tol))
