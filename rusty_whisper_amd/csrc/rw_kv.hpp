@@ -170,10 +170,16 @@ constexpr int PA_WAVES = 4;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 // The running maximum m is only raised when a score passes it by PA_SLACK (in
 // powers of two): then and only then the wavefront's lanes exchange their
-// maxima and scale what they hold.  The maximum's p is kept at LIFT: 2^-30 for
-// bf16 and f32, so that sums of 2^25 values near f32's largest stay in range
-// (and values down to 2^-72 keep their bits).
+// maxima and scale what they hold.  So p is at most 2^5, the maximum's at least
+// 1, and a wavefront's sum l of them at least 1.
+//   What a wavefront, a chunk hands on is its mean of v, sum p v / l, with m and
+// l: means of finite values are finite, and weighted means of means too.  Only a
+// wavefront's own sum p v can pass f32's range, of bf16 or f32 values near its
+// end (WIDE): where a mean comes out infinite or NaN, the wavefront goes over its keys
+// again with p at PA_LOW, and takes those means from there.  (Weights of 2^-30
+// in the first place lost values below 2^-72, and p below 2^-96.)
 constexpr float PA_SLACK = 5.0f;
+constexpr float PA_LOW = 0x1p-40f;  // sums of 2^35 values stay in range
 
 template <class E>
 struct PaTile;  // keys per tile and lane, parts of an f32 operand, the two products
@@ -192,14 +198,14 @@ template <>
 struct PaTile<F16> : PaTile2<F16> {
   static constexpr int PARTS = 3, SUMS = 3;
   static constexpr float MOVE = 0x1p11f;
-  static constexpr float LIFT = 1.0f;
+  static constexpr bool WIDE = false;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct PaTile<BF16> : PaTile2<BF16> {
   static constexpr int PARTS = 3, SUMS = 1;
   static constexpr float MOVE = 1.0f;
-  static constexpr float LIFT = 0x1p-30f;
+  static constexpr bool WIDE = true;
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -208,7 +214,7 @@ struct PaTile<F32> {
   typedef f4 Op;
   static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1, SUMS = 1;
   static constexpr float MOVE = 1.0f;
-  static constexpr float LIFT = 0x1p-30f;
+  static constexpr bool WIDE = true;
   static __device__ f4 mma(Op a, Op b, f4 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -270,6 +276,11 @@ __device__ inline void pa_add(const float (&p)[PaTile<E>::PER], const typename P
       for (int k = 0; k < W::PARTS; ++k) o[i] = W::mma(pf[k], v[i], o[i]);
     }
   }
+}
+
+// a mean of finite values: rounded past f32's largest, it is that
+__device__ inline float pa_mean(float x) {
+  return __builtin_isinf(x) ? __builtin_copysignf(__FLT_MAX__, x) : x;
 }
 
 // exp2(x) for x <= 0 or -inf against a maximum that may be -inf itself
@@ -354,7 +365,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     for (int i = 0; i < ND; ++i) vf[i] = *(const Op *)(p + ((16 * i) << pr));
   };
 
-  int t = k0 / KEYS + wv;
+  const int t0 = k0 / KEYS + wv;
+  int t = t0;
   Where now{};
   if (t < end) now = where(t), load_k(t, now);
 
@@ -392,112 +404,126 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     }
   }
 
-  f4 o[ND];
+  for (float scale = 1.0f;; scale = PA_LOW) {
+    f4 o[ND];
 #pragma unroll
-  for (int i = 0; i < ND; ++i) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = NEG_INF, sum = 0.0f;  // query r's; sum: of this lane's keys
+    for (int i = 0; i < ND; ++i) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = NEG_INF, sum = 0.0f;  // query r's; sum: of this lane's keys
 
-  for (; t < end; t += PA_WAVES) {
-    load_v(t, now);
-    const bool more = t + PA_WAVES < end;
-    Where next{};
-    if (more) next = where(t + PA_WAVES);
-    f4 s[M::SUMS][SUB];
+    for (; t < end; t += PA_WAVES) {
+      load_v(t, now);
+      const bool more = t + PA_WAVES < end;
+      Where next{};
+      if (more) next = where(t + PA_WAVES);
+      f4 s[M::SUMS][SUB];
 #pragma unroll
-    for (int k = 0; k < M::SUMS; ++k)
+      for (int k = 0; k < M::SUMS; ++k)
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) s[k][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < SUB; ++u) s[k][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+      for (int i = 0; i < NC; ++i)
 #pragma unroll
-      for (int k = 0; k < PARTS; ++k)
+        for (int k = 0; k < PARTS; ++k)
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) s[k % M::SUMS][u] = M::mma(kf[u][i], qf[k][i], s[k % M::SUMS][u]);
-    if (more) load_k(t + PA_WAVES, next);
-    float x[PER];
+          for (int u = 0; u < SUB; ++u) s[k % M::SUMS][u] = M::mma(kf[u][i], qf[k][i], s[k % M::SUMS][u]);
+      if (more) load_k(t + PA_WAVES, next);
+      float x[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      x[j] = s[M::SUMS - 1][j >> 2][j & 3];
+      for (int j = 0; j < PER; ++j) {
+        x[j] = s[M::SUMS - 1][j >> 2][j & 3];
 #pragma unroll
-      for (int k = M::SUMS - 2; k >= 0; --k) x[j] = fmaf(x[j], 1.0f / M::MOVE, s[k][j >> 2][j & 3]);
-      x[j] *= c;
+        for (int k = M::SUMS - 2; k >= 0; --k) x[j] = fmaf(x[j], 1.0f / M::MOVE, s[k][j >> 2][j & 3]);
+        x[j] *= c;
+      }
+      // keys behind the length, or in a page outside the pool, have no weight,
+      // and what v holds there (anything) is taken as zero
+      if ((t + 1) * KEYS > n || now.bad0 || now.bad1) {
+        const bool bad = KEYS > 16 && h >= 2 ? now.bad1 : now.bad0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (bad || t * KEYS + PER * h + j >= n) {
+            x[j] = NEG_INF;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) vf[i][j] = (T)0.0f;
+          }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < PER; ++j) top = fmaxf(top, x[j]);
+      if (__builtin_amdgcn_ballot_w64(top > m + PA_SLACK)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float up = fmaxf(m, top), f = pa_weight(m, up);
+        m = up;
+        sum *= f;
+        f4 fr;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i] *= fr;
+      }
+      const float base = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        x[j] = __builtin_amdgcn_exp2f(x[j] - base);
+        if (M::WIDE) x[j] *= scale;
+        sum += x[j];
+      }
+      pa_add<E>(x, vf, o);
+      now = next;
     }
-    // keys behind the length, or in a page outside the pool, have no weight,
-    // and what v holds there (anything) is taken as zero
-    if ((t + 1) * KEYS > n || now.bad0 || now.bad1) {
-      const bool bad = KEYS > 16 && h >= 2 ? now.bad1 : now.bad0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (bad || t * KEYS + PER * h + j >= n) {
-          x[j] = NEG_INF;
-#pragma unroll
-          for (int i = 0; i < ND; ++i) vf[i][j] = (T)0.0f;
-        }
-    }
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < PER; ++j) top = fmaxf(top, x[j]);
-    if (__builtin_amdgcn_ballot_w64(top > m + PA_SLACK)) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float up = fmaxf(m, top), f = pa_weight(m, up);
-      m = up;
-      sum *= f;
-      f4 fr;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) o[i] *= fr;
-    }
-    const float base = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      // (x - m keeps all its bits where p is large; LIFT in the exponent cost some)
-      x[j] = __builtin_amdgcn_exp2f(x[j] - base) * M::LIFT;
-      sum += x[j];
-    }
-    pa_add<E>(x, vf, o);
-    now = next;
-  }
 
-  // the wavefronts' runs: scaled to the largest maximum, summed
-  sum += __shfl_xor(sum, 16);
-  sum += __shfl_xor(sum, 32);
-  if (h == 0) sm[wv][r] = m, sl[wv][r] = sum;
-  __syncthreads();
+    // the wavefront's means
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    const bool first = scale == 1.0f;
+    if (first && h == 0) sm[wv][r] = m, sl[wv][r] = sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // 0: no keys
+    bool over = false;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int qr = 4 * h + i;
-    if (qr >= gq) break;
-    float top = sm[0][qr];
+    for (int i = 0; i < 4; ++i) {
+      const int qr = 4 * h + i;
+      const float f = __shfl(inv, qr);
 #pragma unroll
-    for (int k = 1; k < PA_WAVES; ++k) top = fmaxf(top, sm[k][qr]);
-    const float f = pa_weight(sm[wv][qr], top);
-#pragma unroll
-    for (int d = 0; d < ND; ++d) so[wv][qr][16 * d + r] = o[d][i] * f;
+      for (int d = 0; d < ND; ++d) {
+        const float y = o[d][i] * f;
+        float &mean = so[wv][qr][16 * d + r];
+        if (!M::WIDE || first) mean = y;
+        else if (!__builtin_isfinite(mean)) mean = pa_mean(y);
+        over |= qr < gq && !__builtin_isfinite(y);
+      }
+    }
+    if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
+    t = t0;
+    if (t < end) now = where(t), load_k(t, now);
   }
   __syncthreads();
+
+  // the wavefronts' means, each with its share of the weights
   const int64_t runs = (int64_t)rows * heads * gridDim.y;
   for (int i = threadIdx.x; i < gq * DH; i += 64 * PA_WAVES) {
     const int qr = i / DH, d = i % DH;
-    float top = sm[0][qr], l = 0.0f, y = 0.0f;
+    float top = sm[0][qr], l = 0.0f, y = 0.0f, w[PA_WAVES];
 #pragma unroll
     for (int k = 1; k < PA_WAVES; ++k) top = fmaxf(top, sm[k][qr]);
 #pragma unroll
-    for (int k = 0; k < PA_WAVES; ++k) l += sl[k][qr] * pa_weight(sm[k][qr], top), y += so[k][qr][d];
+    for (int k = 0; k < PA_WAVES; ++k) l += w[k] = sl[k][qr] * pa_weight(sm[k][qr], top);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: no page of the row is in the pool
+#pragma unroll
+    for (int k = 0; k < PA_WAVES; ++k) y += so[k][qr][d] * (w[k] * inv);
     if (direct) {
-      orow[i] = l == 0.0f ? 0.0f : y / l;  // 0: no page of the row is in the pool
+      orow[i] = pa_mean(y);
     } else {
       const int64_t run = ((int64_t)row * heads + hq + qr) * gridDim.y + blockIdx.y;
-      part[run * DH + d] = y;
+      part[run * DH + d] = pa_mean(y);
       if (d == 0) part[runs * DH + 2 * run] = top, part[runs * DH + 2 * run + 1] = l;
     }
   }
 }
 
-// The chunks of one (row, query head): out = sum_z o_z 2^(m_z - m) / sum_z l_z
-// 2^(m_z - m).  A row of one chunk was written by k_paged_attn.  The chunks'
-// weights go to LDS; then SIDE groups of threads, four values each, sum every
+// The chunks of one (row, query head): out = sum_z y_z w_z / sum_z w_z of their
+// means y_z, w_z = l_z 2^(m_z - m).  A row of one chunk was written by
+// k_paged_attn.  The chunks' weights go to LDS; then SIDE groups of threads, four values each, sum every
 // SIDE-th chunk in order, and the groups' sums are added in order.
 constexpr int PA_MAX_SPLIT = 1024;
 template <int DH>
@@ -519,19 +545,21 @@ __global__ __launch_bounds__(256) void k_paged_join(const float *__restrict__ pa
   for (int z = threadIdx.x & 63; z < nz; z += 64) top = fmaxf(top, ml[2 * z]);
   for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
   for (int z = threadIdx.x; z < nz; z += 256) {
-    const float w = pa_weight(ml[2 * z], top);
+    const float w = ml[2 * z + 1] * pa_weight(ml[2 * z], top);
     sw[z] = w;
-    l += ml[2 * z + 1] * w;
+    l += w;
   }
   for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
   if ((threadIdx.x & 63) == 0) sl[threadIdx.x >> 6] = l;
   __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int g = threadIdx.x / W, d = threadIdx.x % W;
   if (d < DH / 4) {
     f4 y{0.0f, 0.0f, 0.0f, 0.0f};
     const f4 *o = (const f4 *)(part + run0 * DH) + d;
 #pragma unroll 4
-    for (int z = g; z < nz; z += SIDE) y += o[z * (DH / 4)] * sw[z];
+    for (int z = g; z < nz; z += SIDE) y += o[z * (DH / 4)] * (sw[z] * inv);
     sy[g][d] = y;
   }
   __syncthreads();
@@ -539,8 +567,7 @@ __global__ __launch_bounds__(256) void k_paged_join(const float *__restrict__ pa
     float y = 0.0f;
 #pragma unroll
     for (int i = 0; i < SIDE; ++i) y += ((const float *)sy[i])[threadIdx.x];
-    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    out[row * ldo + (int64_t)hq * DH + threadIdx.x] = l == 0.0f ? 0.0f : y / l;
+    out[row * ldo + (int64_t)hq * DH + threadIdx.x] = pa_mean(y);
   }
 }
 
