@@ -199,6 +199,7 @@ struct PaTile<F16> : PaTile2<F16> {
   static constexpr int PARTS = 3, SUMS = 3;
   static constexpr float MOVE = 0x1p11f;
   static constexpr bool WIDE = false;
+  static __device__ T part(float x) { return F16::round(x); }
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -206,6 +207,9 @@ struct PaTile<BF16> : PaTile2<BF16> {
   static constexpr int PARTS = 3, SUMS = 1;
   static constexpr float MOVE = 1.0f;
   static constexpr bool WIDE = true;
+  // x's 8 leading bits: three parts are all of f32's 24, and none is beyond the
+  // type's largest (which a rounded one is for x above 3.39e38)
+  static __device__ T part(float x) { return __builtin_bit_cast(T, (uint16_t)(__float_as_uint(x) >> 16)); }
   static __device__ f4 mma(Op a, Op b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -215,6 +219,7 @@ struct PaTile<F32> {
   static constexpr int KEYS = 16, PER = 4, STEP = 16, SUB = 1, PARTS = 1, SUMS = 1;
   static constexpr float MOVE = 1.0f;
   static constexpr bool WIDE = true;
+  static __device__ T part(float x) { return x; }
   static __device__ f4 mma(Op a, Op b, f4 c) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -230,7 +235,7 @@ __device__ inline void pa_parts(const float (&x)[PaTile<E>::PER], typename PaTil
     float rest = x[j];
 #pragma unroll
     for (int p = 0; p < PaTile<E>::PARTS; ++p) {
-      const typename E::T t = E::round(rest);
+      const typename E::T t = PaTile<E>::part(rest);
       o[p][j] = t;
       rest = (rest - (float)t) * PaTile<E>::MOVE;  // exact
     }

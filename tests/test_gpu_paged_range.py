@@ -142,3 +142,30 @@ def test_largest_and_small_values_in_one_head(dtype, n):
     want, tol = attend(q[0].double().cpu().numpy().reshape(-1, DIM), *gather(k, v, 0, table[0], n))
     bad = ~(np.abs(got - want) <= tol + subnormal(n))
     assert not bad.any(), (np.argwhere(bad)[:4], got[bad][:4], want[bad][:4])
+
+
+# ------------------------------------------------- the largest queries
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("q0", [torch.finfo(torch.float32).max, -torch.finfo(torch.float32).max, 3.39e38, 3.3953e38])
+def test_queries_at_the_end_of_f32(dtype, q0):
+    """One value of q and k is not zero; scores are about -32 .. 32 (f16, whose
+    smallest value is 2^-24: of 2^101, the largest take all).  Tolerance as for
+    the first test here, with scores for the gap."""
+    n = 448
+    pages = n // PAGE
+    k, v = pool(dtype, 1, pages, 1, PAGE, DIM, seed=3)
+    k0 = np.random.default_rng(3).integers(-32, 33, n) * 2.0 ** (-24 if dtype == "f16" else -125)
+    k.zero_()
+    k[0, :, 0, :, 0] = torch.from_numpy(k0).cuda().reshape(pages, PAGE).to(k.dtype)
+    q = torch.zeros(1, DIM, device="cuda")
+    q[0, 0] = q0
+    table = np.arange(pages, dtype=np.int32)[None]
+    P = A.KvPages(k, v)
+    got = run(P, q, table, [n])[0, 0]
+    _, V = gather(k, v, 0, table[0], n)
+    s = float(q[0, 0]) * k0 / 8.0
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    tol = 2 * (8 * 33 + 12 + n) * U * (p @ np.abs(V[0]))
+    assert np.all(np.abs(got - p @ V[0]) <= tol), (got[:4], (p @ V[0])[:4])
