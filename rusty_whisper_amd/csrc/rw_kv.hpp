@@ -261,9 +261,10 @@ __device__ inline void pa_split(PaTile<F16>::Op x, PaTile<BF16>::Op &hi, PaTile<
 // o += p v for a tile's weights and 16 ND values.  f16: all six products of the
 // parts, so p v is as exact as in f32 at any size of p.  (In f16 parts, p at 2^10
 // of the maximum, a weight below 2^-13 of the maximum lost bits and one below
-// 2^-35 was nothing, though the sum had it; that took 0.7 to 1.6% less time, and
-// 6.3 us instead of 7.5 for 448 keys of 5 rows.  With the f32 matrix instruction
-// and v converted: 8.5, and 35 us instead of 32.4 for 48 rows of up to 1500 keys.)
+// 2^-35 was nothing, though the sum had it: 162 us for 61 rows of up to 8190 keys,
+// 8 heads of 128 with 4 query heads each, now 164; 16000 keys of 8 rows with 20
+// query heads each, 126 and 136.  The f32 matrix instruction on converted v
+// takes 170 and 145.)
 template <class E, int ND>
 __device__ inline void pa_add(const float (&p)[PaTile<E>::PER], const typename PaTile<E>::Op (&v)[ND], f4 (&o)[ND]) {
   using W = PaTile<std::conditional_t<sizeof(typename E::T) == 2, BF16, E>>;
@@ -293,7 +294,13 @@ __device__ inline float pa_weight(float m, float top) {
   return m == -__builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
 }
 
-template <class E, int DH>
+// ONE: a key head of one query head, which stands in all 16 columns, so that every
+// lane has the weights of its keys and multiplies them with its v in f32, 8 fused
+// multiply-adds per 16 values (o: of value 16 i + r, this lane's keys).  For f16,
+// where the other form splits v: 448 keys of 5 rows, 20 heads of 64: 6.4 us against
+// 7.8; 48 rows of up to 1500: 31.3 and 33; 300 rows of up to 700, 4 heads of 32: 11.6
+// and 14.9; 61 rows of up to 8190, 8 heads of 128: 156 and 158.
+template <class E, int DH, bool ONE>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     const void *__restrict__ kp, const void *__restrict__ vp, const float *__restrict__ q, const int32_t *__restrict__ table,
     const int32_t *__restrict__ seq, const int32_t *__restrict__ lens, float *__restrict__ out, float *__restrict__ part,
@@ -388,7 +395,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
       for (int j = 0; j < PER; j += 4) {
         const f4 y = *(const f4 *)(p + M::STEP * i + j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][j + e] = r < gq ? y[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(x[i][j + e]));
+        for (int e = 0; e < 4; ++e) x[i][j + e] = ONE || r < gq ? y[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(x[i][j + e]));
       }
     int e = 0;
     if (std::is_same_v<E, F16>) {
@@ -410,9 +417,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
   }
 
   for (float scale = 1.0f;; scale = PA_LOW) {
-    f4 o[ND];
+    std::conditional_t<ONE, float, f4> o[ND];
 #pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < ND; ++i) o[i] = {};
     float m = NEG_INF, sum = 0.0f;  // query r's; sum: of this lane's keys
 
     for (; t < end; t += PA_WAVES) {
@@ -461,9 +468,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
         const float up = fmaxf(m, top), f = pa_weight(m, up);
         m = up;
         sum *= f;
-        f4 fr;
+        std::conditional_t<ONE, float, f4> fr;
+        if constexpr (ONE) fr = f;
+        else
 #pragma unroll
-        for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
+          for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[i] *= fr;
       }
@@ -474,7 +483,14 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
         if (M::WIDE) x[j] *= scale;
         sum += x[j];
       }
-      pa_add<E>(x, vf, o);
+      if constexpr (ONE) {
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int j = 0; j < PER; ++j) o[i] = fmaf(x[j], (float)vf[i][j], o[i]);
+      } else {
+        pa_add<E>(x, vf, o);
+      }
       now = next;
     }
 
@@ -484,23 +500,33 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     const bool first = scale == 1.0f;
     if (first && h == 0) sm[wv][r] = m, sl[wv][r] = sum;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // 0: no keys
-    bool over = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int qr = 4 * h + i;
-      const float f = __shfl(inv, qr);
+    if constexpr (ONE) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const float y = o[d][i] * f;
-        float &mean = so[wv][qr][16 * d + r];
-        if (!M::WIDE || first) mean = y;
-        else if (!__builtin_isfinite(mean)) mean = pa_mean(y);
-        over |= qr < gq && !__builtin_isfinite(y);
+        o[d] += __shfl_xor(o[d], 16);
+        o[d] += __shfl_xor(o[d], 32);
+        if (h == 0) so[wv][0][16 * d + r] = o[d] * inv;
       }
+      break;
+    } else {
+      bool over = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int qr = 4 * h + i;
+        const float f = __shfl(inv, qr);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const float y = o[d][i] * f;
+          float &mean = so[wv][qr][16 * d + r];
+          if (!M::WIDE || first) mean = y;
+          else if (!__builtin_isfinite(mean)) mean = pa_mean(y);
+          over |= qr < gq && !__builtin_isfinite(y);
+        }
+      }
+      if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
+      t = t0;
+      if (t < end) now = where(t), load_k(t, now);
     }
-    if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
-    t = t0;
-    if (t < end) now = where(t), load_k(t, now);
   }
   __syncthreads();
 

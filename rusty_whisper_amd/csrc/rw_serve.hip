@@ -187,8 +187,11 @@ static int launch_paged(const PagedCall &c, const PagedPlan &L, hipStream_t s) {
   const int group = c.n_head / w.heads;
   const size_t items = (size_t)c.rows * w.heads;
   const dim3 grid((unsigned)(cdiv(items, 8) * 8 * cdiv(group, 16)), (unsigned)L.nsplit);
-  hipLaunchKernelGGL((k_paged_attn<E, DH>), grid, dim3(64 * PA_WAVES), 0, s, w.k, w.v, c.q, w.table, w.seq, c.len, c.out,
-                     c.part, c.rows, w.heads, group, w.pr, w.n_pages, w.n_seqs, w.ld, c.ldq, c.ldo, c.max_len, L.chunk);
+  auto *kernel = k_paged_attn<E, DH, false>;
+  if constexpr (std::is_same_v<E, F16>)
+    if (group == 1) kernel = k_paged_attn<E, DH, true>;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * PA_WAVES), 0, s, w.k, w.v, c.q, w.table, w.seq, c.len, c.out, c.part,
+                     c.rows, w.heads, group, w.pr, w.n_pages, w.n_seqs, w.ld, c.ldq, c.ldo, c.max_len, L.chunk);
   SERVE_TRY(launched("k_paged_attn"));
   if (L.nsplit == 1) return RW_OK;
   hipLaunchKernelGGL((k_paged_join<DH>), dim3((unsigned)(c.rows * c.n_head)), dim3(256), 0, s, c.part, w.seq, c.len,
