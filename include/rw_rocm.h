@@ -38,9 +38,9 @@
  * transcription threads, src/transcribe.rs:1525-1552).  Host-pointer entries
  * are synchronous.  Device-pointer entries are asynchronous on the stream
  * passed in; called without a workspace they use one buffer of the
- * library's per (device, stream), which a call holds until its launches are
- * queued, so concurrent calls on one stream queue one after the other and
- * never share it.  Calls that pass one caller workspace race on it unless
+ * library's per (device, stream) -- hipStreamPerThread: per thread, as is
+ * the stream --, which a call holds until its launches are queued, so
+ * concurrent calls on one stream queue one after the other and never share it.  Calls that pass one caller workspace race on it unless
  * the caller orders them.  An rw_decoder is one decoding state: its calls
  * must not overlap.
  */

@@ -10,19 +10,67 @@
 //     launches over one buffer: the second queues after the first is done,
 //     and the stream runs them in that order.
 // Callers on different streams use different buffers and never wait for
-// each other.  A replaced buffer is freed through the pool's free function
+// each other.  One handle means another stream in every thread (HIP's per-thread
+// default stream); its key holds the thread's number (ThreadNumber), and
+// collect() frees the buffers of threads that have ended.  A replaced buffer is freed through the pool's free function
 // (hipFree, which waits for the device's queued work first).
 //
 // Host-only C++ (no HIP types), so the logic is tested on the CPU with a
 // plain allocator under ThreadSanitizer.
 #pragma once
 #include <stddef.h>
+#include <stdint.h>
 
 #include <map>
 #include <memory>
 #include <mutex>
+#include <vector>
 
 namespace rw {
+
+// Numbers of threads, from 1 on.  None is given twice (a std::thread::id may be, while
+// work of the thread that had it before is still queued).
+class ThreadNumber {
+ public:
+  static uint64_t mine() {
+    static thread_local uint64_t number = 0;
+    static thread_local AtEnd at_end;
+    if (!number) {
+      std::lock_guard<std::mutex> lk(all().mu);
+      number = at_end.number = ++all().last;
+    }
+    return number;
+  }
+  // the threads that have ended since the last call
+  static std::vector<uint64_t> take_ended() {
+    std::vector<uint64_t> out;
+    std::lock_guard<std::mutex> lk(all().mu);
+    out.swap(all().ended);
+    return out;
+  }
+
+ private:
+  struct All {
+    std::mutex mu;
+    uint64_t last = 0;
+    std::vector<uint64_t> ended;
+  };
+  static All &all() {
+    static All *a = new All;  // threads may end after static objects do
+    return *a;
+  }
+  struct AtEnd {
+    uint64_t number = 0;
+    ~AtEnd() {
+      if (!number) return;
+      std::lock_guard<std::mutex> lk(all().mu);
+      try {
+        all().ended.push_back(number);
+      } catch (...) {  // no memory: its buffers are kept
+      }
+    }
+  };
+};
 
 template <class Key>
 class WorkspacePool {
@@ -75,6 +123,21 @@ class WorkspacePool {
   }
 
   void release(Slot *s) { s->hold.unlock(); }
+
+  // frees the buffers of the keys for which `ended(key)` holds: nobody holds or
+  // asks for them any more
+  template <class F>
+  void collect(F ended) {
+    std::lock_guard<std::mutex> lk(map_mu_);
+    for (auto it = slots_.begin(); it != slots_.end();) {
+      if (!ended(it->first)) {
+        ++it;
+        continue;
+      }
+      if (it->second->p) free_(it->second->p);
+      it = slots_.erase(it);
+    }
+  }
 
  private:
   AllocFn alloc_;

@@ -252,7 +252,14 @@ struct CtxGuard {
 // launches are queued (rw_pool.hpp): no other thread frees or grows it
 // meanwhile, and launches of two threads on one stream never interleave
 // over it.
-using StreamKey = std::pair<int, void *>;
+struct StreamKey {
+  int device;
+  void *stream;
+  uint64_t thread;  // hipStreamPerThread: whose, else 0
+  bool operator<(const StreamKey &o) const {
+    return std::tie(device, stream, thread) < std::tie(o.device, o.stream, o.thread);
+  }
+};
 using WsPool = WorkspacePool<StreamKey>;
 using WsHold = HoldWs<WsPool>;
 
@@ -271,7 +278,14 @@ static WsPool &ws_pool() {
 
 static int stream_workspace(int device, void *stream, size_t bytes, WsHold &hold, void **out) {
   WsPool::Slot *slot = nullptr;
-  if (ws_pool().acquire(std::make_pair(device, stream), bytes, &slot))
+  StreamKey key{device, stream, 0};
+  if (stream == (void *)hipStreamPerThread) {
+    key.thread = ThreadNumber::mine();
+    const std::vector<uint64_t> ended = ThreadNumber::take_ended();
+    if (!ended.empty())
+      ws_pool().collect([&](const StreamKey &k) { return std::find(ended.begin(), ended.end(), k.thread) != ended.end(); });
+  }
+  if (ws_pool().acquire(key, bytes, &slot))
     return fail(RW_ENOMEM, "hipMalloc(%zu) for a stream workspace failed", bytes);
   hold.pool = &ws_pool();
   hold.slot = slot;
