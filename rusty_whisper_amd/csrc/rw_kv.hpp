@@ -556,7 +556,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
 // means y_z, w_z = l_z 2^(m_z - m).  A row of one chunk was written by
 // k_paged_attn.  The chunks' weights go to LDS; then SIDE groups of threads, four values each, sum every
 // SIDE-th chunk in order, and the groups' sums are added in order.
-constexpr int PA_MAX_SPLIT = 1024;
+constexpr int PA_MAX_SPLIT = 512;  // chunks of a row at most: one row alone, two workgroups per CU
 template <int DH>
 __global__ __launch_bounds__(256) void k_paged_join(const float *__restrict__ part, const int32_t *__restrict__ seq,
                                                     const int32_t *__restrict__ lens, int n_seqs, int64_t most,

@@ -155,10 +155,10 @@ static PagedPlan paged_plan(const rw_kv_pages *p, size_t rows, int n_head, size_
   const size_t bytes = max_len * 2 * p->head_size * elem_size(p->dtype);
   size_t nsplit = 1;
   if (bytes > (size_t)256 << 10) {
-    nsplit = std::min(cdiv(bytes, (size_t)128 << 10), 512 / L.base);
+    nsplit = std::min(cdiv(bytes, (size_t)128 << 10), (size_t)PA_MAX_SPLIT / L.base);
     if (rows > 1)
       nsplit = std::max(nsplit, std::min(cdiv(bytes, (size_t)192 << 10), std::min((size_t)4096, 256 * rows) / L.base));
-    nsplit = std::max((size_t)1, std::min(nsplit, (size_t)PA_MAX_SPLIT));
+    nsplit = std::max((size_t)1, nsplit);  // <= PA_MAX_SPLIT: base is no less than rows
   }
   L.most = nsplit;
   L.chunk = (int)(cdiv(std::max(max_len, (size_t)1), nsplit * 128) * 128);
