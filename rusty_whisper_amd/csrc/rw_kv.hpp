@@ -69,7 +69,7 @@ constexpr int KV_ROWS = 32, KV_COLS = 64;
 template <class E>
 __global__ __launch_bounds__(256) void k_kv_write(PagedView w, const float *__restrict__ k, int64_t ldk,
                                                   const float *__restrict__ v, int64_t ldv, int rows,
-                                                  const int32_t *__restrict__ pos, int col_tiles, int tiles) {
+                                                  const int32_t *__restrict__ pos, int col_tiles, int tiles, int row0) {
   using T = typename E::T;
   typedef T Out __attribute__((ext_vector_type(8)));
   __shared__ T sv[KV_COLS][KV_ROWS + 2];
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(256) void k_kv_write(PagedView w, const float *__re
   const int tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);  // gridDim.x: a multiple of 8
   if (tile >= tiles) return;
   const int n = w.heads * w.dim, P = 1 << w.pr, t = threadIdx.x;
-  const int r0 = tile / col_tiles * KV_ROWS, c0 = tile % col_tiles * KV_COLS;
+  const int r0 = row0 + tile / col_tiles * KV_ROWS, c0 = tile % col_tiles * KV_COLS;
   if (t < KV_ROWS) {
     int64_t at = -1;
     if (r0 + t < rows) {

@@ -347,15 +347,18 @@ int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k,
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
   const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
-  const size_t tiles = cdiv(rows, KV_ROWS) * cdiv(n, KV_COLS);
-  if (tiles > MOST_ROWS) return fail(RW_EINVAL, "%zu rows of %zu values", rows, n);
-  const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
+  const size_t cols = cdiv(n, KV_COLS), most = MOST_ROWS / cols * KV_ROWS;  // rows of one launch
+  for (size_t row0 = 0; row0 < rows; row0 += most) {
+    const size_t tiles = cdiv(std::min(most, rows - row0), KV_ROWS) * cols;
+    const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
 #define RW_WRITE(E)                                                                                                \
   hipLaunchKernelGGL((k_kv_write<E>), grid, dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v, (int64_t)ldv, \
-                     (int)rows, pos, (int)cdiv(n, KV_COLS), (int)tiles)
-  BY_TYPE(pages->dtype, RW_WRITE);
+                     (int)rows, pos, (int)cols, (int)tiles, (int)row0)
+    BY_TYPE(pages->dtype, RW_WRITE);
 #undef RW_WRITE
-  return launched("k_kv_write");
+    SERVE_TRY(launched("k_kv_write"));
+  }
+  return RW_OK;
 }
 
 // every id in the pool, no dst twice, no dst a src

@@ -63,3 +63,27 @@ def test_scores_of_64_parts_of_more_than_64_steps():
             assert np.isnan(got) if t >= n else abs(got - (d[t] - np.log(S))) <= tol[t]
         H = np.log(S) - T / S
         assert abs(float(ent[r]) - H) <= 2 * share * (1 + abs(T) / S) + 3 * U * (np.log(S) + abs(T) / S)
+
+
+def test_a_write_of_more_rows_than_one_launch_takes():
+    """2^21 + 33 rows of 8192 values (2^23 + 256 tiles), few of which have a
+    place: around the end of the first launch and at both ends."""
+    heads, dim, page, rows = 64, 128, 16, 2**21 + 33
+    n = heads * dim
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 69 GB for the rows")
+    x = torch.empty(rows, n, device="cuda")
+    at = [0, 1, 31, 32, 2**21 - 32, 2**21 - 1, 2**21, 2**21 + 1, 2**21 + 31, 2**21 + 32]
+    k, v = pool("f32", 1, 1, heads, page, dim, seed=0, fill=-3.0)
+    pos = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    for i, r in enumerate(at):
+        x[r] = torch.arange(n, device="cuda") + i * 2**-8
+        pos[r] = i
+    A.kv_write_dev(A.KvPages(k, v), 0, x, x, rows, i32([[0]]), pos, seq=torch.zeros_like(pos))
+    torch.cuda.synchronize()
+    for i, r in enumerate(at):
+        want = x[r].reshape(heads, dim)
+        assert torch.equal(k[0, 0, :, i], want) and torch.equal(v[0, 0, :, :, i], want), r
+    assert torch.all(k[0, 0, :, len(at):] == -3) and torch.all(v[0, 0, :, :, len(at):] == -3)
+    del x
+    torch.cuda.empty_cache()
