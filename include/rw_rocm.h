@@ -476,9 +476,11 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
  * sees no row of the pool, gets zeros.  Several rows may attend to one sequence,
  * with lengths of their own (the tokens of a prompt, drafted tokens).  max_len
  * sizes the launch: give the longest length, or for a graph the longest that
- * replays will see.  Scores, softmax and sums are f32, products f32-equivalent
- * for every type of pool.  The rows seen and q must be finite; what the pool
- * holds behind a sequence's length has no effect.
+ * replays will see.  Scores, softmax and sums are f32, products as exact as
+ * f32's for every type of pool, weights down to 2^-126 of the largest and values
+ * of any size (f16 pools: values of q below 2^-37 of their head's largest lose
+ * bits).  The rows seen and q must be finite, scores within f32's range; what the
+ * pool holds behind a sequence's length has no effect.
  * The workspace (NULL: one kept per (device, stream), not for a stream that
  * is being captured) holds rw_rocm_paged_attention_workspace_size bytes, 16-byte
  * aligned; 0 for arguments the call would refuse. */

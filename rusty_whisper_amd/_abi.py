@@ -557,6 +557,11 @@ def logits_topk_workspace_size(rows: int, n_vocab: int, k: int) -> int:
 
 
 # ------------------------------------------- keys and values in pages
+#
+# The calls are queued on `stream`, a stream's handle; None is the null stream,
+# whatever torch's current stream is (torch.cuda.current_stream().cuda_stream).
+# Tensors are checked for their type, device and size; pointers given as numbers
+# are taken as they are.
 
 try:  # (a step's calls look at a dozen tensors: types are compared as objects, not by name)
     from torch import bfloat16 as _BF16, float16 as _F16, float32 as _F32, int32 as _I32, uint32 as _U32
@@ -573,15 +578,17 @@ def _pointer(a, what: str) -> int | None:
     return _ptr(a)
 
 
-def _dense(a, dtype, count: int, what: str, device: int | None):
+def _dense(a, dtype, count: int, what: str, device: int | None, other=None):
     """The pointer of a device array of `count` elements, which as a tensor
-    must be dense, of `dtype`, long enough and on the `device` of the call's
-    first tensor (None: that was a pointer)."""
+    must be dense, of `dtype` (or `other`), long enough and on the `device` of the
+    call's first tensor (None: that was a pointer)."""
+    if a is None:
+        return None
     try:
         p = a.data_ptr()
     except AttributeError:
         return _pointer(a, what)
-    if a.dtype is not dtype or not a.is_contiguous():
+    if (a.dtype is not dtype and a.dtype is not other) or not a.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor")
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
@@ -592,6 +599,8 @@ def _dense(a, dtype, count: int, what: str, device: int | None):
 
 def _workspace(a, size: int, device: int | None):
     """The pointer of a workspace of `size` bytes."""
+    if a is None:
+        return None
     try:
         p = a.data_ptr()
     except AttributeError:
@@ -645,8 +654,8 @@ def _rows(a, rows: int, n: int, ld: int | None, what: str, device: int | None, d
     if device is not None and a.get_device() != device:
         raise ValueError(f"{what} is on another device")
     sh, st = a.shape, a.stride()
-    if ld is None and sh == (rows, n) and st[1] == 1:
-        return p, st[0] if rows > 1 else n  # (most calls)
+    if sh == (rows, n) and st[1] == 1 and (ld is None or ld == st[0]):  # (most calls)
+        return p, ld or (st[0] if rows > 1 else n)
     step = _row_step(a, n, what)
     step = ld or step
     if rows > 0 and (rows - 1) * step + n > (1 + sum((x - 1) * y for x, y in zip(sh, st)) if a.numel() else 0):
@@ -812,12 +821,6 @@ class KvBook:
 
 # --------------------------------------------------------- token scores
 
-def _ids(a, count: int, what: str, device: int | None):
-    """_dense of 32-bit ids, signed or not."""
-    unsigned = a is not None and getattr(a, "dtype", None) is _U32
-    return _dense(a, _U32 if unsigned else _I32, count, what, device)
-
-
 def token_logprobs_workspace_size(rows: int, n_vocab: int, k: int) -> int:
     return lib().rw_rocm_token_logprobs_workspace_size(rows, n_vocab, k)
 
@@ -838,9 +841,9 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
             raise ValueError(f"dtype {dtype} for {logits.dtype} logits")
     check(lib().rw_rocm_token_logprobs_dev(
         F32 if dtype is None else dtype, *_rows(logits, rows, n_vocab, ld, "logits", d, _ANY_FLOAT), rows,
-        n_vocab, _ids(tokens, rows * n_tok, "tokens", d), n_tok,
+        n_vocab, _dense(tokens, _I32, rows * n_tok, "tokens", d, _U32), n_tok,
         _dense(logprobs, _F32, rows * n_tok, "logprobs", d),
-        _dense(entropy, _F32, rows, "entropy", d), k, _ids(top_ids, rows * k, "top_ids", d),
+        _dense(entropy, _F32, rows, "entropy", d), k, _dense(top_ids, _I32, rows * k, "top_ids", d, _U32),
         _dense(top_logprobs, _F32, rows * k, "top_logprobs", d), _workspace(workspace, workspace_len, d),
         workspace_len, stream))
 

@@ -34,7 +34,9 @@ namespace rw {
 constexpr int SCORE_TOP = 32;         // alternatives per row at most
 constexpr int SCORE_MAX_PARTS = 64;   // parts of a row: a lane each in k_score_join
 constexpr int SCORE_HEADS = 8;        // alternatives up to which k_score_join compares heads
-constexpr int SCORE_EAGER = 8;        // alternatives up to which every step's candidates are ranked at once
+// Alternatives up to which every step's candidates are ranked at once: 1792 rows
+// with 5 73 us (with 4 here, collected: 76), 366 rows with 12 28.5 (with 16 here: 33.9).
+constexpr int SCORE_EAGER = 8;
 constexpr int SCORE_LINE = 128;       // bytes that the loads of a step are aligned to
 constexpr uint32_t SCORE_NONE = 0xFFFFFFFFu;
 
@@ -114,6 +116,11 @@ __device__ inline float score_dpp_all(float v) {  // every lane has a source
 // (groups of 64 / 2^ceil(log2 k) lanes), or of the values from lo on, moved up
 // by halving while k values lie above; the k-th largest itself where that stops
 // far below it (values of very unlike size, such as masks of the type's lowest).
+//   Halving ends within 3 of k (286 f16 rows with 32 alternatives 30.2 us; at k
+// 29.7 and one row with 5 the same, within 8 32.7), after 6 turns (after 3 36.8,
+// after 10 the same).  The ranking starts 16 above k: 1792 rows that masks of the
+// lowest value leave 700 logits of, 16 alternatives, 93 us, 100 without it (one such row
+// 24.4 and 22.4; rows without masks the same either way).
 __device__ inline float score_bound(float v, int k, float lo) {
   float w = fmaxf(v, score_dpp_all<0xB1>(v));  // pairs
   float o = score_dpp_all<0x4E>(w);            // fours
@@ -183,7 +190,8 @@ struct ScoreBest {
   __device__ inline void take(float w, int i, int c, int k, float *sv, int *si) {
     const int lane = threadIdx.x & 63;
     if (n == k && c <= 4 + k * 3 / 8) {
-      // few: each in its place, 15 instructions that wait for each other
+      // few: each in its place, 15 instructions that wait for each other (366 rows
+      // with 5 alternatives 26.4 us, none so 30.4; with 32, up to 4 so 31.9, these 30.2)
       for (int e = 0; e < c; ++e) {
         const float cv = score_lane(w, e);
         const int ci = __builtin_amdgcn_readlane(i, e);
@@ -332,7 +340,10 @@ __global__ __launch_bounds__(64 * NW) void k_score(const typename E::T *__restri
     if (k == 0) continue;
     const uint64_t pass = __builtin_amdgcn_ballot_w64(mx >= lo);
     if (!pass) continue;
-    // the k-th largest of the lanes' maxima so far is one of the k best
+    // the k-th largest of the lanes' maxima so far is one of the k best (looked for
+    // where more than 4 lanes pass: 1792 rows with 16 alternatives 78.8 us, with 32
+    // 101; more than 1: 80.4, 108; more than 12: 81.5, 96; up to 8 alternatives
+    // k + 3 lanes, k or k + 12 the same)
     if (__builtin_popcountll(pass) > (k <= SCORE_EAGER ? k + 3 : 4) && __builtin_popcountll(__builtin_amdgcn_ballot_w64(st.m >= all)) > k)
       lo = fmaxf(lo, score_bound(st.m, k, all));
 #pragma unroll
