@@ -157,14 +157,14 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t pie
 // Query columns beyond the group's are zeros (a matrix instruction costs the
 // same with 1 or 16 queries, and the matrix cores are a quarter busy at most).
 //
-// Bound by reading k and v once, which at 5.4 TB/s also the score kernel's
-// plain reads do not pass: 131071 f16 keys of 8 heads of 128, 537 MB, 96 us +
-// 5 for the join (counters: 545 MB read, each line once).  61 rows of up to
-// 8190 bf16 keys, 767 MB, 152 + 5 us: the rest is the tail of unlike rows.
-// Measured and left: 8 wavefronts per workgroup (same: one CU draws about 50
-// GB/s either way), 3 wavefronts per SIMD (same; bf16 spills), non-temporal
-// loads (99 -> 113 us: half lines that the next wavefront's tile needs are
-// gone), two or four neighbouring tiles per wavefront (98 -> 111).
+// Bound by reading k and v once: 131071 f16 keys of 8 heads of 128, 537 MB, 96 us
+// (5.6 TB/s; counters: 555 MB, each line once) + 5 for the join.  61 rows of up
+// to 8190 bf16 keys, 767 MB, 158 + 5 us: the rest is the tail of unlike rows.
+// Measured and left (with two f16 parts of p and q): 8 wavefronts per workgroup
+// (same: one CU draws about 50 GB/s either way), 3 wavefronts per SIMD (same; bf16
+// spills), non-temporal loads (99 -> 113 us: half lines that the next
+// wavefront's tile needs are gone), two or four neighbouring tiles per wavefront
+// (98 -> 111).
 
 constexpr int PA_WAVES = 4;
 constexpr float PA_LOG2E = 1.44269504088896340736f;

@@ -19,13 +19,14 @@
 // time (for few alternatives in every step) they are put into the k best: a few
 // one by one, more of them ranked, an entry's rank being the number of entries
 // before it (larger, or equal with a smaller id).  366 rows of 51865 f32 with 20
-// alternatives: 28 us; ranked in every step 35; with 5, every step 22.
+// alternatives: 28 to 31 us; ranked in every step 35; with 5, every step 22.
 //
 // Bound by reading the logits: 1792 rows of 51866 f32, 372 MB, 68 us without
-// alternatives (5.4 TB/s), 71 with 5, 77 with 16, 100 with 32; f16 45 and 58
-// (4.1 TB/s: the exponentials and the conversion begin to show).  Rows whose
-// logits rise with their ids take longest (every step replaces the k best: 180
-// us with 5).  One row: latency, 4.4 us with 5 alternatives and 3.8 for the join.
+// alternatives (5.4 TB/s), 71 with 5, 77 to 80 with 16, 100 to 108 with 32; f16 45
+// and 58 to 68 (4.1 TB/s: the exponentials and the conversion begin to show).
+// Rows whose logits rise with their ids take longest (every step replaces the k
+// best: 204 us with 5).  One row: latency, 4.6 us with 5 alternatives and 3.8 for
+// the join.
 #pragma once
 #include "rw_kv.hpp"
 

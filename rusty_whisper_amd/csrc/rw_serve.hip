@@ -128,18 +128,18 @@ static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size
 // less than nsplit and never falls with max_len.
 //   Up to 256 KB of k and v per row and head: one chunk.  A CU draws 50 GB/s,
 // so 256 KB take it 5 us, and the join's launch takes 3 to 5 (448 f16 keys of
-// 64: 6.2 us, in two chunks 5.4 + 2.9; 1024 keys of 128, 512 KB: 15.1 against
-// 7.4 + 4 in four).
+// 64, 5 rows: 6.5 us, in two chunks 8.4; 1024 keys of 128, 512 KB: 14.9 against
+// 9.9 in four).
 //   Longer: chunks of 128 KB or more, up to 512 workgroups, two per CU (more of
-// them only cost: 131071 keys over 8 heads in 512 workgroups 96 us + join 5.0,
-// in 1024 98 + 5.6, in 2048 104 + 6).
+// them only cost: 131071 keys over 8 heads in 512 workgroups 99 us, in 1024 102,
+// in 2048 110).
 //   Several rows are seldom of one length, and a long one must not be left to
 // itself at the end: up to 256 workgroups per row and 4096 in all, in chunks of
-// 192 KB or more (48 ragged rows of 20 heads: 64.4 us; chunks of 256 KB 66.9, of
-// 384 KB 73.8, of 128 KB 64.6; 11 rows of 10468 keys: 69.7, and 75.6 with 128 KB;
-// four rows of 32768 keys, 8 heads: 99 us, ragged 81, and with up to 4096 111 and
-// 88).  Equal shares of all rows' keys for 512 resident workgroups, found from
-// the lengths on the device, measured 171 us where this takes 157 (61 ragged
+// 192 KB or more (48 ragged f32 rows of 20 heads: 58.2 us; chunks of 256 KB 61.2,
+// of 384 KB 68.5, of 128 KB 58.4; 11 rows of 10468 keys, 8 heads: 88.5 to 89 with
+// any; four f16 rows of 32768 keys, 8 heads: 97 us, ragged 72, and with up to 4096
+// 102 and 79).  Equal shares of all rows' keys for 512 resident workgroups, found from
+// the lengths on the device, measured 171 us where this took 157 (61 ragged
 // rows, 8 heads).
 struct PagedPlan {
   size_t base;  // workgroups per chunk
