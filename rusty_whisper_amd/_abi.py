@@ -612,8 +612,8 @@ def _workspace(a, size: int, device: int | None):
     return p
 
 
-def _row_step(a, n: int, what: str) -> int:
-    """Elements from one row of n values to the next.  A row's values are the
+def _row_step(a, rows: int, n: int, what: str) -> int:
+    """Elements from one of `rows` rows of n values to the next.  A row's values are the
     trailing dimensions of a tensor, which have to be dense, its rows the ones
     before, which have to lie at one distance: [rows, n], a column block of
     wider rows (or their first n columns), [rows, n_head, head_size] out of a
@@ -632,6 +632,8 @@ def _row_step(a, n: int, what: str) -> int:
         return n
     count, step = 1, n  # the rows of dimensions d .. are `step` apart
     for i in range(d - 1, -1, -1):
+        if count >= rows:
+            break
         if sh[i] == 1:
             continue
         if count == 1:
@@ -656,7 +658,7 @@ def _rows(a, rows: int, n: int, ld: int | None, what: str, device: int | None, d
     sh, st = a.shape, a.stride()
     if sh == (rows, n) and st[1] == 1 and (ld is None or ld == st[0]):  # (most calls)
         return p, ld or (st[0] if rows > 1 else n)
-    step = _row_step(a, n, what)
+    step = _row_step(a, rows, n, what)
     step = ld or step
     if rows > 0 and (rows - 1) * step + n > (1 + sum((x - 1) * y for x, y in zip(sh, st)) if a.numel() else 0):
         raise ValueError(f"{what} ends before row {rows - 1} of {n} values does")

@@ -149,3 +149,11 @@ def test_a_type_that_is_not_the_logits_own_is_refused():
             right = A._TORCH_DTYPES[own] == dtype
             with pytest.raises(A.RwError if right else ValueError, match="RW_E" if right else "logits"):
                 A.token_logprobs_dev(x, 1, 8, i32(1, 1), 1, lp, dtype=dtype)
+
+
+def test_only_the_calls_rows_need_one_distance():
+    a = numbered(2, 8, N)[:, :3]  # three rows, and three more 8 rows from the first
+    assert A._rows(a, 3, N, None, "q", None) == (a.data_ptr(), N)
+    assert A._rows(a, 1, N, None, "q", None)[0] == a.data_ptr()
+    with pytest.raises(ValueError, match="one distance"):
+        A._rows(a, 4, N, None, "q", None)
