@@ -284,10 +284,8 @@ __device__ inline void pa_add(const float (&p)[PaTile<E>::PER], const typename P
   }
 }
 
-// a mean of finite values: rounded past f32's largest, it is that
-__device__ inline float pa_mean(float x) {
-  return __builtin_isinf(x) ? __builtin_copysignf(__FLT_MAX__, x) : x;
-}
+// a mean of finite values, rounded past f32's largest, is that
+__device__ inline float pa_largest(float x) { return __builtin_copysignf(__FLT_MAX__, x); }
 
 // exp2(x) for x <= 0 or -inf against a maximum that may be -inf itself
 __device__ inline float pa_weight(float m, float top) {
@@ -519,7 +517,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
           const float y = o[d][i] * f;
           float &mean = so[wv][qr][16 * d + r];
           if (!M::WIDE || first) mean = y;
-          else if (!__builtin_isfinite(mean)) mean = pa_mean(y);
+          else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(o[d][i]) ? pa_largest(y) : y;
           over |= qr < gq && !__builtin_isfinite(y);
         }
       }
@@ -542,11 +540,17 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: no page of the row is in the pool
 #pragma unroll
     for (int k = 0; k < PA_WAVES; ++k) y += so[k][qr][d] * (w[k] * inv);
+    if (M::WIDE && __builtin_isinf(y)) {
+      bool finite = true;
+#pragma unroll
+      for (int k = 0; k < PA_WAVES; ++k) finite &= (bool)__builtin_isfinite(so[k][qr][d]);
+      if (finite) y = pa_largest(y);
+    }
     if (direct) {
-      orow[i] = pa_mean(y);
+      orow[i] = y;
     } else {
       const int64_t run = ((int64_t)row * heads + hq + qr) * gridDim.y + blockIdx.y;
-      part[run * DH + d] = pa_mean(y);
+      part[run * DH + d] = y;
       if (d == 0) part[runs * DH + 2 * run] = top, part[runs * DH + 2 * run + 1] = l;
     }
   }
@@ -598,7 +602,12 @@ __global__ __launch_bounds__(256) void k_paged_join(const float *__restrict__ pa
     float y = 0.0f;
 #pragma unroll
     for (int i = 0; i < SIDE; ++i) y += ((const float *)sy[i])[threadIdx.x];
-    out[row * ldo + (int64_t)hq * DH + threadIdx.x] = pa_mean(y);
+    if (__builtin_isinf(y)) {
+      bool finite = true;
+      for (int z = 0; z < nz; ++z) finite &= (bool)__builtin_isfinite(part[(run0 + z) * DH + threadIdx.x]);
+      if (finite) y = pa_largest(y);
+    }
+    out[row * ldo + (int64_t)hq * DH + threadIdx.x] = y;
   }
 }
 

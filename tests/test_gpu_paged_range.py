@@ -169,3 +169,71 @@ def test_queries_at_the_end_of_f32(dtype, q0):
     p /= p.sum()
     tol = 2 * (8 * 33 + 12 + n) * U * (p @ np.abs(V[0]))
     assert np.all(np.abs(got - p @ V[0]) <= tol), (got[:4], (p @ V[0])[:4])
+
+
+# ------------------------------- key heads of several query heads, infinities
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("gap", [14.0, 20.0, 40.0, 75.0])
+@pytest.mark.parametrize("n", [32, 448, 3000])
+def test_small_weights_of_grouped_heads(dtype, dim, gap, n):
+    """As the first test here, three query heads to a key head, each with an
+    outweighing key of its own, and heads of every size (q's value is
+    sqrt(dim), rounded: the scores' share of the tolerance covers it)."""
+    pages, group = -(-n // PAGE), 3
+    k, v = pool(dtype, 1, pages, 1, PAGE, dim, seed=n + dim)
+    rng = np.random.default_rng(n)
+    s = rng.integers(-32, 33, (pages * PAGE, group)) / 64.0
+    for g in range(group):
+        s[3 + 5 * g, g] = gap
+        v[0, 0, 0, :, 3 + 5 * g] = 0
+    k.zero_()
+    k[0, :, 0, :, :group] = torch.from_numpy(s).cuda().reshape(pages, PAGE, group).to(k.dtype)
+    q = torch.zeros(group, dim, device="cuda")
+    for g in range(group):
+        q[g, g] = dim**0.5
+    table = np.arange(pages, dtype=np.int32)[None]
+    P = A.KvPages(k, v)
+    got = run(P, q.reshape(1, -1), table, [n], group)[0]
+    _, V = gather(k, v, 0, table[0], n)
+    for g in range(group):
+        x = s[:n, g] * (float(q[g, g]) / np.sqrt(dim))
+        p = np.exp(x - x.max())
+        p /= p.sum()
+        tol = 2 * (8 * (gap + 1) + 12 + n) * U * (p @ np.abs(V[0]))
+        assert np.all(np.abs(got[g] - p @ V[0]) <= tol), (g, np.max(np.abs(got[g] - p @ V[0])), np.max(tol))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("group", [2, 17])
+def test_one_key_is_its_value_for_grouped_heads(dtype, group):
+    t = torch.finfo(DTYPES[dtype])
+    k, v = pool(dtype, 1, 1, 1, PAGE, DIM, seed=1)
+    ends = torch.tensor([t.max, t.min, t.tiny, -t.tiny, t.tiny / 2, 0.0, 1.0, t.max / 2, t.smallest_normal * 1.5, t.eps])
+    v[0, 0, 0, : len(ends), 0] = ends.to(v.dtype).cuda()
+    P = A.KvPages(k, v)
+    got = run(P, torch.randn(1, group * DIM, device="cuda"), np.zeros((1, 1), np.int32), [1], group)[0]
+    assert np.array_equal(got, np.broadcast_to(v[0, 0, 0, :, 0].double().cpu().numpy(), got.shape))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("group", [1, 2])
+@pytest.mark.parametrize("n", [1, 40, 3000])
+def test_infinite_values_are_not_made_finite(dtype, group, n):
+    """What kv_write rounded past the type's largest shows in the result, and
+    in its own place only."""
+    n_pages = -(-n // PAGE)
+    k, v = pool(dtype, 1, n_pages, 1, PAGE, DIM, seed=n)
+    v[0, 0, 0, 7, 0] = float("inf")
+    v[0, 0, 0, 9, 0] = -float("inf")
+    q = torch.randn(1, group * DIM, device="cuda")
+    table = np.arange(n_pages, dtype=np.int32)[None]
+    P = A.KvPages(k, v)
+    got = run(P, q, table, [n], group)[0]
+    K, V = gather(k, v, 0, table[0], n)
+    assert not np.isfinite(got[:, [7, 9]]).any()
+    V[:, :, [7, 9]] = 0
+    got[:, [7, 9]] = 0
+    want, tol = attend(q[0].double().cpu().numpy().reshape(-1, DIM), K, V)
+    assert np.all(np.abs(got - want) <= tol)
