@@ -65,11 +65,15 @@ extern "C" {
 #define RW_F32 0
 #define RW_F16 1
 #define RW_BF16 30
+#define RW_I8 24
 #define RW_Q4_0 2
 #define RW_Q4_1 3
 #define RW_Q5_0 6
 #define RW_Q5_1 7
 #define RW_Q8_0 8
+/* (no ggml id) 8-bit floating point, 4 bits of exponent and 3 of mantissa, no
+ * infinities: the largest value is 448 */
+#define RW_E4M3 0x100
 
 typedef struct rw_weight rw_weight;
 
@@ -450,6 +454,7 @@ typedef struct rw_kv_pages {
   int n_head, head_size, page_rows;
   size_t n_layer, n_pages;
   void *k, *v;
+  float *k_scale, *v_scale; /* RW_I8 and RW_E4M3 only; not looked at for other types */
 } rw_kv_pages;
 
 /* Rows k[r], v[r] (f32 [rows, n_head * head_size], row strides ldk, ldv in
@@ -459,6 +464,13 @@ typedef struct rw_kv_pages {
 int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k, size_t ldk, const float *v, size_t ldv,
                          size_t rows, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,
                          const int32_t *pos, void *stream);
+
+/* The reverse: rows pos[r] of sequences seq[r] in `layer` as f32 rows k[r], v[r]
+ * (layout and strides as for rw_rocm_kv_write_dev; exactly what attention
+ * takes them for).  A row whose place the table does not have gets zeros. */
+int rw_rocm_kv_read_dev(const rw_kv_pages *pages, size_t layer, float *k, size_t ldk, float *v, size_t ldv, size_t rows,
+                        const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq, const int32_t *pos,
+                        void *stream);
 
 /* Pages src[i] -> dst[i] of every layer (k and v), i < n.  src and dst are host
  * arrays, used before the call returns (so a captured graph repeats these
@@ -489,6 +501,55 @@ int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const fl
                                 int n_head, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,
                                 const int32_t *len, size_t max_len, float *out, size_t ldo, void *workspace,
                                 size_t workspace_len, void *stream);
+
+/* Attention of several new tokens per sequence: trees of drafted tokens, or
+ * chunks of prompts whose first part is in the pages.  Rows starts[i] ..
+ * starts[i + 1] - 1 of q and out (starts: n_trees + 1 entries) are the nodes of
+ * tree i, whose sequence is seq[i] (NULL: i): node j's key and value are row
+ * past[i] + j of the sequence, written before.  A node sees the sequence's rows
+ * 0 .. past[i] - 1 and, of the tree's own,
+ *   mask NULL   those up to itself (a chunk of a prompt, a chain of drafts)
+ *   mask        node j where bit j % 32 of mask[r][j / 32] is set (n_words words
+ *               per row r of the call; its own bit too, where it is to see itself);
+ *               words or bits beyond the tree's nodes are nothing
+ * Rows of other trees are never seen.  Otherwise as
+ * rw_rocm_paged_attention_dev (heads, layout, precision; a row that sees nothing
+ * gets zeros), and a row of the pool that a node does not see may hold
+ * anything, infinities and NaN too, also where other nodes see it.  Rows of q
+ * and out in no tree are left as they were.  max_rows: the most nodes of a
+ * tree (those beyond are left out); max_len: the largest past + nodes; rows counts q's.
+ * starts, past and mask are on the device, read when the work runs.  n_trees x
+ * max_rows x n_head <= 2^23. */
+size_t rw_rocm_tree_attention_workspace_size(const rw_kv_pages *pages, size_t rows, int n_head, size_t n_trees,
+                                             size_t max_rows, size_t max_len);
+int rw_rocm_tree_attention_dev(const rw_kv_pages *pages, size_t layer, const float *q, size_t ldq, size_t rows, int n_head,
+                               const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq, size_t n_trees,
+                               const int32_t *starts, size_t max_rows, const int32_t *past, const uint32_t *mask,
+                               size_t n_words, size_t max_len, float *out, size_t ldo, void *workspace,
+                               size_t workspace_len, void *stream);
+
+/* The path of each tree that samples agree with.  tokens[r] is the token of node
+ * r, parent[r] its parent's number in the tree (a parent comes before its children; the
+ * first node is the root, the last token that is known already), sampled[r] the
+ * token that was sampled at it (rw_rocm_sample_tokens_dev on its logits).  From
+ * the root, the path goes on to the first child whose token is its parent's sample.
+ * kept[i][0 ..] are the path's nodes, the root first, -1 behind them
+ * (n_trees x max_rows), n_kept[i] their number, next[i] the sample at the last
+ * one: the sequence's next token.  A tree without nodes has n_kept 0 and next
+ * 0xFFFFFFFF.  Nodes from max_rows on are left out.  All arrays on the device. */
+int rw_rocm_tree_accept_dev(const uint32_t *tokens, const int32_t *parent, const uint32_t *sampled, size_t rows,
+                            const int32_t *starts, size_t n_trees, size_t max_rows, int32_t *kept, int32_t *n_kept,
+                            uint32_t *next, void *stream);
+
+/* Rows past[i] + kept[i][j] become rows past[i] + j of sequence seq[i] (NULL:
+ * i), j < n_kept[i] <= ld_kept, in every layer: the accepted path's keys and
+ * values move together (then rw_rocm_kv_book_truncate to past + n_kept gives the
+ * rest back).  kept[i] must rise, as rw_rocm_tree_accept_dev leaves it; entries
+ * without a place are skipped.  The rows from past on must be the sequence's
+ * own, in no page that another sequence of the call lists. */
+int rw_rocm_kv_keep_rows_dev(const rw_kv_pages *pages, const int32_t *table, size_t ld_table, size_t n_seqs,
+                             const int32_t *seq, size_t n_trees, const int32_t *past, const int32_t *kept, size_t ld_kept,
+                             const int32_t *n_kept, void *stream);
 
 /* The book of a pool: which sequence holds which pages (host memory only; no
  * device is needed).  A step of a serving program: extend the sequences by
@@ -554,6 +615,29 @@ int rw_rocm_token_logprobs_dev(int dtype, const void *logits, size_t ld, size_t 
                                const uint32_t *tokens, size_t n_tok, float *logprobs, float *entropy, size_t k,
                                uint32_t *top_ids, float *top_logprobs, void *workspace, size_t workspace_len,
                                void *stream);
+
+/* A token per row of logits [rows, n_vocab] (device, dtype RW_F32, RW_F16 or
+ * RW_BF16, row stride ld in elements), drawn with the row's uniform number
+ * u[r] in [0, 1).  In the order of the logits, larger ones first, equal ones by
+ * lowest id, a token weighs w = e^((x - max) / temperature).  Kept are
+ *   the first top_k              (0 or less: all)
+ *   of these, w >= min_p         (0 or less: all)
+ *   of these, the fewest first ones that have top_p of their weight  (1 or more: all)
+ * and always the first.  The token is the first of them at which the sum of
+ * the weights passes u times their total.  temperature[r] <= 0 takes the
+ * first of the order.  logprobs[r] (NULL: not formed) is the log of the token's share of the kept
+ * weight.  temperature, top_k, top_p and min_p are device arrays, one per row; NULL
+ * switches one off (temperature: 1).
+ * Weights are formed in 64 bits and summed exactly, in steps of 2^-42 of the
+ * largest: the same token at every call.  A row holding NaN or +inf, or only
+ * -inf, and one whose settings are NaN or whose temperature is infinite gets
+ * token 0xFFFFFFFF and NaN.  n_vocab <= 2^20, rows <= 2^23.  The workspace (NULL: one kept per
+ * (device, stream), not for a stream that is being captured) holds
+ * rw_rocm_sample_tokens_workspace_size bytes, 16-byte aligned. */
+size_t rw_rocm_sample_tokens_workspace_size(size_t rows, size_t n_vocab);
+int rw_rocm_sample_tokens_dev(int dtype, const void *logits, size_t ld, size_t rows, size_t n_vocab, const float *u,
+                              const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                              uint32_t *tokens, float *logprobs, void *workspace, size_t workspace_len, void *stream);
 
 /* ---- Model files straight to resident weights ----
  *

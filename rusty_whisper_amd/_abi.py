@@ -23,6 +23,7 @@ CODE_NAMES = {RW_EINVAL: "RW_EINVAL", RW_ENODEV: "RW_ENODEV", RW_EHIP: "RW_EHIP"
 Q4_0, Q4_1, Q5_0, Q5_1, Q8_0 = 2, 3, 6, 7, 8
 DTYPES = (Q4_0, Q4_1, Q5_0, Q5_1, Q8_0)
 F32, F16, BF16 = 0, 1, 30
+I8, E4M3 = 24, 0x100
 QK = 32
 GEMV_MAX_M = 8
 
@@ -47,7 +48,8 @@ class rw_linear(C.Structure):
 class RwKvPages(C.Structure):
     """struct rw_kv_pages (include/rw_rocm.h)."""
     _fields_ = [("dtype", C.c_int), ("n_head", C.c_int), ("head_size", C.c_int), ("page_rows", C.c_int),
-                ("n_layer", C.c_size_t), ("n_pages", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p)]
+                ("n_layer", C.c_size_t), ("n_pages", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
 
 
 _SIGNATURES = {
@@ -116,6 +118,23 @@ _SIGNATURES = {
     "rw_rocm_kv_write_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t,
                                        C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
                                        C.c_void_p]),
+    "rw_rocm_kv_read_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t,
+                                      C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
+                                      C.c_void_p]),
+    "rw_rocm_tree_attention_workspace_size": (C.c_size_t, [C.POINTER(RwKvPages), C.c_size_t, C.c_int, C.c_size_t, C.c_size_t,
+                                                           C.c_size_t]),
+    "rw_rocm_tree_attention_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_int,
+                                             C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p,
+                                             C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p,
+                                             C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rw_rocm_tree_accept_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
+                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "rw_rocm_kv_keep_rows_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t,
+                                           C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "rw_rocm_sample_tokens_workspace_size": (C.c_size_t, [C.c_size_t, C.c_size_t]),
+    "rw_rocm_sample_tokens_dev": (C.c_int, [C.c_int, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
+                                            C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                            C.c_size_t, C.c_void_p]),
     "rw_rocm_kv_copy_pages_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "rw_rocm_paged_attention_workspace_size": (C.c_size_t, [C.POINTER(RwKvPages), C.c_size_t, C.c_int, C.c_size_t]),
     "rw_rocm_paged_attention_dev": (C.c_int, [C.POINTER(RwKvPages), C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t,
@@ -564,10 +583,12 @@ def logits_topk_workspace_size(rows: int, n_vocab: int, k: int) -> int:
 # are taken as they are.
 
 try:  # (a step's calls look at a dozen tensors: types are compared as objects, not by name)
-    from torch import bfloat16 as _BF16, float16 as _F16, float32 as _F32, int32 as _I32, uint32 as _U32
+    from torch import (bfloat16 as _BF16, float8_e4m3fn as _E4M3, float16 as _F16, float32 as _F32, int8 as _I8,
+                       int32 as _I32, uint32 as _U32)
 except ImportError:
-    _BF16 = _F16 = _F32 = _I32 = _U32 = None
+    _BF16 = _E4M3 = _F16 = _F32 = _I8 = _I32 = _U32 = None
 _TORCH_DTYPES = {_F32: F32, _F16: F16, _BF16: BF16}
+_POOL_DTYPES = {**_TORCH_DTYPES, _I8: I8, _E4M3: E4M3}
 _ANY_FLOAT = (_F32, _F16, _BF16)
 
 
@@ -671,24 +692,34 @@ def _host(a: np.ndarray) -> int:
 
 
 class KvPages:
-    """rw_kv_pages over two device tensors: k [n_layer, n_pages, n_head,
+    """rw_kv_pages over device tensors: k [n_layer, n_pages, n_head,
     page_rows, head_size] and v [n_layer, n_pages, n_head, head_size,
-    page_rows], both float32, float16 or bfloat16."""
+    page_rows], both float32, float16 or bfloat16, or both int8 or
+    float8_e4m3fn with k_scale and v_scale, float32 [n_layer, n_pages, n_head,
+    page_rows]."""
 
-    def __init__(self, k, v):
+    def __init__(self, k, v, k_scale=None, v_scale=None):
         L, N, H, P, D = k.shape
         if v.shape != (L, N, H, D, P):
             raise ValueError("v must be [n_layer, n_pages, n_head, head_size, page_rows]")
-        dtype = _TORCH_DTYPES.get(k.dtype)
+        dtype = _POOL_DTYPES.get(k.dtype)
         if k.dtype != v.dtype or dtype is None:
-            raise ValueError("k and v must have one type: float32, float16 or bfloat16")
+            raise ValueError("k and v must have one type: float32, float16, bfloat16, int8 or float8_e4m3fn")
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("k and v must be contiguous")
-        self.k, self.v = k, v  # keeps the tensors alive
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale  # keeps the tensors alive
         self.device = k.get_device()
         if v.get_device() != self.device:
             raise ValueError("k and v are on different devices")
-        self.st = RwKvPages(dtype, H, D, P, L, N, k.data_ptr(), v.data_ptr())
+        scales = [None, None]
+        if dtype in (I8, E4M3):
+            for i, (s, what) in enumerate(((k_scale, "k_scale"), (v_scale, "v_scale"))):
+                if s is None or s.shape != (L, N, H, P):
+                    raise ValueError(f"{what} must be [n_layer, n_pages, n_head, page_rows]")
+                scales[i] = _dense(s, _F32, 0, what, self.device)
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale and v_scale are for int8 and float8_e4m3fn")
+        self.st = RwKvPages(dtype, H, D, P, L, N, k.data_ptr(), v.data_ptr(), *scales)
 
     @property
     def n_values(self) -> int:
@@ -712,6 +743,16 @@ def kv_write_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=No
     n = pages.n_values
     check(lib().rw_rocm_kv_write_dev(pages.st, layer, *_rows(k, rows, n, ldk, "k", d), *_rows(v, rows, n, ldv, "v", d),
                                      rows, t, ld, n_seqs, s, _dense(pos, _I32, rows, "pos", d), stream))
+
+
+def kv_read_dev(pages: KvPages, layer: int, k, v, rows: int, table, pos, seq=None, ldk: int | None = None,
+                ldv: int | None = None, stream: int | None = None) -> None:
+    """Row pos[r] of sequence seq[r] (None: r) into the float32 device rows k[r], v[r]."""
+    d = pages.device
+    t, ld, n_seqs, s = _table_args(table, seq, rows, d)
+    n = pages.n_values
+    check(lib().rw_rocm_kv_read_dev(pages.st, layer, *_rows(k, rows, n, ldk, "k", d), *_rows(v, rows, n, ldv, "v", d),
+                                    rows, t, ld, n_seqs, s, _dense(pos, _I32, rows, "pos", d), stream))
 
 
 def kv_copy_pages_dev(pages: KvPages, src, dst, stream: int | None = None) -> None:
@@ -740,6 +781,62 @@ def paged_attention_dev(pages: KvPages, layer: int, q, rows: int, n_head: int, t
                                             s, _dense(lens, _I32, rows, "lens", d), max_len,
                                             *_rows(out, rows, n, ldo, "out", d),
                                             _workspace(workspace, workspace_len, d), workspace_len, stream))
+
+
+# ------------------------------------------- drafted tokens and chunks
+
+def tree_attention_workspace_size(pages: KvPages, rows: int, n_head: int, n_trees: int, max_rows: int, max_len: int) -> int:
+    return lib().rw_rocm_tree_attention_workspace_size(pages.st, rows, n_head, n_trees, max_rows, max_len)
+
+
+def tree_attention_dev(pages: KvPages, layer: int, q, rows: int, n_head: int, table, starts, max_rows: int, past,
+                       max_len: int, out, mask=None, seq=None, ldq: int | None = None, ldo: int | None = None,
+                       workspace=None, workspace_len: int = 0, stream: int | None = None) -> None:
+    """Rows starts[i] .. starts[i + 1] - 1 of q are the nodes of tree i (as many
+    trees as `past` has entries), node j the row past[i] + j of sequence
+    seq[i] (None: i).  Each sees the rows before past[i] and the nodes whose bits its row of
+    `mask` (32-bit words [rows, n_words]) has set; None: those up to itself.
+    table, starts, past, seq: device int32; max_rows: the most nodes of a tree;
+    max_len: the largest past + nodes."""
+    d = pages.device
+    n_trees = past.numel()
+    t, ld, n_seqs, s = _table_args(table, seq, n_trees, d)
+    n = n_head * pages.st.head_size
+    n_words = 0
+    if mask is not None:
+        if mask.dim() != 2:
+            raise ValueError("mask must be [rows, n_words]")
+        n_words = mask.shape[1]
+    check(lib().rw_rocm_tree_attention_dev(
+        pages.st, layer, *_rows(q, rows, n, ldq, "q", d), rows, n_head, t, ld, n_seqs, s, n_trees,
+        _dense(starts, _I32, n_trees + 1, "starts", d), max_rows, _dense(past, _I32, n_trees, "past", d),
+        _dense(mask, _I32, rows * n_words, "mask", d, _U32), n_words, max_len, *_rows(out, rows, n, ldo, "out", d),
+        _workspace(workspace, workspace_len, d), workspace_len, stream))
+
+
+def tree_accept_dev(tokens, parent, sampled, rows: int, starts, max_rows: int, kept, n_kept, next_tokens,
+                    stream: int | None = None) -> None:
+    """The nodes of each tree that its samples agree with: kept [n_trees,
+    max_rows], n_kept [n_trees], and the token that follows them.  All device
+    arrays of 32-bit integers; as many trees as n_kept has entries."""
+    d = starts.get_device()
+    n = n_kept.numel()
+    check(lib().rw_rocm_tree_accept_dev(
+        _dense(tokens, _I32, rows, "tokens", d, _U32), _dense(parent, _I32, rows, "parent", d),
+        _dense(sampled, _I32, rows, "sampled", d, _U32), rows, _dense(starts, _I32, n + 1, "starts", d), n, max_rows,
+        _dense(kept, _I32, n * max_rows, "kept", d), _dense(n_kept, _I32, n, "n_kept", d),
+        _dense(next_tokens, _I32, n, "next_tokens", d, _U32), stream))
+
+
+def kv_keep_rows_dev(pages: KvPages, table, past, kept, n_kept, seq=None, stream: int | None = None) -> None:
+    """Rows past[i] + kept[i, j] of sequence seq[i] (None: i) become its rows past[i] + j,
+    j < n_kept[i], in every layer.  Device int32; kept: [n_trees, any width]."""
+    d = pages.device
+    n, width = kept.shape
+    t, ld, n_seqs, s = _table_args(table, seq, n, d)
+    check(lib().rw_rocm_kv_keep_rows_dev(pages.st, t, ld, n_seqs, s, n, _dense(past, _I32, n, "past", d),
+                                         _dense(kept, _I32, n * width, "kept", d), width,
+                                         _dense(n_kept, _I32, n, "n_kept", d), stream))
 
 
 class KvBook:
@@ -848,6 +945,32 @@ def token_logprobs_dev(logits, rows: int, n_vocab: int, tokens, n_tok: int, logp
         _dense(entropy, _F32, rows, "entropy", d), k, _dense(top_ids, _I32, rows * k, "top_ids", d, _U32),
         _dense(top_logprobs, _F32, rows * k, "top_logprobs", d), _workspace(workspace, workspace_len, d),
         workspace_len, stream))
+
+
+def sample_tokens_workspace_size(rows: int, n_vocab: int) -> int:
+    return lib().rw_rocm_sample_tokens_workspace_size(rows, n_vocab)
+
+
+def sample_tokens_dev(logits, rows: int, n_vocab: int, u, tokens, logprobs=None, temperature=None, top_k=None,
+                      top_p=None, min_p=None, ld: int | None = None, dtype: int | None = None, workspace=None,
+                      workspace_len: int = 0, stream: int | None = None) -> None:
+    """A token per row of device logits, drawn with the uniform numbers u
+    [rows]; temperature, top_p, min_p: float32 [rows], top_k: int32 [rows] (None: off);
+    `dtype` is taken from a logits tensor (F32 for a pointer)."""
+    d = None
+    if hasattr(logits, "data_ptr"):
+        d = logits.get_device()
+        own = _TORCH_DTYPES.get(logits.dtype, -1)
+        if dtype is None:
+            dtype = own
+        elif dtype != own:
+            raise ValueError(f"dtype {dtype} for {logits.dtype} logits")
+    check(lib().rw_rocm_sample_tokens_dev(
+        F32 if dtype is None else dtype, *_rows(logits, rows, n_vocab, ld, "logits", d, _ANY_FLOAT), rows, n_vocab,
+        _dense(u, _F32, rows, "u", d), _dense(temperature, _F32, rows, "temperature", d),
+        _dense(top_k, _I32, rows, "top_k", d), _dense(top_p, _F32, rows, "top_p", d),
+        _dense(min_p, _F32, rows, "min_p", d), _dense(tokens, _I32, rows, "tokens", d, _U32),
+        _dense(logprobs, _F32, rows, "logprobs", d), _workspace(workspace, workspace_len, d), workspace_len, stream))
 
 
 MODEL_PARSE_ONLY = 1

@@ -1,7 +1,8 @@
 """Build recipe for the package's native libraries (run from __graft_entry__.build()).
 
   librw_rocm.so   hipcc, gfx950 only: csrc/rw_rocm.hip (+ rw_kernels.hpp),
-                  csrc/rw_serve.hip (+ rw_kv.hpp, rw_score.hpp) and the
+                  csrc/rw_serve.hip (+ rw_kv.hpp, rw_kv8.hpp, rw_score.hpp),
+                  csrc/rw_draft.hip (+ rw_tree.hpp, rw_keep.hpp, rw_sample.hpp) and the
                   host-only model loader csrc/rw_model.cpp, side by side
   _rw_quant*.so   g++: the C++ mirror of the reference's quant API
                   (host/rw_quant.cpp) with its pybind11 binding
@@ -59,7 +60,7 @@ def build_rocm(extra: list[str] | None = None) -> str:
     tmp = LIB_ROCM + ".tmp"
     with tempfile.TemporaryDirectory() as d:
         objs, jobs = [], []
-        for src in ("rw_rocm.hip", "rw_serve.hip", "rw_model.cpp"):
+        for src in ("rw_rocm.hip", "rw_serve.hip", "rw_draft.hip", "rw_model.cpp"):
             objs.append(os.path.join(d, src + ".o"))
             cmd = [HIPCC, *[f for f in flags if f != "-shared"], "-c", os.path.join(CSRC, src), "-o", objs[-1]]
             print("+", " ".join(cmd), flush=True)

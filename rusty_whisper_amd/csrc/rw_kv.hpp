@@ -28,6 +28,7 @@ struct PagedView {
   int n_seqs;
   int64_t ld;
   const int32_t *seq;    // [rows], or null: row r is sequence r
+  float *ks, *vs;        // the layer's scales [page][head][row], null: a pool without
 };
 
 #if defined(__HIPCC__)
@@ -126,7 +127,8 @@ struct KvPairs {
 // 16-byte pieces of page id[y], layer z / 2 of k (z even) or v; a page has
 // `piece` of them per layer.  700 pages of 1.57 MB over 24 layers: 430 us, 5.1
 // TB/s read and written, a large copy's rate.
-__global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t piece, int64_t n_pages, KvPairs pairs) {
+[[maybe_unused]] static __global__ __launch_bounds__(256) void k_kv_copy(uint4 *k, uint4 *v, int64_t piece, int64_t n_pages,
+                                                                         KvPairs pairs) {
   uint4 *base = (blockIdx.z & 1 ? v : k) + (int64_t)(blockIdx.z >> 1) * n_pages * piece;
   const int2 id = pairs.id[blockIdx.y];
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -3,125 +3,21 @@
 // book of pages) and the scoring of tokens.
 #include <hip/hip_runtime.h>
 
-#include <stdarg.h>
-#include <stdio.h>
-
 #include <algorithm>
 #include <new>
 #include <stdexcept>
 #include <vector>
 
-#include "rw_internal.hpp"
 #include "rw_kv.hpp"
+#include "rw_kv8.hpp"
 #include "rw_kvbook.hpp"
 #include "rw_rocm.h"
 #include "rw_score.hpp"
+#include "rw_serve.hpp"
 
 using namespace rw;
 
-static int fail(int code, const char *fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  return rw_internal_fail(code, buf);
-}
-
-#define SERVE_TRY(expr)  \
-  do {                   \
-    int rc_ = (expr);    \
-    if (rc_) return rc_; \
-  } while (0)
-
-static int launched(const char *what) {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? RW_OK : fail(RW_EHIP, "launch of %s: %s", what, hipGetErrorString(e));
-}
-
-static size_t cdiv(size_t a, size_t b) { return (a + b - 1) / b; }
-static bool aligned(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
-
-// rows (times heads) of one call: a workgroup of 256 threads each stays below
-// the 2^32 threads a launch may have
-constexpr size_t MOST_ROWS = (size_t)1 << 23;
-
-static int elem_size(int dtype) { return dtype == RW_F32 ? 4 : dtype == RW_F16 || dtype == RW_BF16 ? 2 : 0; }
-
-// ------------------------------------------------------------- checks
-
-// The current device, which has to hold `p` (an array of the call; `what`
-// names it): kernels that ran elsewhere would fault on it.
-static int call_device(const void *p, const char *what, int *dev) {
-  SERVE_TRY(rw_internal_current_device(dev));
-  hipPointerAttribute_t at{};
-  if (hipPointerGetAttributes(&at, p) != hipSuccess) {
-    (void)hipGetLastError();
-    return fail(RW_EINVAL, "%s is not device memory", what);
-  }
-  if (at.type == hipMemoryTypeUnregistered || at.type == hipMemoryTypeHost)
-    return fail(RW_EINVAL, "%s is not device memory", what);
-  if (at.type == hipMemoryTypeDevice && at.device != *dev)
-    return fail(RW_EINVAL, "%s is on device %d, the current device is %d", what, at.device, *dev);
-  return RW_OK;
-}
-
-static int check_pages(const rw_kv_pages *p) {
-  if (!p) return fail(RW_EINVAL, "pages is NULL");
-  if (!elem_size(p->dtype)) return fail(RW_EINVAL, "unsupported dtype %d (RW_F32, RW_F16 or RW_BF16)", p->dtype);
-  if (p->head_size != 32 && p->head_size != 64 && p->head_size != 96 && p->head_size != 128)
-    return fail(RW_EINVAL, "head_size %d: 32, 64, 96 or 128", p->head_size);
-  if (p->page_rows < 16 || p->page_rows > 256 || (p->page_rows & (p->page_rows - 1)))
-    return fail(RW_EINVAL, "page_rows %d: 16, 32, 64, 128 or 256", p->page_rows);
-  if (p->n_head < 1 || p->n_head > 65535) return fail(RW_EINVAL, "n_head %d: between 1 and 65535", p->n_head);
-  if (p->n_layer < 1 || p->n_layer > 32767) return fail(RW_EINVAL, "n_layer %zu: between 1 and 32767", p->n_layer);
-  if (p->n_pages < 1 || p->n_pages > (size_t)INT32_MAX) return fail(RW_EINVAL, "n_pages %zu: between 1 and 2^31 - 1", p->n_pages);
-  if (!p->k || !p->v || !aligned(p->k, 16) || !aligned(p->v, 16))
-    return fail(RW_EINVAL, "the pages' k and v must be 16-byte aligned device memory");
-  return RW_OK;
-}
-
-static int check_rows(const float *a, size_t ld, size_t n, const char *what) {
-  if (!a) return fail(RW_EINVAL, "%s is NULL", what);
-  if (ld < n || ld > ((size_t)1 << 40)) return fail(RW_EINVAL, "%s: row stride %zu for rows of %zu", what, ld, n);
-  if (ld % 4 || !aligned(a, 16)) return fail(RW_EINVAL, "%s rows must be 16-byte aligned", what);
-  return RW_OK;
-}
-
-static int check_table(const int32_t *table, size_t ld, size_t n_seqs, size_t rows, const int32_t *seq,
-                       const int32_t *at, const char *what) {
-  if (!table || !at) return fail(RW_EINVAL, "%s is NULL", table ? what : "table");
-  if (!aligned(table, 4) || !aligned(seq, 4) || !aligned(at, 4)) return fail(RW_EINVAL, "index arrays must be 4-byte aligned");
-  if (ld < 1 || n_seqs < 1 || ld > (size_t)INT32_MAX || n_seqs > (size_t)INT32_MAX)
-    return fail(RW_EINVAL, "a table of %zu sequences and %zu pages each", n_seqs, ld);
-  if (!seq && rows > n_seqs) return fail(RW_EINVAL, "%zu rows for a table of %zu sequences, and no seq", rows, n_seqs);
-  return RW_OK;
-}
-
-static PagedView paged_view(const rw_kv_pages *p, size_t layer, const int32_t *table, size_t ld, size_t n_seqs,
-                            const int32_t *seq) {
-  const size_t off = layer * p->n_pages * p->n_head * p->page_rows * p->head_size * elem_size(p->dtype);
-  return PagedView{(const char *)p->k + off, (const char *)p->v + off, p->n_head, p->head_size,
-                   __builtin_ctz((unsigned)p->page_rows), (int)p->n_pages, table, (int)n_seqs, (int64_t)ld, seq};
-}
-
-// calls f<E>() for the element type of `dtype`
-#define BY_TYPE(dtype, CALL)           \
-  do {                                 \
-    if ((dtype) == RW_F32) CALL(F32);  \
-    else if ((dtype) == RW_F16) CALL(F16); \
-    else CALL(BF16);                   \
-  } while (0)
-
 // ------------------------------------------------------------ attention
-
-static int check_paged_heads(const rw_kv_pages *p, size_t rows, int n_head, size_t max_len) {
-  if (n_head < 1 || n_head % p->n_head)
-    return fail(RW_EINVAL, "n_head %d is not a positive multiple of the pages' %d", n_head, p->n_head);
-  if (rows > MOST_ROWS / n_head) return fail(RW_EINVAL, "%zu rows of %d heads", rows, n_head);
-  if (max_len > (size_t)INT32_MAX) return fail(RW_EINVAL, "max_len %zu", max_len);
-  return RW_OK;
-}
 
 // How a launch cuts its rows' keys: chunks of `chunk` keys, `nsplit` of them
 // for the longest row.  `most`, of which the workspace's size is made, is no
@@ -152,7 +48,7 @@ static PagedPlan paged_plan(const rw_kv_pages *p, size_t rows, int n_head, size_
   const size_t group = (size_t)n_head / p->n_head;
   max_len = std::min(max_len, (size_t)1 << 30);
   L.base = rows * p->n_head * cdiv(group, 16);
-  const size_t bytes = max_len * 2 * p->head_size * elem_size(p->dtype);
+  const size_t bytes = max_len * 2 * p->head_size * pool_size(p->dtype);
   size_t nsplit = 1;
   if (bytes > (size_t)256 << 10) {
     nsplit = std::min(cdiv(bytes, (size_t)128 << 10), (size_t)PA_MAX_SPLIT / L.base);
@@ -208,33 +104,6 @@ static int launch_paged_dim(const PagedCall &c, const PagedPlan &L, hipStream_t 
     default: return launch_paged<E, 128>(c, L, s);
   }
 }
-
-// The workspace of a call: the caller's, or this stream's.  A stream that is
-// being captured has to bring one: the library's may be replaced by a later
-// call while the graph still uses it.
-struct CallWorkspace {
-  void *slot = nullptr;
-  CallWorkspace() = default;
-  CallWorkspace(const CallWorkspace &) = delete;
-  CallWorkspace &operator=(const CallWorkspace &) = delete;
-  ~CallWorkspace() {
-    if (slot) rw_internal_workspace_release(slot);
-  }
-  int take(int dev, void *given, size_t len, size_t need, void *stream, void **out) {
-    *out = given;
-    if (need == 0) return RW_OK;
-    if (given) {
-      if (len < need) return fail(RW_EINVAL, "workspace of %zu bytes < %zu needed", len, need);
-      if (!aligned(given, 16)) return fail(RW_EINVAL, "the workspace must be 16-byte aligned");
-      return RW_OK;
-    }
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    const hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &st);
-    if (e != hipSuccess) return fail(RW_EHIP, "hipStreamIsCapturing: %s", hipGetErrorString(e));
-    if (st != hipStreamCaptureStatusNone) return fail(RW_EINVAL, "a captured call needs a workspace of %zu bytes", need);
-    return rw_internal_workspace(dev, stream, need, &slot, out);
-  }
-};
 
 // ------------------------------------------------------------- scores
 
@@ -299,6 +168,36 @@ static int launch_score(const ScoreCall &c, const ScorePlan &L, hipStream_t s) {
   return launched("k_score_join");
 }
 
+// --------------------------------------------------------- 8-bit writes
+
+template <class E>
+static int launch_write8_of(const PagedView &w, const float *k, size_t ldk, const float *v, size_t ldv, size_t rows,
+                            const int32_t *pos, hipStream_t s) {
+  const size_t most = MOST_ROWS / w.heads * K8_ROWS;  // rows of one launch
+  for (size_t row0 = 0; row0 < rows; row0 += most) {
+    const size_t tiles = cdiv(std::min(most, rows - row0), K8_ROWS) * w.heads;
+    const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
+#define RW_WRITE8(DH)                                                                                              \
+  hipLaunchKernelGGL((k_kv_write8<E, DH>), grid, dim3(256), 0, s, w, k, (int64_t)ldk, v, (int64_t)ldv, (int)rows, pos, \
+                     (int)tiles, (int)row0)
+    switch (w.dim) {
+      case 32: RW_WRITE8(32); break;
+      case 64: RW_WRITE8(64); break;
+      case 96: RW_WRITE8(96); break;
+      default: RW_WRITE8(128); break;
+    }
+#undef RW_WRITE8
+    SERVE_TRY(launched("k_kv_write8"));
+  }
+  return RW_OK;
+}
+
+static int launch_write8(int dtype, const PagedView &w, const float *k, size_t ldk, const float *v, size_t ldv, size_t rows,
+                         const int32_t *pos, hipStream_t s) {
+  return dtype == RW_I8 ? launch_write8_of<I8>(w, k, ldk, v, ldv, rows, pos, s)
+                        : launch_write8_of<E4M3>(w, k, ldk, v, ldv, rows, pos, s);
+}
+
 // ----------------------------------------------------------------- book
 
 struct rw_kv_book {
@@ -347,6 +246,7 @@ int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k,
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
   const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
+  if (scaled(pages->dtype)) return launch_write8(pages->dtype, w, k, ldk, v, ldv, rows, pos, (hipStream_t)stream);
   const size_t cols = cdiv(n, KV_COLS), most = MOST_ROWS / cols * KV_ROWS;  // rows of one launch
   for (size_t row0 = 0; row0 < rows; row0 += most) {
     const size_t tiles = cdiv(std::min(most, rows - row0), KV_ROWS) * cols;
@@ -357,6 +257,36 @@ int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k,
     BY_TYPE(pages->dtype, RW_WRITE);
 #undef RW_WRITE
     SERVE_TRY(launched("k_kv_write"));
+  }
+  return RW_OK;
+}
+
+int rw_rocm_kv_read_dev(const rw_kv_pages *pages, size_t layer, float *k, size_t ldk, float *v, size_t ldv, size_t rows,
+                        const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq, const int32_t *pos,
+                        void *stream) {
+  SERVE_TRY(check_pages(pages));
+  if (layer >= pages->n_layer) return fail(RW_EINVAL, "layer %zu of %zu", layer, pages->n_layer);
+  if (rows == 0) return RW_OK;
+  if (rows > MOST_ROWS) return fail(RW_EINVAL, "rows = %zu: at most %zu", rows, MOST_ROWS);
+  const size_t n = (size_t)pages->n_head * pages->head_size;
+  SERVE_TRY(check_rows(k, ldk, n, "k"));
+  SERVE_TRY(check_rows(v, ldv, n, "v"));
+  SERVE_TRY(check_table(table, ld_table, n_seqs, rows, seq, pos, "pos"));
+  int dev;
+  SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
+  const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
+  const size_t cols = cdiv(n, KV_COLS), most = MOST_ROWS / cols * KV_ROWS;  // rows of one launch
+  for (size_t row0 = 0; row0 < rows; row0 += most) {
+    const size_t tiles = cdiv(std::min(most, rows - row0), KV_ROWS) * cols;
+    const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
+#define RW_READ(E)                                                                                                \
+  hipLaunchKernelGGL((k_kv_read<E>), grid, dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v, (int64_t)ldv, \
+                     (int)rows, pos, (int)cols, (int)tiles, (int)row0)
+    if (pages->dtype == RW_I8) RW_READ(I8);
+    else if (pages->dtype == RW_E4M3) RW_READ(E4M3);
+    else BY_TYPE(pages->dtype, RW_READ);
+#undef RW_READ
+    SERVE_TRY(launched("k_kv_read"));
   }
   return RW_OK;
 }
@@ -387,7 +317,8 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
   }
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
-  const size_t piece = (size_t)pages->n_head * pages->page_rows * pages->head_size * elem_size(pages->dtype) / 16;
+  const size_t page_rows = (size_t)pages->n_head * pages->page_rows;  // of one head
+  const size_t piece = page_rows * pages->head_size * pool_size(pages->dtype) / 16;
   for (size_t i0 = 0; i0 < n; i0 += KV_PAIRS) {
     const size_t m = std::min((size_t)KV_PAIRS, n - i0);
     KvPairs pairs{};
@@ -396,12 +327,18 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
                        dim3(256), 0, (hipStream_t)stream, (uint4 *)pages->k, (uint4 *)pages->v, (int64_t)piece,
                        (int64_t)pages->n_pages, pairs);
     SERVE_TRY(launched("k_kv_copy"));
+    if (!scaled(pages->dtype)) continue;
+    hipLaunchKernelGGL(k_kv_copy, dim3((unsigned)cdiv(page_rows / 4, 256), (unsigned)m, (unsigned)(2 * pages->n_layer)),
+                       dim3(256), 0, (hipStream_t)stream, (uint4 *)pages->k_scale, (uint4 *)pages->v_scale,
+                       (int64_t)(page_rows / 4), (int64_t)pages->n_pages, pairs);
+    SERVE_TRY(launched("k_kv_copy"));
   }
   return RW_OK;
 }
 
 size_t rw_rocm_paged_attention_workspace_size(const rw_kv_pages *pages, size_t rows, int n_head, size_t max_len) {
   if (check_pages(pages) || check_paged_heads(pages, rows, n_head, max_len) || rows == 0) return 0;
+  if (scaled(pages->dtype)) return tree_workspace(pages, n_head, rows, rows, 1, max_len);
   return paged_bytes(paged_plan(pages, rows, n_head, max_len), rows, n_head, pages->head_size);
 }
 
@@ -419,6 +356,14 @@ int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const fl
   SERVE_TRY(check_table(table, ld_table, n_seqs, rows, seq, len, "len"));
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
+  if (scaled(pages->dtype)) {
+    CallWorkspace hold;
+    void *ws = nullptr;
+    SERVE_TRY(hold.take(dev, workspace, workspace_len, tree_workspace(pages, n_head, rows, rows, 1, max_len), stream, &ws));
+    return tree_launch(TreeCall{paged_view(pages, layer, table, ld_table, n_seqs, seq), pages->dtype, q, (int64_t)ldq, rows,
+                                n_head, rows, nullptr, len, 1, nullptr, 0, max_len, out, (int64_t)ldo},
+                       pages, ws, (hipStream_t)stream);
+  }
   PagedCall c{paged_view(pages, layer, table, ld_table, n_seqs, seq), q, (int64_t)ldq, (int)rows, n_head, 0, len, out,
               (int64_t)ldo, nullptr};
   c.max_len = (int)std::min(max_len, std::min((size_t)1 << 30, ld_table * pages->page_rows));

@@ -1,0 +1,609 @@
+// rw_tree.hpp -- attention of several new tokens per sequence over keys and values
+// in pages: trees of drafted tokens (a mask), chunks of prompts (each token sees
+// those before it), and single tokens over 8-bit pages.
+//
+// Row j of tree i sees the rows 0 .. past - 1 of its sequence and, of the tree's own
+// (rows past .. past + nodes - 1 of the sequence), those that its mask's bits name, or 0 .. j
+// without a mask.  The queries of a tree and key head (rows x query heads of the
+// head) are counted together and cut into tiles of 16: the columns of the scores'
+// products, as in rw_kv.hpp, whose operands, precision and treatment of sums this
+// follows; 8-bit pools differ:
+//   keys    as f16, which has all their values, times q in 2 f16 parts (22 bits and
+//           more of every value down to 2^-29 of its query's largest); the score times the key's scale
+//   values  as bf16, which has them too, times p s in 2 bf16 parts (p's weight, s the value's
+//           scale): the second part is rounded, so a weight is off by 2^-17 of itself at most and
+//           on neither side, where the values themselves are off by 2^-8 of their row's largest.
+//           (A third part would cost half a product more and change nothing that the pool can show.)
+#pragma once
+#include "rw_kv8.hpp"
+
+namespace rw {
+
+#if defined(__HIPCC__)
+
+
+// 8 values of a pool of 8 bits, as f16 and as bf16: both exact
+template <class E>
+struct Kv8;
+template <>
+struct Kv8<I8> {
+  static __device__ PaTile<F16>::Op f16(u32x2 a) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // x + 128 below the bits of 1024: 1152 + x
+      const uint32_t u = a[i >> 1] ^ 0x80808080u;
+      const uint32_t b = __builtin_amdgcn_perm(0x64646464u, u, i & 1 ? 0x04030402u : 0x04010400u);
+      const h2 x = __builtin_bit_cast(h2, b) - (_Float16)1152.0f;
+      o[i] = __builtin_bit_cast(uint32_t, x);
+    }
+    return __builtin_bit_cast(PaTile<F16>::Op, o);
+  }
+  static __device__ PaTile<BF16>::Op bf16(u32x2 a) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int w = (int)a[i >> 1], s = 16 * (i & 1);
+      const float x0 = (float)(int8_t)(w >> s), x1 = (float)(int8_t)(w >> (s + 8));
+      o[i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
+    }
+    return __builtin_bit_cast(PaTile<BF16>::Op, o);
+  }
+  static constexpr bool FINITE = true;  // no code is an infinity or a NaN
+};
+template <>
+struct Kv8<E4M3> {
+  static __device__ PaTile<F16>::Op f16(u32x2 a) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = i & 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)a[i >> 1], 1.0f, true))
+                   : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)a[i >> 1], 1.0f, false));
+    return __builtin_bit_cast(PaTile<F16>::Op, o);
+  }
+  static __device__ PaTile<BF16>::Op bf16(u32x2 a) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = i & 1 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)a[i >> 1], 1.0f, true))
+                   : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)a[i >> 1], 1.0f, false));
+    return __builtin_bit_cast(PaTile<BF16>::Op, o);
+  }
+  static constexpr bool FINITE = false;
+};
+
+struct TreeArgs {
+  const void *k, *v;
+  const float *ks, *vs;
+  const float *q;
+  float *out, *part;
+  const int32_t *table, *seq, *starts, *past;
+  const uint32_t *mask;
+  int64_t ldq, ldo, ld_table;
+  int n_words, rows, n_trees, max_rows, kv_heads, group, pr, n_pages, n_seqs, max_len, chunk, qtiles;
+};
+
+// What tree i of a call is: its first row, its rows in this launch, the rows of
+// the sequence before it, the rows it may see, its row of the table.
+struct TreeSpan {
+  int start, rows, past, n;
+  const int32_t *table;
+};
+__device__ inline TreeSpan tree_span(const TreeArgs &a, int i) {
+  constexpr int MOST = 1 << 30;
+  TreeSpan s;
+  const int sq = a.seq ? a.seq[i] : i;
+  const int most = (int)min((int64_t)min(MOST, a.max_len), a.ld_table << a.pr);
+  s.past = min(a.past[i], MOST);
+  int nodes = 0;
+  if (a.starts) {
+    s.start = a.starts[i];
+    nodes = s.start < 0 ? 0 : max(0, min(a.starts[i + 1], a.rows) - s.start);
+    s.rows = min(nodes, a.max_rows);
+  } else {
+    s.start = i, s.rows = 1;
+  }
+  s.n = s.past < 0 || (unsigned)sq >= (unsigned)a.n_seqs ? 0 : min(s.past + nodes, most);
+  s.table = a.table + (int64_t)((unsigned)sq < (unsigned)a.n_seqs ? sq : 0) * a.ld_table;
+  return s;
+}
+// the end of the keys that the queries u0 .. u1 - 1 of a tree see
+__device__ inline int tree_end(const TreeArgs &a, const TreeSpan &s, int u1) {
+  if (!a.starts || a.mask) return s.n;
+  return min(s.n, s.past + (u1 - 1) / a.group + 1);
+}
+// Bits 0 .. PER - 1: whether a row (`node` of its tree, `mask` its words) sees the
+// keys a0 .. a0 + PER - 1
+template <int PER>
+__device__ inline uint32_t tree_sees(const TreeArgs &a, const TreeSpan &s, const uint32_t *mask, int node, int a0) {
+  constexpr uint32_t ALL = PER == 32 ? ~0u : (1u << PER) - 1;
+  const int b = a0 - s.past;
+  uint32_t bits = ALL;
+  if (b > -PER && a.starts) {
+    if (!a.mask) {
+      const int c = node + 1 - b;  // how many of them
+      bits = c <= 0 ? 0 : c >= PER ? ALL : (1u << c) - 1;
+    } else {
+      const int w = max(b, 0) >> 5;
+      const uint32_t lo = w < a.n_words ? mask[w] : 0, hi = w + 1 < a.n_words ? mask[w + 1] : 0;
+      const uint64_t both = ((uint64_t)hi << 32) | lo;
+      bits = b < 0 ? (lo << -b) | ((1u << -b) - 1) : (uint32_t)(both >> (b & 31));
+    }
+  }
+  const int c = s.n - a0;
+  return bits & (c <= 0 ? 0 : c >= PER ? ALL : (1u << c) - 1);
+}
+
+// How a pool's tiles of keys enter the two products.  Lane 16 h + r of a
+// wavefront holds of a tile's KEYS keys the scores of PER h .. PER h + PER - 1 for
+// query r, and their values 16 i + r.
+template <class E, int DH>
+struct TreeTile {
+  using M = PaTile<E>;
+  using T = typename E::T;
+  using QOp = typename M::Op;   // of the scores' product
+  using VM = PaTile<std::conditional_t<sizeof(T) == 2, BF16, E>>;  // of the second one's weights
+  static constexpr bool SCALED = false, WIDE = M::WIDE;
+  static constexpr int KEYS = M::KEYS, SUB = M::SUB, PER = 4 * SUB, PARTS = M::PARTS, SUMS = M::SUMS, STEPS = DH / M::STEP;
+  static constexpr int VAL = M::PER;  // values per lane and step
+  static constexpr float MOVE = M::MOVE;
+  typename M::Op kr[SUB][STEPS], vr[DH / 16];
+  // the first value of step c for the lanes of `h`
+  static __device__ int value(int c, int h) { return M::STEP * c + VAL * h; }
+  __device__ void load_k(const void *base, int64_t at, int s, int slot, int h) {
+    const T *p = (const T *)base + at + (int64_t)slot * DH;
+#pragma unroll
+    for (int c = 0; c < STEPS; ++c) kr[s][c] = *(const typename M::Op *)(p + value(c, h));
+  }
+  __device__ void load_v(const void *base, int64_t at, int slot, int r, int pr) {
+    const T *p = (const T *)base + at + ((int64_t)r << pr) + slot;
+#pragma unroll
+    for (int i = 0; i < DH / 16; ++i) vr[i] = *(const typename M::Op *)(p + ((16 * i) << pr));
+  }
+  __device__ QOp k(int s, int c) const { return kr[s][c]; }
+  static __device__ f4 mma(QOp a, QOp b, f4 c) { return M::mma(a, b, c); }
+  static __device__ void q_parts(const float (&x)[VAL], QOp (&o)[PARTS]) { pa_parts<E>(x, o); }
+  // keys without a row behind them: nothing of what memory holds there
+  __device__ void clear_v(int i, int j) { vr[i][j] = (T)0.0f; }
+  // the bits of values 16 i + r that are infinities or NaN, which are then cleared
+  __device__ uint32_t take_odd(int i) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (!__builtin_isfinite((float)vr[i][j])) odd |= 1u << j, clear_v(i, j);
+    return odd;
+  }
+  // how many keys both bits are set of
+  static __device__ f4 count(uint32_t w, uint32_t v) {
+    typename VM::Op a, b;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      a[j] = (typename VM::T)(w >> j & 1 ? 1.0f : 0.0f);
+      b[j] = (typename VM::T)(v >> j & 1 ? 1.0f : 0.0f);
+    }
+    return VM::mma(a, b, f4{0.0f, 0.0f, 0.0f, 0.0f});
+  }
+  __device__ void add(const float (&p)[PER], f4 (&o)[DH / 16]) const { pa_add<E>(p, vr, o); }
+};
+
+template <class E, int DH>
+struct TreeTile8 {
+  using M = PaTile<F16>;
+  using T = typename E::T;
+  using QOp = M::Op;
+  using VM = PaTile<BF16>;
+  static constexpr bool SCALED = true, WIDE = true;
+  static constexpr int KEYS = 64, SUB = 4, PER = 16, PARTS = 2, SUMS = 2, STEPS = DH / 32, VAL = 8;
+  static constexpr float MOVE = 0x1p11f;
+  u32x4 kr[SUB][(DH + 63) / 64], vr[DH / 16];
+  // 16 bytes per lane are the values of two steps, 8 those of a last odd one
+  static __device__ int value(int c, int h) {
+    return c < DH / 64 * 2 ? 64 * (c / 2) + 16 * h + 8 * (c & 1) : 32 * c + 8 * h;
+  }
+  __device__ void load_k(const void *base, int64_t at, int s, int slot, int h) {
+    const T *p = (const T *)base + at + (int64_t)slot * DH;
+#pragma unroll
+    for (int c = 0; c < DH / 64; ++c) kr[s][c] = *(const u32x4 *)(p + 64 * c + 16 * h);
+    if (DH % 64) {
+      const u32x2 x = *(const u32x2 *)(p + DH / 64 * 64 + 8 * h);
+      kr[s][DH / 64] = u32x4{x[0], x[1], 0, 0};
+    }
+  }
+  __device__ void load_v(const void *base, int64_t at, int slot, int r, int pr) {
+    const T *p = (const T *)base + at + ((int64_t)r << pr) + slot;
+#pragma unroll
+    for (int i = 0; i < DH / 16; ++i) vr[i] = *(const u32x4 *)(p + ((16 * i) << pr));
+  }
+  __device__ QOp k(int s, int c) const {
+    const u32x4 x = kr[s][c / 2];
+    return Kv8<E>::f16(c & 1 ? u32x2{x[2], x[3]} : u32x2{x[0], x[1]});
+  }
+  static __device__ f4 mma(QOp a, QOp b, f4 c) { return M::mma(a, b, c); }
+  static __device__ void q_parts(const float (&x)[VAL], QOp (&o)[PARTS]) {
+#pragma unroll
+    for (int j = 0; j < VAL; ++j) {
+      o[0][j] = (_Float16)x[j];
+      o[1][j] = (_Float16)((x[j] - (float)o[0][j]) * MOVE);
+    }
+  }
+  __device__ void clear_v(int i, int j) { vr[i][j >> 2] &= ~(0xFFu << (8 * (j & 3))); }
+  __device__ uint32_t take_odd(int i) {
+    uint32_t odd = 0;
+    if (!Kv8<E>::FINITE)
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (((vr[i][j >> 2] >> (8 * (j & 3))) & 0x7F) == 0x7F) odd |= 1u << j, clear_v(i, j);
+    return odd;
+  }
+  static __device__ f4 count(uint32_t w, uint32_t v) {
+    f4 c{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < PER; u += 8) {
+      VM::Op a, b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        a[j] = (__bf16)(w >> (u + j) & 1 ? 1.0f : 0.0f);
+        b[j] = (__bf16)(v >> (u + j) & 1 ? 1.0f : 0.0f);
+      }
+      c = VM::mma(a, b, c);
+    }
+    return c;
+  }
+  __device__ void add(const float (&p)[PER], f4 (&o)[DH / 16]) const {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      VM::Op hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        hi[j] = VM::part(p[8 * u + j]);
+        lo[j] = (__bf16)(p[8 * u + j] - (float)hi[j]);
+      }
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i) {
+        const VM::Op b = Kv8<E>::bf16(u ? u32x2{vr[i][2], vr[i][3]} : u32x2{vr[i][0], vr[i][1]});
+        o[i] = VM::mma(lo, b, o[i]);
+        o[i] = VM::mma(hi, b, o[i]);
+      }
+    }
+  }
+};
+template <int DH>
+struct TreeTile<I8, DH> : TreeTile8<I8, DH> {};
+template <int DH>
+struct TreeTile<E4M3, DH> : TreeTile8<E4M3, DH> {};
+
+// One workgroup of PA_WAVES wavefronts per (tree, key/value head, QT tiles of 16
+// queries, chunk of keys).  A wavefront takes every PA_WAVES-th tile of keys, straight from memory, for
+// all of the workgroup's queries.
+template <class E, int DH, int QT>
+__global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(TreeArgs a) {
+  using M = TreeTile<E, DH>;
+  using QOp = typename M::QOp;
+  constexpr int ND = DH / 16, KEYS = M::KEYS, PER = M::PER, SUB = M::SUB, PARTS = M::PARTS, VAL = M::VAL;
+  constexpr int LD = DH + 4, NQ = 16 * QT;
+  constexpr float NEG_INF = -__builtin_huge_valf();
+  __shared__ float so[PA_WAVES][NQ][LD], sm[PA_WAVES][NQ], sl[PA_WAVES][NQ];
+
+  // the query tiles of one (tree, head) run eight workgroups apart, on one XCD
+  const int qi = blockIdx.x / 8 % a.qtiles, item = blockIdx.x / (8 * a.qtiles) * 8 + blockIdx.x % 8;
+  const int hk = item % a.kv_heads, tree = item / a.kv_heads;
+  if (tree >= a.n_trees) return;
+  const TreeSpan sp = tree_span(a, tree);
+  const int u0 = qi * NQ, all = sp.rows * a.group, nq = min(NQ, all - u0);
+  if (nq <= 0) return;
+  const int lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.kv_heads * a.group;
+  const int n = tree_end(a, sp, u0 + nq);
+  // query i of this workgroup: its row and head
+  auto row_of = [&](int i) { return sp.start + (u0 + i) / a.group; };
+  auto head_of = [&](int i) { return hk * a.group + (u0 + i) % a.group; };
+  if (n <= 0) {
+    if (blockIdx.y == 0)
+      for (int i = threadIdx.x; i < nq * DH; i += 64 * PA_WAVES)
+        a.out[row_of(i / DH) * a.ldo + (int64_t)head_of(i / DH) * DH + i % DH] = 0.0f;
+    return;
+  }
+  const int k0 = blockIdx.y * a.chunk;
+  if (k0 >= n) return;
+  const bool direct = n <= a.chunk;
+  const int end = (min(n, k0 + a.chunk) + KEYS - 1) / KEYS;
+  const int P = 1 << a.pr;
+
+  // the pages of this lane's k rows (keys PER (r / 4) on of a tile) and of its values (PER h on)
+  struct Where {
+    int64_t k, v;  // first row of the head, in rows of DH
+    bool bad;      // the page of the lane's values, and scores, is not in the pool
+  };
+  auto where = [&](int t) __attribute__((always_inline)) {
+    Where w;
+    const int pk = sp.table[min(t * KEYS + PER * (r >> 2), n - 1) >> a.pr], pv = sp.table[min(t * KEYS + PER * h, n - 1) >> a.pr];
+    const bool bk = (unsigned)pk >= (unsigned)a.n_pages;
+    w.bad = (unsigned)pv >= (unsigned)a.n_pages;
+    w.k = ((int64_t)(bk ? 0 : pk) * a.kv_heads + hk) << a.pr;
+    w.v = ((int64_t)(w.bad ? 0 : pv) * a.kv_heads + hk) << a.pr;
+    return w;
+  };
+  M tile;
+  f4 ksc[M::SCALED ? SUB : 1], vsc[M::SCALED ? SUB : 1];
+  auto load_k = [&](int t, const Where &w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) tile.load_k(a.k, w.k * DH, s, (t * KEYS + PER * (r >> 2) + 4 * s + (r & 3)) & (P - 1), h);
+  };
+  auto load_v = [&](int t, const Where &w) __attribute__((always_inline)) {
+    const int slot = (t * KEYS + PER * h) & (P - 1);
+    tile.load_v(a.v, w.v * DH, slot, r, a.pr);
+    if constexpr (M::SCALED)
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) ksc[s] = *(const f4 *)(a.ks + w.v + slot + 4 * s), vsc[s] = *(const f4 *)(a.vs + w.v + slot + 4 * s);
+  };
+
+  const int t0 = k0 / KEYS + wv;
+  int t = t0;
+  Where now{};
+  if (t < end) now = where(t), load_k(t, now);
+
+  // q, in the scores' operand order; f16 parts: each query's values scaled by a
+  // power of two so that the largest lies in [2^14, 2^15), undone in `c`
+  QOp qf[QT][PARTS][M::STEPS];
+  float c[QT];
+  const uint32_t *mask[QT];
+  int node[QT];
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    const int i = min(16 * x + r, nq - 1);
+    const bool real = 16 * x + r < nq;
+    node[x] = (u0 + i) / a.group;
+    mask[x] = a.mask ? a.mask + (int64_t)row_of(i) * a.n_words : nullptr;
+    c[x] = PA_LOG2E / __builtin_sqrtf((float)DH);
+    float y[M::STEPS][VAL], top = 0.0f;
+    const float *p = a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH;
+#pragma unroll
+    for (int s = 0; s < M::STEPS; ++s)
+#pragma unroll
+      for (int j = 0; j < VAL; j += 4) {
+        const f4 z = *(const f4 *)(p + M::value(s, h) + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[s][j + e] = real ? z[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(y[s][j + e]));
+      }
+    int e = 0;
+    if (M::MOVE != 1.0f) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+      c[x] = ldexpf(c[x], e);
+    }
+#pragma unroll
+    for (int s = 0; s < M::STEPS; ++s) {
+      QOp o[PARTS];
+      if (M::MOVE != 1.0f)
+#pragma unroll
+        for (int j = 0; j < VAL; ++j) y[s][j] = ldexpf(y[s][j], -e);
+      M::q_parts(y[s], o);
+#pragma unroll
+      for (int k = 0; k < PARTS; ++k) qf[x][k][s] = o[k];
+    }
+  }
+
+  for (float scale = 1.0f;; scale = PA_LOW) {
+    f4 o[QT][ND];
+    float m[QT], sum[QT];  // of query r; sum: of this lane's keys
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[x][i] = {};
+      m[x] = NEG_INF, sum[x] = 0.0f;
+    }
+
+    for (; t < end; t += PA_WAVES) {
+      load_v(t, now);
+      const bool more = t + PA_WAVES < end;
+      Where next{};
+      if (more) next = where(t + PA_WAVES);
+      f4 s[QT][M::SUMS][SUB];
+#pragma unroll
+      for (int x = 0; x < QT; ++x)
+#pragma unroll
+        for (int k = 0; k < M::SUMS; ++k)
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) s[x][k][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < M::STEPS; ++i)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          const QOp kk = tile.k(u, i);
+#pragma unroll
+          for (int x = 0; x < QT; ++x)
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) s[x][k % M::SUMS][u] = M::mma(kk, qf[x][k][i], s[x][k % M::SUMS][u]);
+        }
+      if (more) load_k(t + PA_WAVES, next);
+
+      // keys that no query of the call may see, or that are in no page of the pool: no
+      // weight, and what v holds there (anything) is taken as zero
+      const int a0 = t * KEYS + PER * h;
+      const bool edge = (t + 1) * KEYS > min(n, sp.past) || __builtin_amdgcn_ballot_w64(now.bad);
+      bool odd_any = false;
+      uint32_t odd[(ND + 1) / 2] = {};  // 16 bits for each i
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (now.bad || a0 + j >= n) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) tile.clear_v(i, j);
+          }
+        // a row that one query sees and another does not may hold infinities or NaN:
+        // they leave the products and are given to those who see them
+#pragma unroll
+        for (int i = 0; i < ND; ++i) odd[i / 2] |= tile.take_odd(i) << (16 * (i & 1));
+#pragma unroll
+        for (int i = 0; i < (ND + 1) / 2; ++i) odd_any |= odd[i] != 0;
+        odd_any = __builtin_amdgcn_ballot_w64(odd_any) != 0;
+      }
+#pragma unroll
+      for (int x = 0; x < QT; ++x) {
+        float y[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          y[j] = s[x][M::SUMS - 1][j >> 2][j & 3];
+#pragma unroll
+          for (int k = M::SUMS - 2; k >= 0; --k) y[j] = fmaf(y[j], 1.0f / M::MOVE, s[x][k][j >> 2][j & 3]);
+          y[j] *= c[x];
+          if constexpr (M::SCALED) y[j] *= ksc[j >> 2][j & 3];
+        }
+        uint32_t sees = ~0u;
+        if (edge) {
+          sees = now.bad ? 0 : tree_sees<PER>(a, sp, mask[x], node[x], a0);
+#pragma unroll
+          for (int j = 0; j < PER; ++j)
+            if (!(sees >> j & 1)) y[j] = NEG_INF;
+        }
+        float top = y[0];
+#pragma unroll
+        for (int j = 1; j < PER; ++j) top = fmaxf(top, y[j]);
+        if (__builtin_amdgcn_ballot_w64(top > m[x] + PA_SLACK)) {
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
+          const float up = fmaxf(m[x], top), f = pa_weight(m[x], up);
+          m[x] = up;
+          sum[x] *= f;
+          f4 fr;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
+#pragma unroll
+          for (int i = 0; i < ND; ++i) o[x][i] *= fr;
+        }
+        const float base = m[x] == NEG_INF ? 0.0f : m[x];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          y[j] = __builtin_amdgcn_exp2f(y[j] - base);
+          if (M::WIDE) y[j] *= scale;
+          sum[x] += y[j];
+          if constexpr (M::SCALED) y[j] = edge && !(sees >> j & 1) ? 0.0f : y[j] * vsc[j >> 2][j & 3];
+        }
+        tile.add(y, o[x]);
+        if (odd_any) {
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const f4 z = M::count(sees, odd[i / 2] >> (16 * (i & 1)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (z[e] > 0.0f) o[x][i][e] = __builtin_nanf("");
+          }
+        }
+      }
+      now = next;
+    }
+
+    // the wavefront's means
+    const bool first = scale == 1.0f;
+    bool over = false;
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+      sum[x] += __shfl_xor(sum[x], 16);
+      sum[x] += __shfl_xor(sum[x], 32);
+      if (first && h == 0) sm[wv][16 * x + r] = m[x], sl[wv][16 * x + r] = sum[x];
+      const float inv = sum[x] == 0.0f ? 0.0f : 1.0f / sum[x];  // 0: no keys
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int qr = 16 * x + 4 * h + i;
+        const float f = __shfl(inv, 4 * h + i);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const float y = o[x][d][i] * f;
+          float &mean = so[wv][qr][16 * d + r];
+          if (!M::WIDE || first) mean = y;
+          else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(o[x][d][i]) ? pa_largest(y) : y;
+          over |= qr < nq && !__builtin_isfinite(y);
+        }
+      }
+    }
+    if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
+    t = t0;
+    if (t < end) now = where(t), load_k(t, now);
+  }
+  __syncthreads();
+
+  // the wavefronts' means, each with its share of the weights
+  const int64_t runs = (int64_t)a.rows * heads * gridDim.y;
+  for (int i = threadIdx.x; i < nq * DH; i += 64 * PA_WAVES) {
+    const int qr = i / DH, d = i % DH;
+    float top = sm[0][qr], l = 0.0f, y = 0.0f, w[PA_WAVES];
+#pragma unroll
+    for (int k = 1; k < PA_WAVES; ++k) top = fmaxf(top, sm[k][qr]);
+#pragma unroll
+    for (int k = 0; k < PA_WAVES; ++k) l += w[k] = sl[k][qr] * pa_weight(sm[k][qr], top);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: nothing is seen
+#pragma unroll
+    for (int k = 0; k < PA_WAVES; ++k) y += so[k][qr][d] * (w[k] * inv);
+    if (M::WIDE && __builtin_isinf(y)) {
+      bool finite = true;
+#pragma unroll
+      for (int k = 0; k < PA_WAVES; ++k) finite &= (bool)__builtin_isfinite(so[k][qr][d]);
+      if (finite) y = pa_largest(y);
+    }
+    if (direct) {
+      a.out[row_of(qr) * a.ldo + (int64_t)head_of(qr) * DH + d] = y;
+    } else {
+      const int64_t run = ((int64_t)row_of(qr) * heads + head_of(qr)) * gridDim.y + blockIdx.y;
+      a.part[run * DH + d] = y;
+      if (d == 0) a.part[runs * DH + 2 * run] = top, a.part[runs * DH + 2 * run + 1] = l;
+    }
+  }
+}
+
+// The chunks of one query, joined as k_paged_join joins them.  blockIdx.x = (tree x
+// max_rows + row of the tree) x heads + head; nq: queries per workgroup of k_tree_attn.
+template <int DH>
+__global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int nsplit, int nq) {
+  constexpr int W = DH <= 32 ? 8 : DH <= 64 ? 16 : 32, SIDE = 256 / W;  // W threads of 4 values
+  __shared__ float sw[PA_MAX_SPLIT], sl[4];
+  __shared__ f4 sy[SIDE][DH / 4];
+  const int heads = a.kv_heads * a.group, most = a.starts ? a.max_rows : 1;
+  const int hq = blockIdx.x % heads, tree = blockIdx.x / heads / most, j = blockIdx.x / heads % most;
+  const TreeSpan sp = tree_span(a, tree);
+  if (j >= sp.rows) return;
+  const int u = j * a.group + hq % a.group;
+  const int n = tree_end(a, sp, min(u / nq * nq + nq, sp.rows * a.group));
+  if (n <= a.chunk) return;
+  const int nz = (n + a.chunk - 1) / a.chunk;  // <= nsplit <= PA_MAX_SPLIT
+  const int64_t row = sp.start + j, run0 = (row * heads + hq) * nsplit, runs = (int64_t)a.rows * heads * nsplit;
+  const float *ml = a.part + runs * DH + 2 * run0;
+  float top = -__builtin_huge_valf(), l = 0.0f;
+  for (int z = threadIdx.x & 63; z < nz; z += 64) top = fmaxf(top, ml[2 * z]);
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  for (int z = threadIdx.x; z < nz; z += 256) {
+    const float w = ml[2 * z + 1] * pa_weight(ml[2 * z], top);
+    sw[z] = w;
+    l += w;
+  }
+  for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+  if ((threadIdx.x & 63) == 0) sl[threadIdx.x >> 6] = l;
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int g = threadIdx.x / W, d = threadIdx.x % W;
+  if (d < DH / 4) {
+    f4 y{0.0f, 0.0f, 0.0f, 0.0f};
+    const f4 *o = (const f4 *)(a.part + run0 * DH) + d;
+#pragma unroll 4
+    for (int z = g; z < nz; z += SIDE) y += o[z * (DH / 4)] * (sw[z] * inv);
+    sy[g][d] = y;
+  }
+  __syncthreads();
+  if (threadIdx.x < DH) {
+    float y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SIDE; ++i) y += ((const float *)sy[i])[threadIdx.x];
+    if (__builtin_isinf(y)) {
+      bool finite = true;
+      for (int z = 0; z < nz; ++z) finite &= (bool)__builtin_isfinite(a.part[(run0 + z) * DH + threadIdx.x]);
+      if (finite) y = pa_largest(y);
+    }
+    a.out[row * a.ldo + (int64_t)hq * DH + threadIdx.x] = y;
+  }
+}
+
+#endif  // __HIPCC__
+
+}  // namespace rw
