@@ -10,10 +10,12 @@
 // follows; 8-bit pools differ:
 //   keys    as f16, which has all their values, times q in 2 f16 parts (22 bits and
 //           more of every value down to 2^-29 of its query's largest); the score times the key's scale
-//   values  as bf16, which has them too, times p s in 2 bf16 parts (p's weight, s the value's
-//           scale): the second part is rounded, so a weight is off by 2^-17 of itself at most and
-//           on neither side, where the values themselves are off by 2^-8 of their row's largest.
-//           (A third part would cost half a product more and change nothing that the pool can show.)
+//   values  as bf16, which has them too, times p s (p: the weight, s: the value's
+//           scale) in 3 bf16 parts, all of its bits.  (In 2, 5e-6 of the results was off; in 2 f16
+//           parts, of the largest p s at 2^10 .. 2^15, as little as in 3, but a small weight
+//           lost bits where the value of a large one is zero, and int8 has many zeros.)
+// f16 pools: q in those 2 parts, not 3; of p's 3 parts against v's 2 the product of the
+// least two, 2^-24 of the whole, is left out.
 #pragma once
 #include "rw_kv8.hpp"
 
@@ -44,8 +46,8 @@ struct Kv8<I8> {
     u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int w = (int)a[i >> 1], s = 16 * (i & 1);
-      const float x0 = (float)(int8_t)(w >> s), x1 = (float)(int8_t)(w >> (s + 8));
+      const uint32_t u = a[i >> 1] ^ 0x80808080u;  // x + 128: bytes without a sign have their own conversions
+      const float x0 = (float)(i & 1 ? u >> 16 & 0xFF : u & 0xFF) - 128.0f, x1 = (float)(i & 1 ? u >> 24 : u >> 8 & 0xFF) - 128.0f;
       o[i] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
     }
     return __builtin_bit_cast(PaTile<BF16>::Op, o);
@@ -72,6 +74,15 @@ struct Kv8<E4M3> {
   }
   static constexpr bool FINITE = false;
 };
+
+// the first c bytes of a word (none, some or all)
+__device__ inline uint32_t kv8_first(int c) { return c <= 0 ? 0 : c >= 4 ? ~0u : (1u << (8 * c)) - 1; }
+// which bytes of a word are e4m3's NaN, which become zeros
+__device__ inline uint32_t kv8_take_nan(uint32_t &w) {
+  const uint32_t x = ((w & 0x7F7F7F7Fu) + 0x01010101u) >> 7 & 0x01010101u;
+  w &= ~(x * 0xFFu);
+  return (x | x >> 7 | x >> 14 | x >> 21) & 0xFu;
+}
 
 struct TreeArgs {
   const void *k, *v;
@@ -135,6 +146,37 @@ __device__ inline uint32_t tree_sees(const TreeArgs &a, const TreeSpan &s, const
   return bits & (c <= 0 ? 0 : c >= PER ? ALL : (1u << c) - 1);
 }
 
+// c + how many of a lane's 8 keys both bits are set of
+__device__ inline f4 tree_count(uint32_t w, uint32_t v, f4 c) {
+  PaTile<BF16>::Op a, b;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a[j] = (__bf16)(w >> j & 1 ? 1.0f : 0.0f);
+    b[j] = (__bf16)(v >> j & 1 ? 1.0f : 0.0f);
+  }
+  return PaTile<BF16>::mma(a, b, c);
+}
+// x as two f16, the second at 2^11 of its own size
+__device__ inline void tree_q_halves(const float (&x)[8], PaTile<F16>::Op &hi, PaTile<F16>::Op &lo) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) hi[j] = (_Float16)x[j], lo[j] = (_Float16)((x[j] - (float)hi[j]) * 0x1p11f);
+}
+// weights as 3 bf16
+__device__ inline void tree_parts(const float *p, PaTile<BF16>::Op (&pf)[3]) {
+  float x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = p[j];
+  pa_parts<BF16>(x, pf);
+}
+// o += p v, p in 3 bf16 parts, v as 2
+__device__ inline f4 tree_split_mma(const PaTile<BF16>::Op (&p)[3], PaTile<BF16>::Op hi, PaTile<BF16>::Op lo, f4 o) {
+  o = PaTile<BF16>::mma(p[2], hi, o);
+  o = PaTile<BF16>::mma(p[1], lo, o);
+  o = PaTile<BF16>::mma(p[1], hi, o);
+  o = PaTile<BF16>::mma(p[0], lo, o);
+  return PaTile<BF16>::mma(p[0], hi, o);
+}
+
 // How a pool's tiles of keys enter the two products.  Lane 16 h + r of a
 // wavefront holds of a tile's KEYS keys the scores of PER h .. PER h + PER - 1 for
 // query r, and their values 16 i + r.
@@ -143,11 +185,13 @@ struct TreeTile {
   using M = PaTile<E>;
   using T = typename E::T;
   using QOp = typename M::Op;   // of the scores' product
-  using VM = PaTile<std::conditional_t<sizeof(T) == 2, BF16, E>>;  // of the second one's weights
   static constexpr bool SCALED = false, WIDE = M::WIDE;
-  static constexpr int KEYS = M::KEYS, SUB = M::SUB, PER = 4 * SUB, PARTS = M::PARTS, SUMS = M::SUMS, STEPS = DH / M::STEP;
+  static constexpr int KEYS = M::KEYS, SUB = M::SUB, PER = 4 * SUB, STEPS = DH / M::STEP;
+  static constexpr bool HALF = std::is_same_v<E, F16>;
+  static constexpr int PARTS = HALF ? 2 : M::PARTS, SUMS = HALF ? 2 : M::SUMS;
   static constexpr int VAL = M::PER;  // values per lane and step
   static constexpr float MOVE = M::MOVE;
+  static constexpr int HEAD = DH;
   typename M::Op kr[SUB][STEPS], vr[DH / 16];
   // the first value of step c for the lanes of `h`
   static __device__ int value(int c, int h) { return M::STEP * c + VAL * h; }
@@ -163,28 +207,47 @@ struct TreeTile {
   }
   __device__ QOp k(int s, int c) const { return kr[s][c]; }
   static __device__ f4 mma(QOp a, QOp b, f4 c) { return M::mma(a, b, c); }
-  static __device__ void q_parts(const float (&x)[VAL], QOp (&o)[PARTS]) { pa_parts<E>(x, o); }
-  // keys without a row behind them: nothing of what memory holds there
-  __device__ void clear_v(int i, int j) { vr[i][j] = (T)0.0f; }
+  static __device__ void q_parts(const float (&x)[VAL], QOp (&o)[PARTS]) {
+    if constexpr (HALF) tree_q_halves(x, o[0], o[1]);
+    else pa_parts<E>(x, o);
+  }
+  // the keys from the c-th on have no row behind them: nothing of what memory holds there
+  __device__ void keep_v(int c) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (j >= c)
+#pragma unroll
+        for (int i = 0; i < DH / 16; ++i) vr[i][j] = (T)0.0f;
+  }
   // the bits of values 16 i + r that are infinities or NaN, which are then cleared
   __device__ uint32_t take_odd(int i) {
     uint32_t odd = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (!__builtin_isfinite((float)vr[i][j])) odd |= 1u << j, clear_v(i, j);
+      if (!__builtin_isfinite((float)vr[i][j])) odd |= 1u << j, vr[i][j] = (T)0.0f;
     return odd;
   }
   // how many keys both bits are set of
   static __device__ f4 count(uint32_t w, uint32_t v) {
-    typename VM::Op a, b;
+    if constexpr (sizeof(T) == 2) {
+      return tree_count(w, v, f4{0.0f, 0.0f, 0.0f, 0.0f});
+    } else {
+      typename M::Op a, b;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      a[j] = (typename VM::T)(w >> j & 1 ? 1.0f : 0.0f);
-      b[j] = (typename VM::T)(v >> j & 1 ? 1.0f : 0.0f);
+      for (int j = 0; j < PER; ++j) a[j] = w >> j & 1 ? 1.0f : 0.0f, b[j] = v >> j & 1 ? 1.0f : 0.0f;
+      return M::mma(a, b, f4{0.0f, 0.0f, 0.0f, 0.0f});
     }
-    return VM::mma(a, b, f4{0.0f, 0.0f, 0.0f, 0.0f});
   }
-  __device__ void add(const float (&p)[PER], f4 (&o)[DH / 16]) const { pa_add<E>(p, vr, o); }
+  __device__ void add(const float (&p)[PER], f4 (&o)[DH / 16]) const {
+    if constexpr (HALF) {
+      PaTile<BF16>::Op pf[3], hi, lo;
+      pa_parts<BF16>(p, pf);
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i) pa_split(vr[i], hi, lo), o[i] = tree_split_mma(pf, hi, lo, o[i]);
+    } else {
+      pa_add<E>(p, vr, o);
+    }
+  }
 };
 
 template <class E, int DH>
@@ -192,10 +255,10 @@ struct TreeTile8 {
   using M = PaTile<F16>;
   using T = typename E::T;
   using QOp = M::Op;
-  using VM = PaTile<BF16>;
   static constexpr bool SCALED = true, WIDE = true;
   static constexpr int KEYS = 64, SUB = 4, PER = 16, PARTS = 2, SUMS = 2, STEPS = DH / 32, VAL = 8;
   static constexpr float MOVE = 0x1p11f;
+  static constexpr int HEAD = DH;
   u32x4 kr[SUB][(DH + 63) / 64], vr[DH / 16];
   // 16 bytes per lane are the values of two steps, 8 those of a last odd one
   static __device__ int value(int c, int h) {
@@ -221,49 +284,40 @@ struct TreeTile8 {
   }
   static __device__ f4 mma(QOp a, QOp b, f4 c) { return M::mma(a, b, c); }
   static __device__ void q_parts(const float (&x)[VAL], QOp (&o)[PARTS]) {
+    tree_q_halves(x, o[0], o[1]);
+  }
+  __device__ void keep_v(int c) {
 #pragma unroll
-    for (int j = 0; j < VAL; ++j) {
-      o[0][j] = (_Float16)x[j];
-      o[1][j] = (_Float16)((x[j] - (float)o[0][j]) * MOVE);
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t mask = kv8_first(c - 4 * k);
+#pragma unroll
+      for (int i = 0; i < DH / 16; ++i) vr[i][k] &= mask;
     }
   }
-  __device__ void clear_v(int i, int j) { vr[i][j >> 2] &= ~(0xFFu << (8 * (j & 3))); }
   __device__ uint32_t take_odd(int i) {
     uint32_t odd = 0;
     if (!Kv8<E>::FINITE)
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (((vr[i][j >> 2] >> (8 * (j & 3))) & 0x7F) == 0x7F) odd |= 1u << j, clear_v(i, j);
+      for (int k = 0; k < 4; ++k) {
+        uint32_t w = vr[i][k];
+        odd |= kv8_take_nan(w) << (4 * k);
+        vr[i][k] = w;
+      }
     return odd;
   }
   static __device__ f4 count(uint32_t w, uint32_t v) {
-    f4 c{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int u = 0; u < PER; u += 8) {
-      VM::Op a, b;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        a[j] = (__bf16)(w >> (u + j) & 1 ? 1.0f : 0.0f);
-        b[j] = (__bf16)(v >> (u + j) & 1 ? 1.0f : 0.0f);
-      }
-      c = VM::mma(a, b, c);
-    }
-    return c;
+    return tree_count(w >> 8, v >> 8, tree_count(w, v, f4{0.0f, 0.0f, 0.0f, 0.0f}));
   }
   __device__ void add(const float (&p)[PER], f4 (&o)[DH / 16]) const {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      VM::Op hi, lo;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        hi[j] = VM::part(p[8 * u + j]);
-        lo[j] = (__bf16)(p[8 * u + j] - (float)hi[j]);
-      }
+      PaTile<BF16>::Op pf[3];
+      tree_parts(p + 8 * u, pf);
 #pragma unroll
       for (int i = 0; i < DH / 16; ++i) {
-        const VM::Op b = Kv8<E>::bf16(u ? u32x2{vr[i][2], vr[i][3]} : u32x2{vr[i][0], vr[i][1]});
-        o[i] = VM::mma(lo, b, o[i]);
-        o[i] = VM::mma(hi, b, o[i]);
+        const PaTile<BF16>::Op b = Kv8<E>::bf16(u ? u32x2{vr[i][2], vr[i][3]} : u32x2{vr[i][0], vr[i][1]});
+#pragma unroll
+        for (int k = 2; k >= 0; --k) o[i] = PaTile<BF16>::mma(pf[k], b, o[i]);
       }
     }
   }
@@ -273,6 +327,92 @@ struct TreeTile<I8, DH> : TreeTile8<I8, DH> {};
 template <int DH>
 struct TreeTile<E4M3, DH> : TreeTile8<E4M3, DH> {};
 
+// A query's running softmax (lane 16 h + r: query r) and its tile's output (lane
+// 16 h + r: queries 4 h .., values 16 i + r).
+template <bool SCALED, bool WIDE, int ND>
+struct TreeSum {
+  f4 o[ND];
+  float m, sum;  // largest score, this lane's sum of weights
+  __device__ void clear() {
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i] = {};
+    m = -__builtin_huge_valf(), sum = 0.0f;
+  }
+  // scores (log2; -inf: not seen) become the weights that enter the product with v
+  template <int PER>
+  __device__ __forceinline__ void weigh(float (&y)[PER], const f4 *vsc, uint32_t sees, int h, float scale) {
+    float top = y[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) top = fmaxf(top, y[j]);
+    if (__builtin_amdgcn_ballot_w64(top > m + PA_SLACK)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float next = fmaxf(m, top), f = pa_weight(m, next);
+      m = next;
+      sum *= f;
+      f4 fr;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[i] *= fr;
+    }
+    const float base = m == -__builtin_huge_valf() ? 0.0f : m;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      y[j] = __builtin_amdgcn_exp2f(y[j] - base);
+      if (WIDE) y[j] *= scale;
+      sum += y[j];
+      if constexpr (SCALED) y[j] = sees >> j & 1 ? y[j] * vsc[j >> 2][j & 3] : 0.0f;
+    }
+  }
+  // values that are infinities or NaN and that not every query sees: NaN for those that do
+  __device__ void spoil(int i, f4 seen) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (seen[e] > 0.0f) o[i][e] = __builtin_nanf("");
+  }
+  // what makes of a query's o its mean (0: it saw nothing); sum is then the query's
+  __device__ float mean() {
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    return sum == 0.0f ? 0.0f : 1.0f / sum;
+  }
+};
+
+// Query r's values in the scores' operand order; f16 parts: scaled by a power of two
+// so that the largest lies in [2^14, 2^15), undone in the factor that is returned
+template <class M, class T>
+__device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf) {
+  float c = PA_LOG2E / __builtin_sqrtf((float)M::HEAD);
+  float y[M::STEPS][M::VAL], top = 0.0f;
+#pragma unroll
+  for (int s = 0; s < M::STEPS; ++s)
+#pragma unroll
+    for (int j = 0; j < M::VAL; j += 4) {
+      const f4 z = *(const f4 *)(p + M::value(s, h) + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[s][j + e] = real ? z[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(y[s][j + e]));
+    }
+  int e = 0;
+  if (M::MOVE != 1.0f) {
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+    c = ldexpf(c, e);
+  }
+#pragma unroll
+  for (int s = 0; s < M::STEPS; ++s) {
+    typename M::QOp o[M::PARTS];
+    if (M::MOVE != 1.0f)
+#pragma unroll
+      for (int j = 0; j < M::VAL; ++j) y[s][j] = ldexpf(y[s][j], -e);
+    M::q_parts(y[s], o);
+#pragma unroll
+    for (int k = 0; k < M::PARTS; ++k) qf[k][s] = o[k];
+  }
+  return c;
+}
+
 // One workgroup of PA_WAVES wavefronts per (tree, key/value head, QT tiles of 16
 // queries, chunk of keys).  A wavefront takes every PA_WAVES-th tile of keys, straight from memory, for
 // all of the workgroup's queries.
@@ -280,7 +420,7 @@ template <class E, int DH, int QT>
 __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(TreeArgs a) {
   using M = TreeTile<E, DH>;
   using QOp = typename M::QOp;
-  constexpr int ND = DH / 16, KEYS = M::KEYS, PER = M::PER, SUB = M::SUB, PARTS = M::PARTS, VAL = M::VAL;
+  constexpr int ND = DH / 16, KEYS = M::KEYS, PER = M::PER, SUB = M::SUB, PARTS = M::PARTS;
   constexpr int LD = DH + 4, NQ = 16 * QT;
   constexpr float NEG_INF = -__builtin_huge_valf();
   __shared__ float so[PA_WAVES][NQ][LD], sm[PA_WAVES][NQ], sl[PA_WAVES][NQ];
@@ -343,8 +483,6 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
   Where now{};
   if (t < end) now = where(t), load_k(t, now);
 
-  // q, in the scores' operand order; f16 parts: each query's values scaled by a
-  // power of two so that the largest lies in [2^14, 2^15), undone in `c`
   QOp qf[QT][PARTS][M::STEPS];
   float c[QT];
   const uint32_t *mask[QT];
@@ -352,48 +490,15 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
 #pragma unroll
   for (int x = 0; x < QT; ++x) {
     const int i = min(16 * x + r, nq - 1);
-    const bool real = 16 * x + r < nq;
     node[x] = (u0 + i) / a.group;
     mask[x] = a.mask ? a.mask + (int64_t)row_of(i) * a.n_words : nullptr;
-    c[x] = PA_LOG2E / __builtin_sqrtf((float)DH);
-    float y[M::STEPS][VAL], top = 0.0f;
-    const float *p = a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH;
-#pragma unroll
-    for (int s = 0; s < M::STEPS; ++s)
-#pragma unroll
-      for (int j = 0; j < VAL; j += 4) {
-        const f4 z = *(const f4 *)(p + M::value(s, h) + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[s][j + e] = real ? z[e] : 0.0f, top = fmaxf(top, __builtin_fabsf(y[s][j + e]));
-      }
-    int e = 0;
-    if (M::MOVE != 1.0f) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
-      c[x] = ldexpf(c[x], e);
-    }
-#pragma unroll
-    for (int s = 0; s < M::STEPS; ++s) {
-      QOp o[PARTS];
-      if (M::MOVE != 1.0f)
-#pragma unroll
-        for (int j = 0; j < VAL; ++j) y[s][j] = ldexpf(y[s][j], -e);
-      M::q_parts(y[s], o);
-#pragma unroll
-      for (int k = 0; k < PARTS; ++k) qf[x][k][s] = o[k];
-    }
+    c[x] = tree_q<M>(a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH, 16 * x + r < nq, h, qf[x]);
   }
 
   for (float scale = 1.0f;; scale = PA_LOW) {
-    f4 o[QT][ND];
-    float m[QT], sum[QT];  // of query r; sum: of this lane's keys
+    TreeSum<M::SCALED, M::WIDE, ND> acc[QT];
 #pragma unroll
-    for (int x = 0; x < QT; ++x) {
-#pragma unroll
-      for (int i = 0; i < ND; ++i) o[x][i] = {};
-      m[x] = NEG_INF, sum[x] = 0.0f;
-    }
+    for (int x = 0; x < QT; ++x) acc[x].clear();
 
     for (; t < end; t += PA_WAVES) {
       load_v(t, now);
@@ -426,12 +531,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
       bool odd_any = false;
       uint32_t odd[(ND + 1) / 2] = {};  // 16 bits for each i
       if (edge) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (now.bad || a0 + j >= n) {
-#pragma unroll
-            for (int i = 0; i < ND; ++i) tile.clear_v(i, j);
-          }
+        tile.keep_v(now.bad ? 0 : n - a0);
         // a row that one query sees and another does not may hold infinities or NaN:
         // they leave the products and are given to those who see them
 #pragma unroll
@@ -458,39 +558,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
           for (int j = 0; j < PER; ++j)
             if (!(sees >> j & 1)) y[j] = NEG_INF;
         }
-        float top = y[0];
+        acc[x].template weigh<PER>(y, vsc, sees, h, scale);
+        tile.add(y, acc[x].o);
+        if (odd_any)
 #pragma unroll
-        for (int j = 1; j < PER; ++j) top = fmaxf(top, y[j]);
-        if (__builtin_amdgcn_ballot_w64(top > m[x] + PA_SLACK)) {
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float up = fmaxf(m[x], top), f = pa_weight(m[x], up);
-          m[x] = up;
-          sum[x] *= f;
-          f4 fr;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) fr[i] = __shfl(f, 4 * h + i);
-#pragma unroll
-          for (int i = 0; i < ND; ++i) o[x][i] *= fr;
-        }
-        const float base = m[x] == NEG_INF ? 0.0f : m[x];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          y[j] = __builtin_amdgcn_exp2f(y[j] - base);
-          if (M::WIDE) y[j] *= scale;
-          sum[x] += y[j];
-          if constexpr (M::SCALED) y[j] = edge && !(sees >> j & 1) ? 0.0f : y[j] * vsc[j >> 2][j & 3];
-        }
-        tile.add(y, o[x]);
-        if (odd_any) {
-#pragma unroll
-          for (int i = 0; i < ND; ++i) {
-            const f4 z = M::count(sees, odd[i / 2] >> (16 * (i & 1)));
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (z[e] > 0.0f) o[x][i][e] = __builtin_nanf("");
-          }
-        }
+          for (int i = 0; i < ND; ++i) acc[x].spoil(i, M::count(sees, odd[i / 2] >> (16 * (i & 1))));
       }
       now = next;
     }
@@ -500,20 +572,18 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
     bool over = false;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      sum[x] += __shfl_xor(sum[x], 16);
-      sum[x] += __shfl_xor(sum[x], 32);
-      if (first && h == 0) sm[wv][16 * x + r] = m[x], sl[wv][16 * x + r] = sum[x];
-      const float inv = sum[x] == 0.0f ? 0.0f : 1.0f / sum[x];  // 0: no keys
+      const float inv = acc[x].mean();
+      if (first && h == 0) sm[wv][16 * x + r] = acc[x].m, sl[wv][16 * x + r] = acc[x].sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int qr = 16 * x + 4 * h + i;
         const float f = __shfl(inv, 4 * h + i);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-          const float y = o[x][d][i] * f;
+          const float y = acc[x].o[d][i] * f;
           float &mean = so[wv][qr][16 * d + r];
           if (!M::WIDE || first) mean = y;
-          else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(o[x][d][i]) ? pa_largest(y) : y;
+          else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(acc[x].o[d][i]) ? pa_largest(y) : y;
           over |= qr < nq && !__builtin_isfinite(y);
         }
       }

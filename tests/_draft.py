@@ -3,7 +3,6 @@ definitions in 64 bits."""
 import numpy as np
 import torch
 
-from _paged import U, attend, i32
 
 POOLS = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i8": torch.int8, "e4m3": torch.float8_e4m3fn}
 TOP = {"i8": 127.0, "e4m3": 448.0}
@@ -49,16 +48,6 @@ def gather_any(pool, layer, pages, n):
     h, d = K.shape[1], K.shape[3]
     return (K.permute(1, 0, 2, 3).reshape(h, -1, d)[:, :n].cpu().numpy(),
             V.permute(1, 0, 3, 2).reshape(h, -1, d)[:, :n].cpu().numpy())
-
-
-def attend_any(q, K, V, kind):
-    """attend() of tests/_paged.py; 8-bit pools give each weight 16 bits, so 2^-17 of
-    sum p |v| more may be lost."""
-    out, tol = attend(q, K, V)
-    if kind in TOP and K.shape[1]:
-        extra, _ = attend(q, K, np.abs(V))
-        tol = tol + 2.0 ** -17 * extra
-    return out, tol
 
 
 def quantized(x, kind):

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from _draft import POOLS, TOP, accept, ancestors, any_pool, attend_any, bytes_of, quantized, sample, trees, words
-from _paged import i32, tables
+from _draft import POOLS, TOP, accept, ancestors, any_pool, bytes_of, quantized, sample, trees, words
+from _paged import attend, i32, tables
 from rusty_whisper_amd import _abi as A
 
 pytestmark = pytest.mark.gpu
@@ -165,8 +165,7 @@ class Program:
                     seen = np.arange(len(new[0])) <= past[i] + j
                     if masks is not None:
                         seen[past[i] :] = masks[i][j]
-                    want, tol = attend_any(q[a + j].double().cpu().numpy().reshape(-1, DIM), *(x[seen].transpose(1, 0, 2) for x in new),
-                                           self.kind)
+                    want, tol = attend(q[a + j].double().cpu().numpy().reshape(-1, DIM), *(x[seen].transpose(1, 0, 2) for x in new))
                     got = out[a + j].double().cpu().numpy().reshape(-1, DIM)
                     assert np.all(np.abs(got - want) <= tol), (layer, i, j)
         return starts, past, table

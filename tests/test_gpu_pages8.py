@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from _draft import POOLS, TOP, any_pool, attend_any, bytes_of, gather_any, quantized
-from _paged import U, i32, tables
+from _draft import POOLS, TOP, any_pool, bytes_of, gather_any, quantized
+from _paged import attend, i32, tables
 from rusty_whisper_amd import _abi as A
 
 pytestmark = pytest.mark.gpu
@@ -199,7 +199,7 @@ def check_attention(pool, kind, layer, q, n_head, table, lens, seq, got):
         row = table[seq[r]]
         n = max(0, min(int(n), len(row) * page))
         K, V = gather_any(pool, layer, row[: -(-n // page)], n)
-        want, tol = attend_any(q[r].double().cpu().numpy().reshape(n_head, -1), K, V, kind)
+        want, tol = attend(q[r].double().cpu().numpy().reshape(n_head, -1), K, V)
         err = np.abs(got[r].reshape(n_head, -1) - want)
         assert np.all(err <= tol), (r, n, float(err.max()), float(tol[err > tol].min()))
 

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from _draft import POOLS, TOP, ancestors, any_pool, attend_any, bytes_of, gather_any, trees, words
-from _paged import i32, tables
+from _draft import POOLS, TOP, ancestors, any_pool, bytes_of, gather_any, trees, words
+from _paged import attend, i32, tables
 from rusty_whisper_amd import _abi as A
 
 pytestmark = pytest.mark.gpu
@@ -72,7 +72,7 @@ class Call:
                 else:
                     seen[past:] |= self.masks[i][j]
                 q = self.q[r].double().cpu().numpy().reshape(G, -1)
-                want, tol = attend_any(q, K[:, seen], V[:, seen], self.kind)
+                want, tol = attend(q, K[:, seen], V[:, seen])
                 err = np.abs(got[r].reshape(G, -1) - want)
                 assert np.all(err <= tol), (i, j, past, n, float(err.max()))
                 done[r] = True
