@@ -338,16 +338,18 @@ struct TreeSum {
     for (int i = 0; i < ND; ++i) o[i] = {};
     m = -__builtin_huge_valf(), sum = 0.0f;
   }
-  // scores (log2; -inf: not seen) become the weights that enter the product with v
+  // scores (c of them: log2; -inf: not seen) become the weights that enter the product with v
   template <int PER>
-  __device__ __forceinline__ void weigh(float (&y)[PER], const f4 *vsc, uint32_t sees, int h, float scale) {
+  __device__ __forceinline__ void weigh(float (&y)[PER], float c, const f4 *vsc, uint32_t sees, int h, float scale) {
     float top = y[0];
 #pragma unroll
     for (int j = 1; j < PER; ++j) top = fmaxf(top, y[j]);
+    top *= c;
     if (__builtin_amdgcn_ballot_w64(top > m + PA_SLACK)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float next = fmaxf(m, top), f = pa_weight(m, next);
+      // (each query's own: what others see changes no bit of it)
+      const float next = top > m + PA_SLACK ? top : m, f = pa_weight(m, next);
       m = next;
       sum *= f;
       f4 fr;
@@ -359,8 +361,8 @@ struct TreeSum {
     const float base = m == -__builtin_huge_valf() ? 0.0f : m;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      y[j] = __builtin_amdgcn_exp2f(y[j] - base);
-      if (WIDE) y[j] *= scale;
+      y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], c, -base));
+      if (WIDE && scale != 1.0f) y[j] *= scale;
       sum += y[j];
       if constexpr (SCALED) y[j] = sees >> j & 1 ? y[j] * vsc[j >> 2][j & 3] : 0.0f;
     }
@@ -480,8 +482,12 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
 
   const int t0 = k0 / KEYS + wv;
   int t = t0;
-  Where now{};
-  if (t < end) now = where(t), load_k(t, now);
+  Where now{}, next{};
+  auto begin = [&]() __attribute__((always_inline)) {
+    if (t < end) now = where(t), load_k(t, now);
+    if (t + PA_WAVES < end) next = where(t + PA_WAVES);
+  };
+  begin();
 
   QOp qf[QT][PARTS][M::STEPS];
   float c[QT];
@@ -503,8 +509,6 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
     for (; t < end; t += PA_WAVES) {
       load_v(t, now);
       const bool more = t + PA_WAVES < end;
-      Where next{};
-      if (more) next = where(t + PA_WAVES);
       f4 s[QT][M::SUMS][SUB];
 #pragma unroll
       for (int x = 0; x < QT; ++x)
@@ -523,6 +527,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
             for (int k = 0; k < PARTS; ++k) s[x][k % M::SUMS][u] = M::mma(kk, qf[x][k][i], s[x][k % M::SUMS][u]);
         }
       if (more) load_k(t + PA_WAVES, next);
+      // (the pages of the tile after that: they are there when its keys are asked for)
+      Where after{};
+      if (t + 2 * PA_WAVES < end) after = where(t + 2 * PA_WAVES);
 
       // keys that no query of the call may see, or that are in no page of the pool: no
       // weight, and what v holds there (anything) is taken as zero
@@ -548,7 +555,6 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
           y[j] = s[x][M::SUMS - 1][j >> 2][j & 3];
 #pragma unroll
           for (int k = M::SUMS - 2; k >= 0; --k) y[j] = fmaf(y[j], 1.0f / M::MOVE, s[x][k][j >> 2][j & 3]);
-          y[j] *= c[x];
           if constexpr (M::SCALED) y[j] *= ksc[j >> 2][j & 3];
         }
         uint32_t sees = ~0u;
@@ -558,13 +564,13 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
           for (int j = 0; j < PER; ++j)
             if (!(sees >> j & 1)) y[j] = NEG_INF;
         }
-        acc[x].template weigh<PER>(y, vsc, sees, h, scale);
+        acc[x].template weigh<PER>(y, c[x], vsc, sees, h, scale);
         tile.add(y, acc[x].o);
         if (odd_any)
 #pragma unroll
           for (int i = 0; i < ND; ++i) acc[x].spoil(i, M::count(sees, odd[i / 2] >> (16 * (i & 1))));
       }
-      now = next;
+      now = next, next = after;
     }
 
     // the wavefront's means
@@ -590,7 +596,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
     }
     if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
     t = t0;
-    if (t < end) now = where(t), load_k(t, now);
+    begin();
   }
   __syncthreads();
 
@@ -619,6 +625,357 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
       a.part[run * DH + d] = y;
       if (d == 0) a.part[runs * DH + 2 * run] = top, a.part[runs * DH + 2 * run + 1] = l;
     }
+  }
+}
+
+// ------------------------------------------------- many queries of a tree
+//
+// The same with keys and values through LDS: the workgroup's wavefronts share a
+// tile of them, each for 16 QW queries of its own, so that memory and L2 give a
+// tile once for 64 QW queries and not once for 16.  What a wavefront reads
+// of LDS are the operands themselves, 16 bytes a lane: K's rows lie in the order of
+// the score product's rows, 8-bit values are converted and f16's v split where they are written,
+// and the 16-byte units of a row are exchanged so that 16 lanes' reads fall into all banks.
+
+// units (16 bytes, 8 values) of a tile row of UNITS: where unit `col` of row `row` lies
+template <int UNITS>
+__device__ inline int tree_unit(int row, int col) {
+  if constexpr (UNITS == 12) {
+    const int c = col + (row >> 2 & 3);
+    return row * 12 + (c >= 12 ? c - 12 : c);
+  } else {
+    return row * UNITS + (col ^ (row / (16 / UNITS) & (UNITS - 1)));
+  }
+}
+
+template <class E, int DH>
+struct TreeShared {
+  using T = typename E::T;
+  static constexpr bool SCALED = sizeof(T) == 1, HALF = std::is_same_v<E, F16>, WIDE = !HALF;
+  using KE = std::conditional_t<std::is_same_v<E, BF16>, BF16, F16>;
+  using M = PaTile<KE>;      // of the scores' product
+  using W = PaTile<BF16>;    // of the second one
+  using QOp = typename M::Op;
+  static constexpr int PARTS = std::is_same_v<E, BF16> ? 3 : 2, SUMS = std::is_same_v<E, BF16> ? 1 : 2;
+  static constexpr float MOVE = SUMS == 2 ? 0x1p11f : 1.0f;
+  static constexpr int HEAD = DH, STEPS = DH / 32, VAL = 8;
+  static constexpr int KEYS = SCALED || DH <= 64 ? 64 : 32;  // of a tile
+  static constexpr int PLANES = HALF ? 2 : 1;                 // of v
+  static constexpr int KU = DH / 8, VU = KEYS / 8;            // units of a row of K, of V
+  static constexpr int RAW = 16 / sizeof(T);                  // values of 16 bytes of the pool
+  static constexpr int LOADS = KEYS * DH / RAW;               // of 16 bytes, of K and of V each
+  static constexpr int PER = (LOADS + 255) / 256;             // per thread
+  static __device__ int value(int c, int h) { return 32 * c + 8 * h; }
+  static __device__ void q_parts(const float (&x)[8], QOp (&o)[PARTS]) {
+    if constexpr (SUMS == 2) tree_q_halves(x, o[0], o[1]);
+    else pa_parts<BF16>(x, o);
+  }
+  struct Lds {  // a tile
+    u32x4 k[KEYS * KU], v[PLANES][DH * VU];
+    float ks[SCALED ? KEYS : 4], vs[SCALED ? KEYS : 4];
+    unsigned long long odd[DH];  // keys whose value is an infinity or a NaN
+  };
+  // the row of K's tile that key `key` has: 16 s + 4 h + i for key 32 (s / 2) + 8 h + 4 (s % 2) + i
+  static __device__ int k_row(int key) { return (key & 32) + (key >> 2 & 1) * 16 + (key >> 3 & 3) * 4 + (key & 3); }
+};
+
+template <class E, int DH, int QW, bool BIG>
+__global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
+  using S = TreeShared<E, DH>;
+  using T = typename E::T;
+  constexpr int ND = DH / 16, KEYS = S::KEYS, PER = S::PER, PARTS = S::PARTS, SUMS = S::SUMS, RAW = S::RAW, NQ = 64 * QW;
+  constexpr float NEG_INF = -__builtin_huge_valf();
+  // One tile is computed with while the next is written; what is special about a tile (1: odd
+  // values, 2: pages outside the pool) is cleared two tiles ahead
+  __shared__ typename S::Lds lds[2];
+  __shared__ int flags[3];
+
+  const int qi = blockIdx.x / 8 % a.qtiles, item = blockIdx.x / (8 * a.qtiles) * 8 + blockIdx.x % 8;
+  const int hk = item % a.kv_heads, tree = item / a.kv_heads;
+  if (tree >= a.n_trees) return;
+  const TreeSpan sp = tree_span(a, tree);
+  const int u0 = qi * NQ, all = sp.rows * a.group, nq = min(NQ, all - u0);
+  if (nq <= 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int heads = a.kv_heads * a.group;
+  const int n = tree_end(a, sp, u0 + nq);
+  auto row_of = [&](int i) { return sp.start + (u0 + i) / a.group; };
+  auto head_of = [&](int i) { return hk * a.group + (u0 + i) % a.group; };
+  if (n <= 0) {
+    if (blockIdx.y == 0)
+      for (int i = tid; i < nq * DH; i += 256) a.out[row_of(i / DH) * a.ldo + (int64_t)head_of(i / DH) * DH + i % DH] = 0.0f;
+    return;
+  }
+  const int k0 = blockIdx.y * a.chunk;
+  if (k0 >= n) return;
+  const bool direct = n <= a.chunk;
+  const int t0 = k0 / KEYS, end = (min(n, k0 + a.chunk) + KEYS - 1) / KEYS, P = 1 << a.pr;
+  // this wavefront's queries, and the end of what they see
+  const int w0 = 16 * QW * wv, wq = min(16 * QW, nq - w0), wn = wq <= 0 ? 0 : tree_end(a, sp, u0 + w0 + wq);
+
+  typename S::QOp qf[QW][PARTS][S::STEPS];
+  float c[QW];
+  const uint32_t *mask[QW];
+  int node[QW];
+#pragma unroll
+  for (int x = 0; x < QW; ++x) {
+    const int i = min(w0 + 16 * x + r, nq - 1);
+    node[x] = (u0 + i) / a.group;
+    mask[x] = a.mask ? a.mask + (int64_t)row_of(i) * a.n_words : nullptr;
+    c[x] = tree_q<S>(a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH, w0 + 16 * x + r < nq, h, qf[x]);
+  }
+
+  // What this thread brings of a tile: 16 bytes of K's rows and of V's.  Pages no shorter
+  // than a tile (BIG): its one page is the same for all threads, which add what is their
+  // own for every tile; else each thread looks its pages up.
+  u32x4 kr[PER], vr[PER];
+  float kscale = 0.0f, vscale = 0.0f;
+  int kp[BIG ? 1 : PER], vp[BIG ? 1 : PER], scale_page = 0;
+  uint32_t vbad = 0;  // which of vr are of no page of the pool
+  constexpr int KL = DH / RAW, VL = KEYS / RAW;  // loads of a row of K, of V
+  auto key_of = [&](int i) { return (i * 256 + tid) / KL; };
+  auto group_of = [&](int i) { return (i * 256 + tid) % VL * RAW; };  // first key
+  auto page_of = [&](int key) { return sp.table[min(key, n - 1) >> a.pr]; };
+  auto in_pool = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
+  auto first = [&](int page) { return ((int64_t)(in_pool(page) ? page : 0) * a.kv_heads + hk) << a.pr; };
+  auto pages = [&](int t) __attribute__((always_inline)) {
+    if constexpr (BIG) {
+      // (a scalar load: a vector load's result would be waited for together with the tile's own, which are behind it)
+      typedef const __attribute__((address_space(4))) int32_t *Scalar;
+      kp[0] = ((Scalar)(uintptr_t)sp.table)[__builtin_amdgcn_readfirstlane(min(t * KEYS, n - 1) >> a.pr)];
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) kp[i] = page_of(t * KEYS + min(key_of(i), KEYS - 1)), vp[i] = page_of(t * KEYS + group_of(i));
+      if (S::SCALED && tid < KEYS) scale_page = page_of(t * KEYS + tid);
+    }
+  };
+  auto load = [&](int t) __attribute__((always_inline)) {
+    vbad = 0;
+    const int64_t one = BIG ? first(kp[0]) : 0;
+    const int at = t * KEYS & (P - 1);
+    const char *kb = (const char *)a.k + (one + at) * (DH * (int)sizeof(T)), *vb = (const char *)a.v + (one * DH + at) * (int)sizeof(T);
+    if (BIG && !in_pool(kp[0])) vbad = ~0u;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = i * 256 + tid;
+      if (S::LOADS % 256 && e >= S::LOADS) break;
+      if constexpr (BIG) {
+        kr[i] = *(const u32x4 *)(kb + (uint32_t)e * 16);
+        vr[i] = *(const u32x4 *)(vb + (((uint32_t)(e / VL) << a.pr) * (uint32_t)sizeof(T) + (uint32_t)(e % VL) * 16));
+      } else {
+        vbad |= in_pool(vp[i]) ? 0u : 1u << i;
+        kr[i] = *(const u32x4 *)((const T *)a.k + (first(kp[i]) + ((t * KEYS + key_of(i)) & (P - 1))) * DH + e % KL * RAW);
+        vr[i] = *(const u32x4 *)((const T *)a.v + first(vp[i]) * DH + ((int64_t)(e / VL) << a.pr) + ((t * KEYS + group_of(i)) & (P - 1)));
+      }
+    }
+    if (S::SCALED && tid < KEYS) {
+      const int64_t row = BIG ? one + at + tid : first(scale_page) + ((t * KEYS + tid) & (P - 1));
+      kscale = a.ks[row], vscale = a.vs[row];
+    }
+  };
+  // ... goes to LDS
+  auto store = [&](int t, bool edge) __attribute__((always_inline)) {
+    typename S::Lds &l = lds[t & 1];
+    auto put = [&](int i, u32x4 y) __attribute__((always_inline)) {
+      const int e = i * 256 + tid, krow = S::k_row(key_of(i)), kc = e % KL, value = e / VL, vc = e % VL;
+      if constexpr (S::SCALED) {
+        const u32x4 x = kr[i];
+        l.k[tree_unit<S::KU>(krow, 2 * kc)] = __builtin_bit_cast(u32x4, Kv8<E>::f16(u32x2{x[0], x[1]}));
+        l.k[tree_unit<S::KU>(krow, 2 * kc + 1)] = __builtin_bit_cast(u32x4, Kv8<E>::f16(u32x2{x[2], x[3]}));
+        l.v[0][tree_unit<S::VU>(value, 2 * vc)] = __builtin_bit_cast(u32x4, Kv8<E>::bf16(u32x2{y[0], y[1]}));
+        l.v[0][tree_unit<S::VU>(value, 2 * vc + 1)] = __builtin_bit_cast(u32x4, Kv8<E>::bf16(u32x2{y[2], y[3]}));
+      } else {
+        l.k[tree_unit<S::KU>(krow, kc)] = kr[i];
+        if constexpr (S::HALF) {
+          typename S::W::Op hi, lo;
+          pa_split(__builtin_bit_cast(PaTile<F16>::Op, y), hi, lo);
+          l.v[0][tree_unit<S::VU>(value, vc)] = __builtin_bit_cast(u32x4, hi);
+          l.v[1][tree_unit<S::VU>(value, vc)] = __builtin_bit_cast(u32x4, lo);
+        } else {
+          l.v[0][tree_unit<S::VU>(value, vc)] = y;
+        }
+      }
+    };
+    if (S::SCALED && tid < KEYS) l.ks[tid] = kscale, l.vs[tid] = vscale;
+    if (!edge && !__builtin_amdgcn_ballot_w64(vbad != 0)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (S::LOADS % 256 && i * 256 + tid >= S::LOADS) break;
+        put(i, vr[i]);
+      }
+      return;
+    }
+    int special = vbad ? 2 : 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = i * 256 + tid;
+      if (S::LOADS % 256 && e >= S::LOADS) break;
+      const int vc = e % VL, have = vbad >> i & 1 ? 0 : n - (t * KEYS + vc * RAW);  // keys with a row behind them
+      u32x4 y = vr[i];
+      uint32_t odd = 0;
+      if constexpr (S::SCALED) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t w = y[j] & kv8_first(have - 4 * j);
+          if (!Kv8<E>::FINITE) odd |= kv8_take_nan(w) << (4 * j);
+          y[j] = w;
+        }
+      } else {
+        typename PaTile<E>::Op z = __builtin_bit_cast(typename PaTile<E>::Op, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (j >= have) z[j] = (T)0.0f;
+          if (!__builtin_isfinite((float)z[j])) odd |= 1u << j, z[j] = (T)0.0f;
+        }
+        y = __builtin_bit_cast(u32x4, z);
+      }
+      put(i, y);
+      if (odd && edge) atomicOr(&l.odd[e / VL], (unsigned long long)odd << (vc * RAW)), special |= 1;
+    }
+    if (special) atomicOr(&flags[t % 3], special);
+  };
+
+  for (float scale = 1.0f;; scale = PA_LOW) {
+    TreeSum<S::SCALED, S::WIDE, ND> acc[QW];
+#pragma unroll
+    for (int x = 0; x < QW; ++x) acc[x].clear();
+    auto edge_of = [&](int t) { return (t + 1) * KEYS > min(n, sp.past); };
+    auto clear_odd = [&](int t) __attribute__((always_inline)) {
+      if (tid < DH) lds[t & 1].odd[tid] = 0;
+      __syncthreads();
+    };
+    pages(t0);
+    load(t0);
+    if (t0 + 1 < end) pages(t0 + 1);
+    __syncthreads();  // (a second time: the first is done)
+    if (tid < 3) flags[tid] = 0;
+    clear_odd(t0);
+    store(t0, edge_of(t0));
+
+    for (int t = t0; t < end; ++t) {
+      __syncthreads();  // tile t is there, and t - 1 is done with
+      const bool edge = edge_of(t), more = t + 1 < end;
+      if (more) {
+        load(t + 1);
+        if (t + 2 < end) pages(t + 2);
+      }
+      if (tid == 0) flags[(t + 2) % 3] = 0;
+      const typename S::Lds &l = lds[t & 1];
+      if (t * KEYS < wn) {
+        const int special = flags[t % 3];
+        const bool odd_any = special & 1, bad_any = special & 2;
+#pragma unroll
+      for (int u = 0; u < KEYS / 32; ++u) {
+        f4 s[QW][SUMS][2];
+#pragma unroll
+        for (int x = 0; x < QW; ++x)
+#pragma unroll
+          for (int k = 0; k < SUMS; ++k) s[x][k][0] = s[x][k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < S::STEPS; ++i)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const auto kk = __builtin_bit_cast(typename S::QOp, l.k[tree_unit<S::KU>(32 * u + 16 * b + r, 4 * i + h)]);
+#pragma unroll
+            for (int x = 0; x < QW; ++x)
+#pragma unroll
+              for (int k = 0; k < PARTS; ++k) s[x][k % SUMS][b] = S::M::mma(kk, qf[x][k][i], s[x][k % SUMS][b]);
+          }
+        const int a0 = t * KEYS + 32 * u + 8 * h;
+        f4 ksc[2], vsc[2];
+        if constexpr (S::SCALED)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) ksc[b] = *(const f4 *)&l.ks[32 * u + 8 * h + 4 * b], vsc[b] = *(const f4 *)&l.vs[32 * u + 8 * h + 4 * b];
+        uint32_t there = 0xFF;
+        if (bad_any && !in_pool(page_of(a0))) there = 0;
+        typename S::W::Op pf[QW][3];
+        uint32_t sees[QW];
+#pragma unroll
+        for (int x = 0; x < QW; ++x) {
+          float y[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            y[j] = s[x][SUMS - 1][j >> 2][j & 3];
+            if (SUMS == 2) y[j] = fmaf(y[j], 1.0f / S::MOVE, s[x][0][j >> 2][j & 3]);
+            if constexpr (S::SCALED) y[j] *= ksc[j >> 2][j & 3];
+          }
+          sees[x] = 0xFF;
+          if (edge || bad_any) {
+            sees[x] = there & tree_sees<8>(a, sp, mask[x], node[x], a0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (!(sees[x] >> j & 1)) y[j] = NEG_INF;
+          }
+          acc[x].template weigh<8>(y, c[x], vsc, sees[x], h, scale);
+          pa_parts<BF16>(y, pf[x]);
+        }
+        // (two outputs in turn: a matrix instruction waits for the one before it on the same)
+#pragma unroll
+        for (int i = 0; i < ND; i += 2) {
+          typename S::W::Op v[S::PLANES][2];
+#pragma unroll
+          for (int p = 0; p < S::PLANES; ++p)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              v[p][e] = __builtin_bit_cast(typename S::W::Op, l.v[p][tree_unit<S::VU>(16 * (i + e) + r, 4 * u + h)]);
+          // parts of p (2: least) and of v (1: less)
+          auto add = [&](int k, int p) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 0; x < QW; ++x)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) acc[x].o[i + e] = S::W::mma(pf[x][k], v[p][e], acc[x].o[i + e]);
+          };
+          add(2, 0);
+          if (S::HALF) add(1, S::PLANES - 1);
+          add(1, 0);
+          if (S::HALF) add(0, S::PLANES - 1);
+          add(0, 0);
+        }
+        if (odd_any && edge)
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const uint32_t odd = (uint32_t)(l.odd[16 * i + r] >> (32 * u + 8 * h)) & 0xFF;
+#pragma unroll
+            for (int x = 0; x < QW; ++x) acc[x].spoil(i, tree_count(sees[x], odd, f4{0.0f, 0.0f, 0.0f, 0.0f}));
+          }
+      }
+      }
+      if (more) {
+        if (edge_of(t + 1)) clear_odd(t + 1);
+        store(t + 1, edge_of(t + 1));
+      }
+    }
+
+    // the means, to where they go (a second time: where the first ones are not finite)
+    const bool again = scale != 1.0f;
+    bool over = false;
+    const int64_t runs = (int64_t)a.rows * heads * gridDim.y;
+#pragma unroll
+    for (int x = 0; x < QW; ++x) {
+      const float inv = acc[x].mean();
+      const int mine = w0 + 16 * x + r;
+      if (!direct && !again && h == 0 && mine < nq) {
+        const int64_t run = ((int64_t)row_of(mine) * heads + head_of(mine)) * gridDim.y + blockIdx.y;
+        a.part[runs * DH + 2 * run] = acc[x].m, a.part[runs * DH + 2 * run + 1] = acc[x].sum;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int qr = w0 + 16 * x + 4 * h + i;
+        const float f = __shfl(inv, 4 * h + i);
+        if (qr >= nq) continue;
+        float *dst = direct ? a.out + row_of(qr) * a.ldo + (int64_t)head_of(qr) * DH
+                            : a.part + (((int64_t)row_of(qr) * heads + head_of(qr)) * gridDim.y + blockIdx.y) * DH;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const float y = acc[x].o[d][i] * f;
+          if (!again) dst[16 * d + r] = y;
+          else if (!__builtin_isfinite(dst[16 * d + r]))
+            dst[16 * d + r] = __builtin_isinf(y) && __builtin_isfinite(acc[x].o[d][i]) ? pa_largest(y) : y;
+          over |= !__builtin_isfinite(y);
+        }
+      }
+    }
+    if (!S::WIDE || again || !__syncthreads_or(over)) break;
   }
 }
 
@@ -672,6 +1029,56 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int nsplit, int n
     }
     a.out[row * a.ldo + (int64_t)hq * DH + threadIdx.x] = y;
   }
+}
+
+// The same for up to JOIN_FEW chunks: a wavefront a query, a lane a chunk's weight.
+// (24 trees of up to 48 rows, 32 heads, 7 chunks: .. us, a workgroup each 34.8)
+constexpr int JOIN_FEW = 64;
+template <int DH>
+__global__ __launch_bounds__(256) void k_tree_join_few(TreeArgs a, int nsplit, int nq, int queries) {
+  const int heads = a.kv_heads * a.group, most = a.starts ? a.max_rows : 1;
+  const int i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= queries) return;
+  const int hq = i % heads, tree = i / heads / most, j = i / heads % most;
+  const TreeSpan sp = tree_span(a, tree);
+  if (j >= sp.rows) return;
+  const int u = j * a.group + hq % a.group;
+  const int n = tree_end(a, sp, min(u / nq * nq + nq, sp.rows * a.group));
+  if (n <= a.chunk) return;
+  const int nz = (n + a.chunk - 1) / a.chunk;
+  const int64_t row = sp.start + j, run0 = (row * heads + hq) * nsplit, runs = (int64_t)a.rows * heads * nsplit;
+  const float *ml = a.part + runs * DH + 2 * run0, *o = a.part + run0 * DH;
+  const float m = lane < nz ? ml[2 * lane] : -__builtin_huge_valf(), l = lane < nz ? ml[2 * lane + 1] : 0.0f;
+  float top = m;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const float w = l * pa_weight(m, top);
+  float total = w;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x);
+  const float share = total == 0.0f ? 0.0f : w * (1.0f / total);
+  constexpr int V = (DH + 63) / 64;
+  float y[V] = {};
+  bool finite[V];
+#pragma unroll
+  for (int d = 0; d < V; ++d) finite[d] = true;
+  for (int z0 = 0; z0 < nz; z0 += 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // (four loads on their way; behind the last chunk: it again, of no weight)
+      const int z = min(z0 + e, nz - 1);
+      const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(share), z)), f = z0 + e < nz ? s : 0.0f;
+#pragma unroll
+      for (int d = 0; d < V; ++d)
+        if (DH % 64 == 0 || 64 * d + lane < DH) {
+          const float x = o[z * DH + 64 * d + lane];
+          y[d] += x * f;
+          finite[d] &= (bool)__builtin_isfinite(x);
+        }
+    }
+#pragma unroll
+  for (int d = 0; d < V; ++d)
+    if (DH % 64 == 0 || 64 * d + lane < DH)
+      a.out[row * a.ldo + (int64_t)hq * DH + 64 * d + lane] = __builtin_isinf(y[d]) && finite[d] ? pa_largest(y[d]) : y[d];
 }
 
 #endif  // __HIPCC__
