@@ -19,7 +19,7 @@ namespace rw {
 
 // How a launch cuts its trees' queries and keys, as PagedPlan does for single rows.
 struct TreePlan {
-  int nq;         // queries per workgroup: 16 (k_tree_attn) or 64 (k_tree_shared)
+  int nq;         // queries per workgroup: 16 (k_tree_attn), 64 or 128 (k_tree_shared)
   size_t qtiles;  // workgroups per tree, key head and chunk
   int chunk, nsplit;
   size_t most;
@@ -28,7 +28,7 @@ static TreePlan tree_plan(const rw_kv_pages *p, int n_head, size_t n_trees, size
   TreePlan L{};
   const size_t queries = (size_t)n_head / p->n_head * max_rows;
   max_len = std::min(max_len, (size_t)1 << 30);
-  L.nq = queries <= 16 || p->dtype == RW_F32 ? 16 : 64;
+  L.nq = queries <= 16 || p->dtype == RW_F32 ? 16 : p->dtype == RW_F16 && queries > 64 ? 128 : 64;
   L.qtiles = cdiv(queries, L.nq);
   const size_t base = n_trees * p->n_head * L.qtiles;
   const size_t bytes = max_len * 2 * (p->head_size * pool_size(p->dtype) + (scaled(p->dtype) ? 4 : 0));
@@ -53,10 +53,13 @@ size_t tree_workspace(const rw_kv_pages *p, int n_head, size_t rows, size_t n_tr
 template <class E, int DH>
 static int launch_tree(const TreeArgs &a, const TreePlan &L, size_t join, hipStream_t s) {
   const dim3 grid((unsigned)(cdiv((size_t)a.n_trees * a.kv_heads, 8) * 8 * L.qtiles), (unsigned)L.nsplit);
-  auto *kernel = k_tree_attn<E, DH, 1>;
+  auto *kernel = k_tree_attn<E, DH>;
   if constexpr (!std::is_same_v<E, F32>)
     if (L.nq > 16)
       kernel = 1 << a.pr >= TreeShared<E, DH>::KEYS ? k_tree_shared<E, DH, 1, true> : k_tree_shared<E, DH, 1, false>;
+  if constexpr (std::is_same_v<E, F16>)
+    if (L.nq > 64)
+      kernel = 1 << a.pr >= TreeShared<E, DH>::KEYS ? k_tree_shared<E, DH, 2, true> : k_tree_shared<E, DH, 2, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a);
   SERVE_TRY(launched(L.nq > 16 ? "k_tree_shared" : "k_tree_attn"));
   if (L.nsplit == 1) return RW_OK;

@@ -174,64 +174,100 @@ __global__ __launch_bounds__(256) void k_kv_write8(PagedView w, const float *__r
   }
 }
 
-// Rows of pages as f32: KV_ROWS rows x KV_COLS values per workgroup, v through LDS.
-// A row without a place reads as zeros.
-template <class E>
+// Rows of pages as f32: K8_ROWS rows of one head per workgroup, values as they are
+// stored through LDS.  v's rows are innermost in a page: its words hold GROUP rows of
+// one value, and are read whole where rows follow each other.  A row without a place
+// reads as zeros.
+template <class E, int DH>
 __global__ __launch_bounds__(256) void k_kv_read(PagedView w, float *__restrict__ k, int64_t ldk, float *__restrict__ v,
-                                                 int64_t ldv, int rows, const int32_t *__restrict__ pos, int col_tiles,
-                                                 int tiles, int row0) {
+                                                 int64_t ldv, int rows, const int32_t *__restrict__ pos, int tiles, int row0) {
   using T = typename E::T;
   typedef T In __attribute__((ext_vector_type(8)));
-  __shared__ float sv[KV_ROWS][KV_COLS + 1];
-  __shared__ int page[KV_ROWS], slot[KV_ROWS];
-  const int tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  constexpr int LANES = DH <= 32 ? 4 : DH <= 64 ? 8 : 16;  // of a row; DH / 8 of them have values
+  constexpr int STEP = 256 / LANES, PASSES = K8_ROWS / STEP > 1 ? K8_ROWS / STEP : 1;
+  constexpr int GROUP = 4 / sizeof(T), GROUPS = K8_ROWS / GROUP + (GROUP > 1), WORDS = (GROUPS * DH + 255) / 256;
+  __shared__ alignas(16) T sv[K8_ROWS][DH + 16 / sizeof(T)];
+  __shared__ int page[K8_ROWS], slot[K8_ROWS], whole[GROUPS];  // whole: the page of a group's rows, -1: one by one
+  __shared__ float scale[2][K8_ROWS];
+  const int tile = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);  // gridDim.x: a multiple of 8
   if (tile >= tiles) return;
-  const int n = w.heads * w.dim, t = threadIdx.x;
-  const int r0 = row0 + tile / col_tiles * KV_ROWS, c0 = tile % col_tiles * KV_COLS;
-  if (t < KV_ROWS) {
+  const int t = threadIdx.x, head = tile % w.heads, r0 = row0 + tile / w.heads * K8_ROWS;
+  if (t < K8_ROWS) {
     int at = -1, sl = 0;
     if (r0 + t < rows) at = kv_place(w, r0 + t, pos[r0 + t], &sl);
     page[t] = at, slot[t] = sl;
   }
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < KV_ROWS * KV_COLS / 256; ++j) {
-    const int e = j * 256 + t, row = e % KV_ROWS, c = c0 + e / KV_ROWS;
-    float x = 0.0f;
-    if (c < n && page[row] >= 0) {
-      x = E::load((const T *)w.v + (((int64_t)page[row] * n + c) << w.pr) + slot[row]);
-      if (w.vs) x *= w.vs[(((int64_t)page[row] * w.heads + c / w.dim) << w.pr) + slot[row]];
+  // groups of rows from the first that begins one in its page on (one before it and one behind are short)
+  const int shift = GROUP == 1 ? 0 : (-slot[0] & (GROUP - 1)) - GROUP;
+  if (t < GROUPS) {
+    const int i0 = shift + GROUP * t;
+    int at = -1;
+    if (i0 >= 0 && i0 + GROUP <= K8_ROWS && (slot[i0] & (GROUP - 1)) == 0) {
+      at = page[i0];
+      for (int j = 1; j < GROUP; ++j) at = page[i0 + j] == at && slot[i0 + j] == slot[i0] + j ? at : -1;
     }
-    sv[row][c - c0] = x;
+    whole[t] = at;
   }
-  const int i = t / (KV_COLS / 8), c = c0 + t % (KV_COLS / 8) * 8;
-  const bool in = r0 + i < rows && c < n;
-  f4 y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-  if (in && page[i] >= 0) {
-    const int64_t at = (((int64_t)page[i] * w.heads + c / w.dim) << w.pr) + slot[i];
-    const T *p = (const T *)w.k + at * w.dim + c % w.dim;
-    In a = *(const In *)p;
-    const float s = w.ks ? w.ks[at] : 1.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const T b = a[j];
-      y[j >> 2][j & 3] = E::load(&b) * s;
-    }
-  }
-  if (in) {
-    float *o = k + (int64_t)(r0 + i) * ldk + c;
-    *(f4 *)o = y[0], *(f4 *)(o + 4) = y[1];
+  if (w.ks && t >= 64 && t < 64 + 2 * K8_ROWS) {
+    const int i = t % K8_ROWS, side = (t - 64) / K8_ROWS;
+    scale[side][i] = page[i] < 0 ? 1.0f : (side ? w.vs : w.ks)[(((int64_t)page[i] * w.heads + head) << w.pr) + slot[i]];
   }
   __syncthreads();
-  if (in) {
-    float *o = v + (int64_t)(r0 + i) * ldv + c;
+
+  // all loads on their way before the first is waited for
+  const int d = t % LANES * 8;
+  In a[PASSES];
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      f4 x;
+  for (int p = 0; p < PASSES; ++p) {
+    const int i = min(p * STEP + t / LANES, K8_ROWS - 1);
+    const int64_t row = (((int64_t)max(page[i], 0) * w.heads + head) << w.pr) + slot[i];
+    a[p] = *(const In *)((const T *)w.k + row * DH + min(d, DH - 8));
+  }
+  auto v_at = [&](int at, int value) { return (const T *)w.v + ((((int64_t)at * w.heads + head) * DH + value) << w.pr); };
+  uint32_t word[WORDS];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = sv[i][c - c0 + 4 * p + j];
-      *(f4 *)(o + 4 * p) = x;
+  for (int x = 0; x < WORDS; ++x) {
+    const int e = min(x * 256 + t, GROUPS * DH - 1), g = e % GROUPS, at = whole[g];
+    word[x] = *(const uint32_t *)(v_at(max(at, 0), e / GROUPS) + (at < 0 ? 0 : slot[shift + GROUP * g]));
+  }
+#pragma unroll
+  for (int x = 0; x < WORDS; ++x) {
+    const int e = x * 256 + t, g = e % GROUPS, value = e / GROUPS, i0 = shift + GROUP * g;
+    if (e >= GROUPS * DH) break;
+    T y[GROUP];
+    __builtin_memcpy(y, &word[x], 4);
+    if (whole[g] < 0)
+#pragma unroll
+      for (int j = 0; j < GROUP; ++j) {
+        const int i = i0 + j;
+        y[j] = i >= 0 && i < K8_ROWS && page[i] >= 0 ? v_at(page[i], value)[slot[i]] : (T)0;
+      }
+#pragma unroll
+    for (int j = 0; j < GROUP; ++j)
+      if (GROUP == 1 || (i0 + j >= 0 && i0 + j < K8_ROWS)) sv[i0 + j][value] = y[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int i = p * STEP + t / LANES;
+    if (i >= K8_ROWS || r0 + i >= rows || d >= DH) continue;
+    const In b = *(const In *)&sv[i][d];
+    const bool have = page[i] >= 0;
+    f4 y[2][2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const T xk = a[p][j], xv = b[j];
+      y[0][j >> 2][j & 3] = have ? E::load(&xk) : 0.0f, y[1][j >> 2][j & 3] = E::load(&xv);
     }
+    if (w.ks) {
+      const float sk = scale[0][i], sx = scale[1][i];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) y[0][h] *= sk, y[1][h] *= sx;
+    }
+    float *ok = k + (int64_t)(r0 + i) * ldk + head * DH + d, *ov = v + (int64_t)(r0 + i) * ldv + head * DH + d;
+    *(f4 *)ok = y[0][0], *(f4 *)(ok + 4) = y[0][1];
+    *(f4 *)ov = y[1][0], *(f4 *)(ov + 4) = y[1][1];
   }
 }
 

@@ -198,6 +198,27 @@ static int launch_write8(int dtype, const PagedView &w, const float *k, size_t l
                         : launch_write8_of<E4M3>(w, k, ldk, v, ldv, rows, pos, s);
 }
 
+template <class E>
+static int launch_read(const PagedView &w, float *k, size_t ldk, float *v, size_t ldv, size_t rows, const int32_t *pos, hipStream_t s) {
+  const size_t most = MOST_ROWS / w.heads * K8_ROWS;  // rows of one launch
+  for (size_t row0 = 0; row0 < rows; row0 += most) {
+    const size_t tiles = cdiv(std::min(most, rows - row0), K8_ROWS) * w.heads;
+    const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
+#define RW_READ(DH)                                                                                                    \
+  hipLaunchKernelGGL((k_kv_read<E, DH>), grid, dim3(256), 0, s, w, k, (int64_t)ldk, v, (int64_t)ldv, (int)rows, pos, \
+                     (int)tiles, (int)row0)
+    switch (w.dim) {
+      case 32: RW_READ(32); break;
+      case 64: RW_READ(64); break;
+      case 96: RW_READ(96); break;
+      default: RW_READ(128); break;
+    }
+#undef RW_READ
+    SERVE_TRY(launched("k_kv_read"));
+  }
+  return RW_OK;
+}
+
 // ----------------------------------------------------------------- book
 
 struct rw_kv_book {
@@ -275,19 +296,11 @@ int rw_rocm_kv_read_dev(const rw_kv_pages *pages, size_t layer, float *k, size_t
   int dev;
   SERVE_TRY(call_device(pages->k, "the pages' k", &dev));
   const PagedView w = paged_view(pages, layer, table, ld_table, n_seqs, seq);
-  const size_t cols = cdiv(n, KV_COLS), most = MOST_ROWS / cols * KV_ROWS;  // rows of one launch
-  for (size_t row0 = 0; row0 < rows; row0 += most) {
-    const size_t tiles = cdiv(std::min(most, rows - row0), KV_ROWS) * cols;
-    const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
-#define RW_READ(E)                                                                                                \
-  hipLaunchKernelGGL((k_kv_read<E>), grid, dim3(256), 0, (hipStream_t)stream, w, k, (int64_t)ldk, v, (int64_t)ldv, \
-                     (int)rows, pos, (int)cols, (int)tiles, (int)row0)
-    if (pages->dtype == RW_I8) RW_READ(I8);
-    else if (pages->dtype == RW_E4M3) RW_READ(E4M3);
-    else BY_TYPE(pages->dtype, RW_READ);
+#define RW_READ(E) SERVE_TRY(launch_read<E>(w, k, ldk, v, ldv, rows, pos, (hipStream_t)stream))
+  if (pages->dtype == RW_I8) RW_READ(I8);
+  else if (pages->dtype == RW_E4M3) RW_READ(E4M3);
+  else BY_TYPE(pages->dtype, RW_READ);
 #undef RW_READ
-    SERVE_TRY(launched("k_kv_read"));
-  }
   return RW_OK;
 }
 

@@ -23,7 +23,6 @@ namespace rw {
 
 #if defined(__HIPCC__)
 
-
 // 8 values of a pool of 8 bits, as f16 and as bf16: both exact
 template <class E>
 struct Kv8;
@@ -415,15 +414,15 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf)
   return c;
 }
 
-// One workgroup of PA_WAVES wavefronts per (tree, key/value head, QT tiles of 16
-// queries, chunk of keys).  A wavefront takes every PA_WAVES-th tile of keys, straight from memory, for
+// One workgroup of PA_WAVES wavefronts per (tree, key/value head, 16 queries,
+// chunk of keys).  A wavefront takes every PA_WAVES-th tile of keys, straight from memory, for
 // all of the workgroup's queries.
-template <class E, int DH, int QT>
-__global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(TreeArgs a) {
+template <class E, int DH>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   using M = TreeTile<E, DH>;
   using QOp = typename M::QOp;
   constexpr int ND = DH / 16, KEYS = M::KEYS, PER = M::PER, SUB = M::SUB, PARTS = M::PARTS;
-  constexpr int LD = DH + 4, NQ = 16 * QT;
+  constexpr int LD = DH + 4, NQ = 16;
   constexpr float NEG_INF = -__builtin_huge_valf();
   __shared__ float so[PA_WAVES][NQ][LD], sm[PA_WAVES][NQ], sl[PA_WAVES][NQ];
 
@@ -489,42 +488,30 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
   };
   begin();
 
-  QOp qf[QT][PARTS][M::STEPS];
-  float c[QT];
-  const uint32_t *mask[QT];
-  int node[QT];
-#pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    const int i = min(16 * x + r, nq - 1);
-    node[x] = (u0 + i) / a.group;
-    mask[x] = a.mask ? a.mask + (int64_t)row_of(i) * a.n_words : nullptr;
-    c[x] = tree_q<M>(a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH, 16 * x + r < nq, h, qf[x]);
-  }
+  QOp qf[PARTS][M::STEPS];
+  const int mine = min(r, nq - 1), node = (u0 + mine) / a.group;
+  const uint32_t *mask = a.mask ? a.mask + (int64_t)row_of(mine) * a.n_words : nullptr;
+  const float c = tree_q<M>(a.q + row_of(mine) * a.ldq + (int64_t)head_of(mine) * DH, r < nq, h, qf);
 
   for (float scale = 1.0f;; scale = PA_LOW) {
-    TreeSum<M::SCALED, M::WIDE, ND> acc[QT];
-#pragma unroll
-    for (int x = 0; x < QT; ++x) acc[x].clear();
+    TreeSum<M::SCALED, M::WIDE, ND> acc;
+    acc.clear();
 
     for (; t < end; t += PA_WAVES) {
       load_v(t, now);
       const bool more = t + PA_WAVES < end;
-      f4 s[QT][M::SUMS][SUB];
+      f4 s[M::SUMS][SUB];
 #pragma unroll
-      for (int x = 0; x < QT; ++x)
+      for (int k = 0; k < M::SUMS; ++k)
 #pragma unroll
-        for (int k = 0; k < M::SUMS; ++k)
-#pragma unroll
-          for (int u = 0; u < SUB; ++u) s[x][k][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = 0; u < SUB; ++u) s[k][u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < M::STEPS; ++i)
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
           const QOp kk = tile.k(u, i);
 #pragma unroll
-          for (int x = 0; x < QT; ++x)
-#pragma unroll
-            for (int k = 0; k < PARTS; ++k) s[x][k % M::SUMS][u] = M::mma(kk, qf[x][k][i], s[x][k % M::SUMS][u]);
+          for (int k = 0; k < PARTS; ++k) s[k % M::SUMS][u] = M::mma(kk, qf[k][i], s[k % M::SUMS][u]);
         }
       if (more) load_k(t + PA_WAVES, next);
       // (the pages of the tile after that: they are there when its keys are asked for)
@@ -547,51 +534,45 @@ __global__ __launch_bounds__(64 * PA_WAVES, QT == 1 ? 2 : 1) void k_tree_attn(Tr
         for (int i = 0; i < (ND + 1) / 2; ++i) odd_any |= odd[i] != 0;
         odd_any = __builtin_amdgcn_ballot_w64(odd_any) != 0;
       }
+      float y[PER];
 #pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        float y[PER];
+      for (int j = 0; j < PER; ++j) {
+        y[j] = s[M::SUMS - 1][j >> 2][j & 3];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          y[j] = s[x][M::SUMS - 1][j >> 2][j & 3];
-#pragma unroll
-          for (int k = M::SUMS - 2; k >= 0; --k) y[j] = fmaf(y[j], 1.0f / M::MOVE, s[x][k][j >> 2][j & 3]);
-          if constexpr (M::SCALED) y[j] *= ksc[j >> 2][j & 3];
-        }
-        uint32_t sees = ~0u;
-        if (edge) {
-          sees = now.bad ? 0 : tree_sees<PER>(a, sp, mask[x], node[x], a0);
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if (!(sees >> j & 1)) y[j] = NEG_INF;
-        }
-        acc[x].template weigh<PER>(y, c[x], vsc, sees, h, scale);
-        tile.add(y, acc[x].o);
-        if (odd_any)
-#pragma unroll
-          for (int i = 0; i < ND; ++i) acc[x].spoil(i, M::count(sees, odd[i / 2] >> (16 * (i & 1))));
+        for (int k = M::SUMS - 2; k >= 0; --k) y[j] = fmaf(y[j], 1.0f / M::MOVE, s[k][j >> 2][j & 3]);
+        if constexpr (M::SCALED) y[j] *= ksc[j >> 2][j & 3];
       }
+      uint32_t sees = ~0u;
+      if (edge) {
+        sees = now.bad ? 0 : tree_sees<PER>(a, sp, mask, node, a0);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (!(sees >> j & 1)) y[j] = NEG_INF;
+      }
+      acc.template weigh<PER>(y, c, vsc, sees, h, scale);
+      tile.add(y, acc.o);
+      if (odd_any)
+#pragma unroll
+        for (int i = 0; i < ND; ++i) acc.spoil(i, M::count(sees, odd[i / 2] >> (16 * (i & 1))));
       now = next, next = after;
     }
 
     // the wavefront's means
     const bool first = scale == 1.0f;
     bool over = false;
+    const float inv = acc.mean();
+    if (first && h == 0) sm[wv][r] = acc.m, sl[wv][r] = acc.sum;
 #pragma unroll
-    for (int x = 0; x < QT; ++x) {
-      const float inv = acc[x].mean();
-      if (first && h == 0) sm[wv][16 * x + r] = acc[x].m, sl[wv][16 * x + r] = acc[x].sum;
+    for (int i = 0; i < 4; ++i) {
+      const int qr = 4 * h + i;
+      const float f = __shfl(inv, 4 * h + i);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int qr = 16 * x + 4 * h + i;
-        const float f = __shfl(inv, 4 * h + i);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const float y = acc[x].o[d][i] * f;
-          float &mean = so[wv][qr][16 * d + r];
-          if (!M::WIDE || first) mean = y;
-          else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(acc[x].o[d][i]) ? pa_largest(y) : y;
-          over |= qr < nq && !__builtin_isfinite(y);
-        }
+      for (int d = 0; d < ND; ++d) {
+        const float y = acc.o[d][i] * f;
+        float &mean = so[wv][qr][16 * d + r];
+        if (!M::WIDE || first) mean = y;
+        else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(acc.o[d][i]) ? pa_largest(y) : y;
+        over |= qr < nq && !__builtin_isfinite(y);
       }
     }
     if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
@@ -865,80 +846,80 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
         const int special = flags[t % 3];
         const bool odd_any = special & 1, bad_any = special & 2;
 #pragma unroll
-      for (int u = 0; u < KEYS / 32; ++u) {
-        f4 s[QW][SUMS][2];
+        for (int u = 0; u < KEYS / 32; ++u) {
+          f4 s[QW][SUMS][2];
 #pragma unroll
-        for (int x = 0; x < QW; ++x)
+          for (int x = 0; x < QW; ++x)
 #pragma unroll
-          for (int k = 0; k < SUMS; ++k) s[x][k][0] = s[x][k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = 0; k < SUMS; ++k) s[x][k][0] = s[x][k][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < S::STEPS; ++i)
+          for (int i = 0; i < S::STEPS; ++i)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const auto kk = __builtin_bit_cast(typename S::QOp, l.k[tree_unit<S::KU>(32 * u + 16 * b + r, 4 * i + h)]);
+            for (int b = 0; b < 2; ++b) {
+              const auto kk = __builtin_bit_cast(typename S::QOp, l.k[tree_unit<S::KU>(32 * u + 16 * b + r, 4 * i + h)]);
 #pragma unroll
-            for (int x = 0; x < QW; ++x)
+              for (int x = 0; x < QW; ++x)
 #pragma unroll
-              for (int k = 0; k < PARTS; ++k) s[x][k % SUMS][b] = S::M::mma(kk, qf[x][k][i], s[x][k % SUMS][b]);
+                for (int k = 0; k < PARTS; ++k) s[x][k % SUMS][b] = S::M::mma(kk, qf[x][k][i], s[x][k % SUMS][b]);
+            }
+          const int a0 = t * KEYS + 32 * u + 8 * h;
+          f4 ksc[2], vsc[2];
+          if constexpr (S::SCALED)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) ksc[b] = *(const f4 *)&l.ks[32 * u + 8 * h + 4 * b], vsc[b] = *(const f4 *)&l.vs[32 * u + 8 * h + 4 * b];
+          uint32_t there = 0xFF;
+          if (bad_any && !in_pool(page_of(a0))) there = 0;
+          typename S::W::Op pf[QW][3];
+          uint32_t sees[QW];
+#pragma unroll
+          for (int x = 0; x < QW; ++x) {
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              y[j] = s[x][SUMS - 1][j >> 2][j & 3];
+              if (SUMS == 2) y[j] = fmaf(y[j], 1.0f / S::MOVE, s[x][0][j >> 2][j & 3]);
+              if constexpr (S::SCALED) y[j] *= ksc[j >> 2][j & 3];
+            }
+            sees[x] = 0xFF;
+            if (edge || bad_any) {
+              sees[x] = there & tree_sees<8>(a, sp, mask[x], node[x], a0);
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (!(sees[x] >> j & 1)) y[j] = NEG_INF;
+            }
+            acc[x].template weigh<8>(y, c[x], vsc, sees[x], h, scale);
+            pa_parts<BF16>(y, pf[x]);
           }
-        const int a0 = t * KEYS + 32 * u + 8 * h;
-        f4 ksc[2], vsc[2];
-        if constexpr (S::SCALED)
+          // (two outputs in turn: a matrix instruction waits for the one before it on the same)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) ksc[b] = *(const f4 *)&l.ks[32 * u + 8 * h + 4 * b], vsc[b] = *(const f4 *)&l.vs[32 * u + 8 * h + 4 * b];
-        uint32_t there = 0xFF;
-        if (bad_any && !in_pool(page_of(a0))) there = 0;
-        typename S::W::Op pf[QW][3];
-        uint32_t sees[QW];
+          for (int i = 0; i < ND; i += 2) {
+            typename S::W::Op v[S::PLANES][2];
 #pragma unroll
-        for (int x = 0; x < QW; ++x) {
-          float y[8];
+            for (int p = 0; p < S::PLANES; ++p)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            y[j] = s[x][SUMS - 1][j >> 2][j & 3];
-            if (SUMS == 2) y[j] = fmaf(y[j], 1.0f / S::MOVE, s[x][0][j >> 2][j & 3]);
-            if constexpr (S::SCALED) y[j] *= ksc[j >> 2][j & 3];
+              for (int e = 0; e < 2; ++e)
+                v[p][e] = __builtin_bit_cast(typename S::W::Op, l.v[p][tree_unit<S::VU>(16 * (i + e) + r, 4 * u + h)]);
+            // parts of p (2: least) and of v (1: less)
+            auto add = [&](int k, int p) __attribute__((always_inline)) {
+#pragma unroll
+              for (int x = 0; x < QW; ++x)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) acc[x].o[i + e] = S::W::mma(pf[x][k], v[p][e], acc[x].o[i + e]);
+            };
+            add(2, 0);
+            if (S::HALF) add(1, S::PLANES - 1);
+            add(1, 0);
+            if (S::HALF) add(0, S::PLANES - 1);
+            add(0, 0);
           }
-          sees[x] = 0xFF;
-          if (edge || bad_any) {
-            sees[x] = there & tree_sees<8>(a, sp, mask[x], node[x], a0);
+          if (odd_any && edge)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (!(sees[x] >> j & 1)) y[j] = NEG_INF;
-          }
-          acc[x].template weigh<8>(y, c[x], vsc, sees[x], h, scale);
-          pa_parts<BF16>(y, pf[x]);
+            for (int i = 0; i < ND; ++i) {
+              const uint32_t odd = (uint32_t)(l.odd[16 * i + r] >> (32 * u + 8 * h)) & 0xFF;
+#pragma unroll
+              for (int x = 0; x < QW; ++x) acc[x].spoil(i, tree_count(sees[x], odd, f4{0.0f, 0.0f, 0.0f, 0.0f}));
+            }
         }
-        // (two outputs in turn: a matrix instruction waits for the one before it on the same)
-#pragma unroll
-        for (int i = 0; i < ND; i += 2) {
-          typename S::W::Op v[S::PLANES][2];
-#pragma unroll
-          for (int p = 0; p < S::PLANES; ++p)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              v[p][e] = __builtin_bit_cast(typename S::W::Op, l.v[p][tree_unit<S::VU>(16 * (i + e) + r, 4 * u + h)]);
-          // parts of p (2: least) and of v (1: less)
-          auto add = [&](int k, int p) __attribute__((always_inline)) {
-#pragma unroll
-            for (int x = 0; x < QW; ++x)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) acc[x].o[i + e] = S::W::mma(pf[x][k], v[p][e], acc[x].o[i + e]);
-          };
-          add(2, 0);
-          if (S::HALF) add(1, S::PLANES - 1);
-          add(1, 0);
-          if (S::HALF) add(0, S::PLANES - 1);
-          add(0, 0);
-        }
-        if (odd_any && edge)
-#pragma unroll
-          for (int i = 0; i < ND; ++i) {
-            const uint32_t odd = (uint32_t)(l.odd[16 * i + r] >> (32 * u + 8 * h)) & 0xFF;
-#pragma unroll
-            for (int x = 0; x < QW; ++x) acc[x].spoil(i, tree_count(sees[x], odd, f4{0.0f, 0.0f, 0.0f, 0.0f}));
-          }
-      }
       }
       if (more) {
         if (edge_of(t + 1)) clear_odd(t + 1);
