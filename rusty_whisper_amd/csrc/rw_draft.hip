@@ -18,6 +18,15 @@ using namespace rw;
 namespace rw {
 
 // How a launch cuts its trees' queries and keys, as PagedPlan does for single rows.
+// Queries: 16 per workgroup where no more are there and for f32 (whose products take 16
+// times bf16's time each, so that sharing loads gains nothing).  64 with keys and values through LDS
+// otherwise; f16 pools 128 from 65 on, since each value is there in two parts and a part
+// read from LDS then has two products: 4 chunks of 512 rows behind 4100, 8 heads of 4 x 128: 487 us by
+// 128, 626 by 64; bf16 and 8-bit pools 524 and 530 by 128, 512 and 528 by 64.
+// Keys: in one chunk up to 256 KB a head.  One tree is cut as far as the join goes, a batch
+// into chunks of 192 KB, as many as fill the device's 512 workgroups some four times over:
+// 24 trees of up to 48 rows of 8 heads of 4 x 128, up to 6048 keys, i8: 600 in all 258 us, 1200 191, 2048 188, 4096 186; 61
+// single rows of up to 8191 keys, e4m3: chunks of 96 KB 126 us, 192 KB 110, 384 KB 111.
 struct TreePlan {
   int nq;         // queries per workgroup: 16 (k_tree_attn), 64 or 128 (k_tree_shared)
   size_t qtiles;  // workgroups per tree, key head and chunk
@@ -36,7 +45,7 @@ static TreePlan tree_plan(const rw_kv_pages *p, int n_head, size_t n_trees, size
   if (bytes > (size_t)256 << 10) {
     nsplit = std::min(cdiv(bytes, (size_t)128 << 10), (size_t)PA_MAX_SPLIT / base);
     if (n_trees > 1)
-      nsplit = std::max(nsplit, std::min(cdiv(bytes, (size_t)192 << 10), std::min((size_t)(L.nq > 16 ? 2048 : 4096), 256 * n_trees) / base));
+      nsplit = std::max(nsplit, std::min(cdiv(bytes, (size_t)192 << 10), std::min((size_t)2048, 256 * n_trees) / base));
     nsplit = std::max((size_t)1, nsplit);
   }
   L.most = nsplit;

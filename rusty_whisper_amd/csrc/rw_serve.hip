@@ -198,14 +198,14 @@ static int launch_write8(int dtype, const PagedView &w, const float *k, size_t l
                         : launch_write8_of<E4M3>(w, k, ldk, v, ldv, rows, pos, s);
 }
 
-template <class E>
-static int launch_read(const PagedView &w, float *k, size_t ldk, float *v, size_t ldv, size_t rows, const int32_t *pos, hipStream_t s) {
-  const size_t most = MOST_ROWS / w.heads * K8_ROWS;  // rows of one launch
+template <class E, int ROWS>
+static int launch_read_of(const PagedView &w, float *k, size_t ldk, float *v, size_t ldv, size_t rows, const int32_t *pos, hipStream_t s) {
+  const size_t most = MOST_ROWS / w.heads * ROWS;  // rows of one launch
   for (size_t row0 = 0; row0 < rows; row0 += most) {
-    const size_t tiles = cdiv(std::min(most, rows - row0), K8_ROWS) * w.heads;
+    const size_t tiles = cdiv(std::min(most, rows - row0), ROWS) * w.heads;
     const dim3 grid((unsigned)cdiv(tiles, 8) * 8);
 #define RW_READ(DH)                                                                                                    \
-  hipLaunchKernelGGL((k_kv_read<E, DH>), grid, dim3(256), 0, s, w, k, (int64_t)ldk, v, (int64_t)ldv, (int)rows, pos, \
+  hipLaunchKernelGGL((k_kv_read<E, DH, ROWS>), grid, dim3(256), 0, s, w, k, (int64_t)ldk, v, (int64_t)ldv, (int)rows, pos, \
                      (int)tiles, (int)row0)
     switch (w.dim) {
       case 32: RW_READ(32); break;
@@ -217,6 +217,13 @@ static int launch_read(const PagedView &w, float *k, size_t ldk, float *v, size_
     SERVE_TRY(launched("k_kv_read"));
   }
   return RW_OK;
+}
+
+// (ROWS = 64 where that still fills the device: see k_kv_read)
+template <class E>
+static int launch_read(const PagedView &w, float *k, size_t ldk, float *v, size_t ldv, size_t rows, const int32_t *pos, hipStream_t s) {
+  return rows * w.heads >= ((size_t)1 << 17) ? launch_read_of<E, 64>(w, k, ldk, v, ldv, rows, pos, s)
+                                             : launch_read_of<E, 32>(w, k, ldk, v, ldv, rows, pos, s);
 }
 
 // ----------------------------------------------------------------- book

@@ -175,6 +175,36 @@ def test_rows_read_back(kind, heads, dim, page):
             assert np.array_equal(got.cpu().numpy()[at], x[:, pos[at]].transpose(1, 0, 2).reshape(-1, n).astype(np.float32))
 
 
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("heads,dim,page", [(40, 32, 16), (40, 96, 64), (80, 64, 32)])
+def test_many_rows_read_back(kind, heads, dim, page):
+    # (what is read by 64 rows at a time): runs of rows, single ones, and some without a place
+    lens = [20 * page, 13 * page + 3]
+    pool = any_pool(kind, 1, 36, heads, page, dim, 4)
+    table = tables(lens, page, 36, 5)
+    rng = np.random.default_rng(1)
+    rows = 131072 // heads + 37
+    seq, pos = rng.integers(0, 2, rows), np.zeros(rows, np.int64)
+    r = 0
+    while r < rows:
+        n = min(rows - r, int(rng.choice([1, 2, 7, 64, 100])))
+        s = int(rng.integers(0, 2))
+        first = int(rng.integers(0, lens[s]))
+        seq[r : r + n], pos[r : r + n] = s, (first + np.arange(n)) % lens[s]
+        r += n
+    gone = rng.random(rows) < 0.03
+    pos[gone] = -1
+    n = heads * dim
+    k, v = torch.empty(rows, n, device="cuda"), torch.empty(rows, n, device="cuda")
+    A.kv_read_dev(A.KvPages(*pool), 0, k, v, rows, i32(table), i32(pos), seq=i32(seq))
+    for s in range(2):
+        K, V = gather_any(pool, 0, table[s, : -(-lens[s] // page)], lens[s])
+        at = (seq == s) & ~gone
+        for got, x in ((k, K), (v, V)):
+            assert np.array_equal(got.cpu().numpy()[at], x[:, pos[at]].transpose(1, 0, 2).reshape(-1, n).astype(np.float32))
+    assert not k.cpu().numpy()[gone].any() and not v.cpu().numpy()[gone].any()
+
+
 @pytest.mark.parametrize("kind", KINDS8)
 def test_page_copies_take_the_scales(kind):
     pool = any_pool(kind, 3, 9, 2, 16, 32, 3)
