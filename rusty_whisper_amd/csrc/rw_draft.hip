@@ -235,7 +235,7 @@ int rw_rocm_sample_tokens_dev(int dtype, const void *logits, size_t ld, size_t r
   CallWorkspace hold;
   void *ws = nullptr;
   SERVE_TRY(hold.take(dev, workspace, workspace_len, rw_rocm_sample_tokens_workspace_size(rows, n_vocab), stream, &ws));
-  const SampleArgs a{u, temperature, top_k, top_p, min_p, tokens, logprobs, (int64_t)ld, (int)n_vocab};
+  const SampleArgs a{u, temperature, top_k, top_p, min_p, tokens, logprobs, (int64_t)ld, (int)n_vocab, (int)rows};
   return sample_launch(dtype, logits, a, rows, (hipStream_t)stream);
 }
 

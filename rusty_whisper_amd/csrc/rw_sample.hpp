@@ -38,7 +38,7 @@ struct SampleArgs {
   uint32_t *tokens;
   float *logprobs;
   int64_t ld;
-  int n;
+  int n, rows;
 };
 
 #if defined(__HIPCC__)
@@ -425,7 +425,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 4) void k_sample(const typename E::
   constexpr float INF = __builtin_huge_valf();
   constexpr int V = SampleRow<E>::V;
   __shared__ SampleShared s;
-  const int64_t r = blockIdx.x;
+  const int64_t r = blockIdx.y * (int64_t)gridDim.x + blockIdx.x;
+  if (r >= a.rows) return;
   const SampleRow<E> row(logits + r * a.ld, a.n);
   const float t = a.temperature ? a.temperature[r] : 1.0f, u = a.u[r];
   const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f;
@@ -526,7 +527,9 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 4) void k_sample(const typename E::
 
 template <class E>
 int sample_launch_of(const void *logits, const SampleArgs &a, size_t rows, hipStream_t s) {
-  hipLaunchKernelGGL((k_sample<E>), dim3((unsigned)rows), dim3(SAMPLE_THREADS), 0, s, (const typename E::T *)logits, a);
+  const size_t x = std::min(rows, (size_t)1 << 20);  // (2^32 threads side by side are too many for a launch)
+  const dim3 grid((unsigned)x, (unsigned)cdiv(rows, x));
+  hipLaunchKernelGGL((k_sample<E>), grid, dim3(SAMPLE_THREADS), 0, s, (const typename E::T *)logits, a);
   return launched("k_sample");
 }
 

@@ -109,6 +109,45 @@ def test_rows_that_cannot_be_kept(kind):
     assert torch.equal(bytes_of(pool[0])[0, 0, :, 1], bytes_of(pool[0])[0, 0, :, 3])
 
 
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+def test_a_captured_end_of_a_step_replayed_with_other_contents(kind):
+    """Accepted paths and their rows in one graph, beside eager work on a stream of its own."""
+    rng = np.random.default_rng(4)
+    heads, dim, page, layers, sizes, past = 2, 64, 16, 3, [30, 17, 40], [5, 0, 22]
+    lens = np.add(past, sizes)
+    table = tables(lens, page, 9, 6)
+    starts = np.concatenate([[0], np.cumsum(sizes)])
+    total, most = int(starts[-1]), max(sizes)
+    pool = any_pool(kind, layers, 9, heads, page, dim, 5)
+    eager = [x.clone() for x in pool]
+    dev = dict(tokens=i32(np.zeros(total)), parent=i32(np.zeros(total)), sampled=i32(np.zeros(total)), starts=i32(starts), table=i32(table),
+               past=i32(past))
+    made = [torch.zeros((3, most), dtype=torch.int32, device="cuda")] + [torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(2)]
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+    def step(pages, s):
+        A.tree_accept_dev(dev["tokens"], dev["parent"], dev["sampled"], total, dev["starts"], most, *made, stream=s)
+        A.kv_keep_rows_dev(pages, dev["table"], dev["past"], made[0], made[1], stream=s)
+
+    with torch.cuda.graph(graph, stream=stream):
+        step(A.KvPages(*pool), stream.cuda_stream)
+    for turn in range(4):
+        parent = np.concatenate([np.array(p, np.int64) for p in trees(rng, sizes)])
+        for name, x in (("tokens", rng.integers(0, 2, total)), ("sampled", rng.integers(0, 2, total)), ("parent", parent)):
+            dev[name].copy_(i32(x))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        by_graph = [x.cpu().numpy() for x in made]
+        step(A.KvPages(*eager), 0)
+        torch.cuda.synchronize()
+        for a, b in zip(by_graph, made):
+            assert np.array_equal(a, b.cpu().numpy())
+        assert by_graph[1].max() > 1  # something moved
+        for a, b in zip(pool, eager):
+            assert torch.equal(bytes_of(a), bytes_of(b))
+
+
 LAYERS, HEADS, GROUP, DIM, PAGE, N_PAGES, VOCAB = 2, 2, 2, 64, 16, 40, 499
 N = HEADS * DIM
 

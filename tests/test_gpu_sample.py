@@ -204,3 +204,16 @@ def test_a_captured_call_replayed_with_other_contents():
         graph.replay()
         torch.cuda.synchronize()
         check(logits, u.cpu().numpy(), (tok.cpu().numpy().view(np.uint32), lp.cpu().numpy()), top_p=0.9)
+
+
+def test_more_rows_than_a_launch_has_threads_for():
+    rows = 2**23  # of 512 threads each
+    x = torch.rand(rows, 1, device="cuda").repeat(1, 2)
+    x[:, 0] += 1
+    x[rows - 5, 1] = 3
+    tok = torch.full((rows,), 77, dtype=torch.int32, device="cuda")
+    A.sample_tokens_dev(x, rows, 2, torch.zeros(rows, device="cuda"), tok)
+    torch.cuda.synchronize()
+    assert tok[rows - 5] == 1
+    tok[rows - 5] = 0
+    assert not tok.any()

@@ -130,6 +130,41 @@ def test_over_chunks_of_keys(kind, n_trees, past, nodes, heads, dim, group):
         c.check(c.run())
 
 
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("n_trees,past,nodes,heads,dim,group,page", [(1, 30000, 21, 1, 64, 4, 16), (3, 5000, 50, 2, 128, 3, 256),
+                                                                    (2, 3000, 70, 1, 96, 2, 32), (2, 2500, 9, 2, 32, 8, 128)])
+def test_many_queries_over_chunks_of_keys(kind, n_trees, past, nodes, heads, dim, group, page):
+    """(keys and values shared by 64 or 128 queries: pages longer and shorter than their tiles)"""
+    rng = np.random.default_rng(nodes)
+    pasts = [past] + [int(rng.integers(0, past)) for _ in range(n_trees - 1)]
+    sizes = [nodes] + [int(rng.integers(1, nodes + 1)) for _ in range(n_trees - 1)]
+    for masks in ([rng.random((n, n)) < 0.3 for n in sizes], None):
+        c = Call(kind, heads, group, dim, page, pasts, sizes, masks, seed=past)
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("page", [16, 128])
+def test_many_queries_with_pages_that_are_not_there(kind, page):
+    """Their rows, in the middle and at the end, are not seen, whatever v's tile held."""
+    n, past, nodes = 2, [300, 700], [20, 33]
+    c = Call(kind, 1, 4, 64, page, past, nodes, None, seed=11)
+    whole = c.table.copy()
+    gone = [np.zeros(p + m, bool) for p, m in zip(past, nodes)]
+    for i in range(n):
+        for at in (1, (past[i] + nodes[i] - 1) // page):
+            gone[i][at * page : (at + 1) * page] = True
+            c.table[c.seq[i]][at] = c.n_pages if at == 1 else -1
+    got = c.run()
+    for i in range(n):
+        K, V = gather_any(c.pool, 1, whole[c.seq[i]][: -(-(past[i] + nodes[i]) // page)], past[i] + nodes[i])
+        for j in range(nodes[i]):
+            r = c.starts[i] + j
+            seen = (np.arange(past[i] + nodes[i]) <= past[i] + j) & ~gone[i]
+            y, tol = attend(c.q[r].double().cpu().numpy().reshape(4, -1), K[:, seen], V[:, seen])
+            assert np.all(np.abs(got[r].reshape(4, -1) - y) <= tol), (i, j)
+
+
 def spoil(c, tree, node, what):
     """k, v (and scales) of a node's row become `what`."""
     row = int(c.past[tree]) + node
@@ -290,3 +325,26 @@ def test_rows_at_a_distance():
     got = c.run(out=out[:, 4:260])
     assert np.array_equal(got, want)
     assert torch.all(out[:, :4] == 5) and torch.all(out[:, 260:] == 5)
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("nodes", [3, 50])
+def test_pages_behind_4_gib(kind, nodes):
+    """The same pages at the far end of a large pool: the same bits."""
+    c = Call(kind, 1, 2, 128, 128, [700, 90], [nodes, nodes], None, seed=12)
+    want = c.run()
+    small, size = c.pool, bytes_of(c.pool[0]).element_size()
+    far = 2**32 // (128 * 128 * size) + 50  # pages of a layer
+    c.pool = [torch.empty((x.shape[0], far) + tuple(x.shape[2:]), dtype=x.dtype, device="cuda") for x in small]
+    for big, x in zip(c.pool, small):
+        bytes_of(big)[:, far - c.n_pages :] = bytes_of(x)
+    c.table = c.table + np.int32(far - c.n_pages)
+    assert np.array_equal(c.run(), want)
+    # ... and rows read back from there
+    rows = 790
+    k, v = (torch.empty(rows, 128, device="cuda") for _ in range(2))
+    A.kv_read_dev(A.KvPages(*c.pool), 1, k, v, rows, i32(c.table), i32(np.arange(rows) % 90), seq=i32(np.arange(rows) % 2))
+    K, V = gather_any(small, 1, c.table[1, : 1] - np.int32(far - c.n_pages), 90)
+    at = np.arange(rows) % 2 == 1
+    for got, x in ((k, K), (v, V)):
+        assert np.array_equal(got.cpu().numpy()[at], x[:, np.arange(rows)[at] % 90].transpose(1, 0, 2).reshape(-1, 128).astype(np.float32))
