@@ -436,9 +436,13 @@ size_t rw_rocm_logits_topk_workspace_size(size_t rows, size_t n_vocab, size_t k)
  *   k  [n_layer][n_pages][n_head][page_rows][head_size]
  *   v  [n_layer][n_pages][n_head][head_size][page_rows]
  * (v with the rows of a page innermost: the order in which attention's
- * products read it).  dtype is RW_F32, RW_F16 or RW_BF16, head_size 32, 64, 96
- * or 128, page_rows 16, 32, 64, 128 or 256; n_head counts key/value heads; k and v
- * are 16-byte aligned.  The struct is read during the calls only.
+ * products read it).  dtype is RW_F32, RW_F16, RW_BF16, or one of 8 bits: RW_I8 (whole
+ * numbers -127 .. 127) or RW_E4M3 (1 sign, 4 exponent and 3 fraction bits, largest 448);
+ * head_size 32, 64, 96 or 128, page_rows 16, 32, 64, 128 or 256; n_head counts
+ * key/value heads; k and v are 16-byte aligned.  Values of 8 bits have one scale per
+ * row and head, k's in k_scale and v's in v_scale, f32, 16-byte aligned:
+ *   k_scale, v_scale  [n_layer][n_pages][n_head][page_rows]
+ * and stand for value times scale (read back: rounded once to f32).  The struct is read during the calls only.
  *
  * The entries below take device pointers on the current device and are queued
  * on `stream`.  The table is [n_seqs][ld_table] page ids: row s lists the pages
@@ -460,14 +464,20 @@ typedef struct rw_kv_pages {
 /* Rows k[r], v[r] (f32 [rows, n_head * head_size], row strides ldk, ldv in
  * floats, 16-byte aligned) become row pos[r] of sequence seq[r] in `layer`,
  * rounded once to the pool's type (to infinity beyond its range).  Where two
- * rows of a call have the same place, the place holds values of either. */
+ * rows of a call have the same place, the place holds values of either.
+ * 8 bits: the scale of a row's head is its largest magnitude / 127 (RW_I8) or
+ * 448 (RW_E4M3) in f32, at least 2^-126; a value is the nearest that the type has to
+ * x / scale, ties to even: it reads back within scale / 2 of x (RW_I8), within 2^-4 of x
+ * or 2^-10 of the scale, the larger (RW_E4M3).  A row's head that holds an infinity or a NaN gets
+ * the scale NaN and reads back as NaN.  (Two rows with the same place: values and scales of
+ * either, in any mix.) */
 int rw_rocm_kv_write_dev(const rw_kv_pages *pages, size_t layer, const float *k, size_t ldk, const float *v, size_t ldv,
                          size_t rows, const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq,
                          const int32_t *pos, void *stream);
 
 /* The reverse: rows pos[r] of sequences seq[r] in `layer` as f32 rows k[r], v[r]
- * (layout and strides as for rw_rocm_kv_write_dev; exactly what attention
- * takes them for).  A row whose place the table does not have gets zeros. */
+ * (layout and strides as for rw_rocm_kv_write_dev): what attention takes them
+ * for, exactly but for a scale's product, which is rounded once.  A row whose place the table does not have gets zeros. */
 int rw_rocm_kv_read_dev(const rw_kv_pages *pages, size_t layer, float *k, size_t ldk, float *v, size_t ldv, size_t rows,
                         const int32_t *table, size_t ld_table, size_t n_seqs, const int32_t *seq, const int32_t *pos,
                         void *stream);
@@ -491,7 +501,8 @@ int rw_rocm_kv_copy_pages_dev(const rw_kv_pages *pages, const int32_t *src, cons
  * replays will see.  Scores, softmax and sums are f32, products as exact as
  * f32's for every type of pool, weights down to 2^-126 of the largest and values
  * of any size (f16 pools: values of q below 2^-37 of their head's largest lose
- * bits).  The rows seen and q must be finite, scores within f32's range; what the
+ * bits; 8-bit pools: q keeps 22 bits, of values below 2^-29 of their head's largest
+ * fewer).  The rows seen and q must be finite, scores within f32's range; what the
  * pool holds behind a sequence's length has no effect.
  * The workspace (NULL: one kept per (device, stream), not for a stream that
  * is being captured) holds rw_rocm_paged_attention_workspace_size bytes, 16-byte
@@ -513,8 +524,8 @@ int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const fl
  *               per row r of the call; its own bit too, where it is to see itself);
  *               words or bits beyond the tree's nodes are nothing
  * Rows of other trees are never seen.  Otherwise as
- * rw_rocm_paged_attention_dev (heads, layout, precision; a row that sees nothing
- * gets zeros), and a row of the pool that a node does not see may hold
+ * rw_rocm_paged_attention_dev (heads, layout, precision, f16 pools' q as 8-bit ones'; a
+ * row that sees nothing gets zeros), and a row of the pool that a node does not see may hold
  * anything, infinities and NaN too, also where other nodes see it.  Rows of q
  * and out in no tree are left as they were.  max_rows: the most nodes of a
  * tree (those beyond are left out); max_len: the largest past + nodes; rows counts q's.
