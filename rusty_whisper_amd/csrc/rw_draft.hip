@@ -212,10 +212,8 @@ int rw_rocm_kv_keep_rows_dev(const rw_kv_pages *pages, const int32_t *table, siz
   return RW_OK;
 }
 
-size_t rw_rocm_sample_tokens_workspace_size(size_t rows, size_t n_vocab) {
-  if (rows == 0 || rows > MOST_ROWS || n_vocab == 0 || n_vocab > SAMPLE_VOCAB) return 0;
-  return 0;
-}
+// (a row's histograms are in its workgroup's LDS)
+size_t rw_rocm_sample_tokens_workspace_size(size_t, size_t) { return 0; }
 
 int rw_rocm_sample_tokens_dev(int dtype, const void *logits, size_t ld, size_t rows, size_t n_vocab, const float *u,
                               const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
