@@ -455,32 +455,30 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   const int end = (min(n, k0 + a.chunk) + KEYS - 1) / KEYS;
   const int P = 1 << a.pr;
 
-  // the pages of this lane's k rows (keys PER (r / 4) on of a tile) and of its values (PER h on)
+  // The pages of this lane's k rows (keys PER (r / 4) on of a tile) and of its values (PER h
+  // on).  Only read here: what is computed of them waits for them, and for the loads before them
   struct Where {
-    int64_t k, v;  // first row of the head, in rows of DH
-    bool bad;      // the page of the lane's values, and scores, is not in the pool
+    int k, v;
   };
   auto where = [&](int t) __attribute__((always_inline)) {
-    Where w;
-    const int pk = sp.table[min(t * KEYS + PER * (r >> 2), n - 1) >> a.pr], pv = sp.table[min(t * KEYS + PER * h, n - 1) >> a.pr];
-    const bool bk = (unsigned)pk >= (unsigned)a.n_pages;
-    w.bad = (unsigned)pv >= (unsigned)a.n_pages;
-    w.k = ((int64_t)(bk ? 0 : pk) * a.kv_heads + hk) << a.pr;
-    w.v = ((int64_t)(w.bad ? 0 : pv) * a.kv_heads + hk) << a.pr;
-    return w;
+    return Where{sp.table[min(t * KEYS + PER * (r >> 2), n - 1) >> a.pr], sp.table[min(t * KEYS + PER * h, n - 1) >> a.pr]};
   };
+  auto in_pool = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
+  auto first = [&](int page) { return ((int64_t)(in_pool(page) ? page : 0) * a.kv_heads + hk) << a.pr; };  // row of the head
   M tile;
   f4 ksc[M::SCALED ? SUB : 1], vsc[M::SCALED ? SUB : 1];
   auto load_k = [&](int t, const Where &w) __attribute__((always_inline)) {
+    const int64_t row = first(w.k);
 #pragma unroll
-    for (int s = 0; s < SUB; ++s) tile.load_k(a.k, w.k * DH, s, (t * KEYS + PER * (r >> 2) + 4 * s + (r & 3)) & (P - 1), h);
+    for (int s = 0; s < SUB; ++s) tile.load_k(a.k, row * DH, s, (t * KEYS + PER * (r >> 2) + 4 * s + (r & 3)) & (P - 1), h);
   };
   auto load_v = [&](int t, const Where &w) __attribute__((always_inline)) {
     const int slot = (t * KEYS + PER * h) & (P - 1);
-    tile.load_v(a.v, w.v * DH, slot, r, a.pr);
+    const int64_t row = first(w.v);
+    tile.load_v(a.v, row * DH, slot, r, a.pr);
     if constexpr (M::SCALED)
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) ksc[s] = *(const f4 *)(a.ks + w.v + slot + 4 * s), vsc[s] = *(const f4 *)(a.vs + w.v + slot + 4 * s);
+      for (int s = 0; s < SUB; ++s) ksc[s] = *(const f4 *)(a.ks + row + slot + 4 * s), vsc[s] = *(const f4 *)(a.vs + row + slot + 4 * s);
   };
 
   const int t0 = k0 / KEYS + wv;
@@ -517,19 +515,20 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
 #pragma unroll
           for (int k = 0; k < PARTS; ++k) s[k % M::SUMS][u] = M::mma(kk, qf[k][i], s[k % M::SUMS][u]);
         }
-      if (more) load_k(t + PA_WAVES, next);
-      // (the pages of the tile after that: they are there when its keys are asked for)
+      // (the pages of the tile after the next: they are there when its keys are asked for)
       Where after{};
       if (t + 2 * PA_WAVES < end) after = where(t + 2 * PA_WAVES);
+      if (more) load_k(t + PA_WAVES, next);
 
       // keys that no query of the call may see, or that are in no page of the pool: no
       // weight, and what v holds there (anything) is taken as zero
       const int a0 = t * KEYS + PER * h;
-      const bool edge = (t + 1) * KEYS > min(n, sp.past) || __builtin_amdgcn_ballot_w64(now.bad);
+      const bool bad = !in_pool(now.v);
+      const bool edge = (t + 1) * KEYS > min(n, sp.past) || __builtin_amdgcn_ballot_w64(bad);
       bool odd_any = false;
       uint32_t odd[(ND + 1) / 2] = {};  // 16 bits for each i
       if (edge) {
-        tile.keep_v(now.bad ? 0 : n - a0);
+        tile.keep_v(bad ? 0 : n - a0);
         // a row that one query sees and another does not may hold infinities or NaN:
         // they leave the products and are given to those who see them
 #pragma unroll
@@ -548,7 +547,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
       }
       uint32_t sees = ~0u;
       if (edge) {
-        sees = now.bad ? 0 : tree_sees<PER>(a, sp, mask, node, a0);
+        sees = bad ? 0 : tree_sees<PER>(a, sp, mask, node, a0);
 #pragma unroll
         for (int j = 0; j < PER; ++j)
           if (!(sees >> j & 1)) y[j] = NEG_INF;
