@@ -381,7 +381,10 @@ struct TreeSum {
 };
 
 // Query r's values in the scores' operand order; f16 parts: scaled by a power of two
-// so that the largest lies in [2^14, 2^15), undone in the factor that is returned
+// so that the largest lies in [2^14, 2^15), undone in the factor that is returned.  That power is 2^120
+// at most, so that the factor (2^-120 times 0.13 and more) is no zero, which times an unseen
+// key's -inf would be NaN: values below 2^-105 then lie lower, where a subnormal one, a multiple of
+// 2^-149, still is the sum of its two parts, and a normal one, at 2^-6 at least, keeps 22 bits.
 template <class M, class T>
 __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf) {
   float c = PA_LOG2E / __builtin_sqrtf((float)M::HEAD);
@@ -398,7 +401,7 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf)
   if (M::MOVE != 1.0f) {
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+    e = top > 0.0f ? max(__builtin_amdgcn_frexp_expf(top) - 15, -120) : 0;
     c = ldexpf(c, e);
   }
 #pragma unroll

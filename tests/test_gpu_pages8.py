@@ -323,3 +323,19 @@ def test_a_captured_call_replayed_with_other_contents(kind):
         out.zero_()
         with pytest.raises(A.RwError, match="captured call needs a workspace"):
             A.paged_attention_dev(pages, 0, q, rows, heads * 2, t, n, most, out, stream=torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("kind", KINDS8)
+@pytest.mark.parametrize("q_power,k_power", [(-149, 0), (-140, 0), (-134, 0), (-120, 0), (-101, 0), (-40, 0)])
+@pytest.mark.parametrize("group", [1, 20])
+def test_queries_and_key_scales_of_any_size(kind, q_power, k_power, group):
+    heads, dim, page, lens = 2, 64, 32, [200, 1, 77]
+    table = tables(lens, page, 12, 1)
+    pool = any_pool(kind, 1, 12, heads, page, dim, 2)
+    pool[2] = torch.from_numpy(np.ldexp(pool[2].double().cpu().numpy(), k_power).astype(np.float32)).cuda()
+    q = np.random.default_rng(7).standard_normal((3, heads * group * dim)) * 2
+    q = torch.from_numpy(np.ldexp(q, q_power).astype(np.float32)).cuda()
+    assert torch.any(q != 0)
+    got = attention(pool, 0, q, heads * group, table, lens, 200)
+    assert np.isfinite(got).all()
+    check_attention(pool, kind, 0, q, heads * group, table, lens, np.arange(3), got)

@@ -348,3 +348,24 @@ def test_pages_behind_4_gib(kind, nodes):
     at = np.arange(rows) % 2 == 1
     for got, x in ((k, K), (v, V)):
         assert np.array_equal(got.cpu().numpy()[at], x[:, np.arange(rows)[at] % 90].transpose(1, 0, 2).reshape(-1, 128).astype(np.float32))
+
+
+def scaled_by(x, power):
+    """x times 2^power, rounded once to f32 (subnormal values too)."""
+    return torch.from_numpy(np.ldexp(x.double().cpu().numpy(), power).astype(np.float32)).cuda()
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("power", [-149, -140, -134, -127, -120, -104, -60, 60, 100])
+@pytest.mark.parametrize("nodes", [3, 40])
+def test_queries_of_any_size(kind, power, nodes):
+    """Finite ones down to f32's smallest; the ends of rows lie inside tiles."""
+    for masks in (None, [np.eye(nodes, dtype=bool)]):
+        c = Call(kind, 1, 2, 64, 16, [41], [nodes], masks, seed=power % 97)
+        if power > 0:  # (keys of zero, so that scores stay in range)
+            c.pool[0].zero_() if kind not in TOP else bytes_of(c.pool[0]).zero_()
+        c.q = scaled_by(c.q, power)
+        assert torch.any(c.q != 0)
+        got = c.run()
+        assert np.isfinite(got).all()
+        c.check(got)
