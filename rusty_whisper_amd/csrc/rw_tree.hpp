@@ -9,7 +9,8 @@
 // products, as in rw_kv.hpp, whose operands, precision and treatment of sums this
 // follows; 8-bit pools differ:
 //   keys    as f16, which has all their values, times q in 2 f16 parts (22 bits and
-//           more of every value down to 2^-29 of its query's largest); the score times the key's scale
+//           more of every value down to 2^-29 of its query's largest); the score times the key's
+//           scale and, where q is small, what brings q back to its own size
 //   values  as bf16, which has them too, times p s (p: the weight, s: the value's
 //           scale) in 3 bf16 parts, all of its bits.  (In 2, 5e-6 of the results was off; in 2 f16
 //           parts, of the largest p s at 2^10 .. 2^15, as little as in 3, but a small weight
@@ -385,9 +386,14 @@ struct TreeSum {
 // at most, so that the factor (2^-120 times 0.13 and more) is no zero, which times an unseen
 // key's -inf would be NaN: values below 2^-105 then lie lower, where a subnormal one, a multiple of
 // 2^-149, still is the sum of its two parts, and a normal one, at 2^-6 at least, keeps 22 bits.
+//   A key's scale may be as large as f32 goes.  So the part of that factor that makes smaller, and 2^-4
+// more for the root of the head's size, is `low`, which the scale is multiplied by: a score that is in
+// range in the end then is before the factor.  (Where low times a scale is no normal number
+// and loses bits, the score is below 2^-93.)
 template <class M, class T>
-__device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf) {
+__device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf, float &low) {
   float c = PA_LOG2E / __builtin_sqrtf((float)M::HEAD);
+  low = 1.0f;
   float y[M::STEPS][M::VAL], top = 0.0f;
 #pragma unroll
   for (int s = 0; s < M::STEPS; ++s)
@@ -402,7 +408,9 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf)
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     e = top > 0.0f ? max(__builtin_amdgcn_frexp_expf(top) - 15, -120) : 0;
-    c = ldexpf(c, e);
+    const int before = M::SCALED ? min(e - 4, 0) : 0;
+    low = ldexpf(low, before);
+    c = ldexpf(c, e - before);
   }
 #pragma unroll
   for (int s = 0; s < M::STEPS; ++s) {
@@ -496,7 +504,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   QOp qf[PARTS][M::STEPS];
   const int mine = min(r, nq - 1), node = (u0 + mine) / a.group;
   const uint32_t *mask = a.mask ? a.mask + (int64_t)row_of(mine) * a.n_words : nullptr;
-  const float c = tree_q<M>(a.q + row_of(mine) * a.ldq + (int64_t)head_of(mine) * DH, r < nq, h, qf);
+  float low;
+  const float c = tree_q<M>(a.q + row_of(mine) * a.ldq + (int64_t)head_of(mine) * DH, r < nq, h, qf, low);
 
   for (float scale = 1.0f;; scale = PA_LOW) {
     TreeSum<M::SCALED, M::WIDE, ND> acc;
@@ -546,7 +555,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
         y[j] = s[M::SUMS - 1][j >> 2][j & 3];
 #pragma unroll
         for (int k = M::SUMS - 2; k >= 0; --k) y[j] = fmaf(y[j], 1.0f / M::MOVE, s[k][j >> 2][j & 3]);
-        if constexpr (M::SCALED) y[j] *= ksc[j >> 2][j & 3];
+        if constexpr (M::SCALED) y[j] *= low * ksc[j >> 2][j & 3];
       }
       uint32_t sees = ~0u;
       if (edge) {
@@ -709,7 +718,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
   const int w0 = 16 * QW * wv, wq = min(16 * QW, nq - w0), wn = wq <= 0 ? 0 : tree_end(a, sp, u0 + w0 + wq);
 
   typename S::QOp qf[QW][PARTS][S::STEPS];
-  float c[QW];
+  float c[QW], low[QW];
   const uint32_t *mask[QW];
   int node[QW];
 #pragma unroll
@@ -717,7 +726,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
     const int i = min(w0 + 16 * x + r, nq - 1);
     node[x] = (u0 + i) / a.group;
     mask[x] = a.mask ? a.mask + (int64_t)row_of(i) * a.n_words : nullptr;
-    c[x] = tree_q<S>(a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH, w0 + 16 * x + r < nq, h, qf[x]);
+    c[x] = tree_q<S>(a.q + row_of(i) * a.ldq + (int64_t)head_of(i) * DH, w0 + 16 * x + r < nq, h, qf[x], low[x]);
   }
 
   // What this thread brings of a tile: 16 bytes of K's rows and of V's.  Pages no shorter
@@ -892,7 +901,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
             for (int j = 0; j < 8; ++j) {
               y[j] = s[x][SUMS - 1][j >> 2][j & 3];
               if (SUMS == 2) y[j] = fmaf(y[j], 1.0f / S::MOVE, s[x][0][j >> 2][j & 3]);
-              if constexpr (S::SCALED) y[j] *= ksc[j >> 2][j & 3];
+              if constexpr (S::SCALED) y[j] *= low[x] * ksc[j >> 2][j & 3];
             }
             sees[x] = 0xFF;
             if (edge || bad_any) {

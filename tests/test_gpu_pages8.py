@@ -326,7 +326,7 @@ def test_a_captured_call_replayed_with_other_contents(kind):
 
 
 @pytest.mark.parametrize("kind", KINDS8)
-@pytest.mark.parametrize("q_power,k_power", [(-149, 0), (-140, 0), (-134, 0), (-120, 0), (-101, 0), (-40, 0)])
+@pytest.mark.parametrize("q_power,k_power", [(-149, 0), (-140, 0), (-134, 0), (-120, 0), (-101, 101), (-120, 120), (-40, 40), (100, -100)])
 @pytest.mark.parametrize("group", [1, 20])
 def test_queries_and_key_scales_of_any_size(kind, q_power, k_power, group):
     heads, dim, page, lens = 2, 64, 32, [200, 1, 77]

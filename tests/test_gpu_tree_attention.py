@@ -369,3 +369,17 @@ def test_queries_of_any_size(kind, power, nodes):
         got = c.run()
         assert np.isfinite(got).all()
         c.check(got)
+
+
+@pytest.mark.parametrize("kind", list(TOP))
+@pytest.mark.parametrize("power", [-116, -90, -40, 40, 90, 101, 112, 120])
+@pytest.mark.parametrize("nodes", [3, 40])
+def test_key_scales_of_any_size(kind, power, nodes):
+    """Keys of 2^power of the usual size and queries of 2^-power of theirs: the scores are the usual ones."""
+    for masks in (None, [np.eye(nodes, dtype=bool)]):
+        c = Call(kind, 1, 2, 64, 16, [41], [nodes], masks, seed=5)
+        c.pool[2] = scaled_by(c.pool[2], power)
+        c.q = scaled_by(c.q, -power)
+        got = c.run()
+        assert np.isfinite(got).all()
+        c.check(got)
