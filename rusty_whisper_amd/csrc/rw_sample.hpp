@@ -446,7 +446,8 @@ __global__ __launch_bounds__(SAMPLE_THREADS, 4) void k_sample(const typename E::
     }
     return;
   }
-  if (t <= 0.0f || top_k == 1) {  // the first of the order
+  // the first of the order: also where no weight has min_p, those of the largest logits (1) neither
+  if (t <= 0.0f || top_k == 1 || min_p > 1.0f) {
     int id = INT32_MAX;
     if (own == top)  // (few threads)
       row.template each_one<1>([&](float x, int i) {

@@ -217,3 +217,19 @@ def test_more_rows_than_a_launch_has_threads_for():
     assert tok[rows - 5] == 1
     tok[rows - 5] = 0
     assert not tok.any()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n", [2, 1000, 51866])
+def test_a_min_p_above_1_keeps_the_first_alone(dtype, n):
+    """Also where others equal it; of 1 it keeps those that do."""
+    logits = (torch.randn(4, n, device="cuda").clamp(max=0.5)).to(DTYPES[dtype])
+    logits[:, n // 2 :] = 0.5  # half of them are the largest
+    logits[3] = 0.5
+    first = (logits == 0.5).cpu().numpy().argmax(1).tolist()
+    for p in (1.0000001, 1.5, float("inf")):
+        for kw in (dict(), dict(top_p=0.9), dict(top_k=3), dict(t=0.3)):
+            tok, lp = draw(logits, 0.9375, min_p=p, **kw)
+            assert tok.tolist() == first and np.all(lp == 0), (p, kw)
+    u = np.array([0.123457, 0.5000031, 0.987653, 0.76543], np.float32)
+    check(logits, u, draw(logits, u, min_p=1.0), min_p=1.0)
