@@ -809,6 +809,11 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
       }
       return;
     }
+    // v behind the rows and in pages that are not there (anything): zeros.  At an edge, where a row that one
+    // query sees and another does not may hold infinities or NaN, these leave the products and are given to
+    // those who see them.  Another tile of which pages are not there keeps what the others hold, which all
+    // queries see (BIG: it has no others)
+    const bool take = BIG || edge;
     int special = vbad ? 2 : 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -821,7 +826,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t w = y[j] & kv8_first(have - 4 * j);
-          if (!Kv8<E>::FINITE) odd |= kv8_take_nan(w) << (4 * j);
+          if (!Kv8<E>::FINITE && take) odd |= kv8_take_nan(w) << (4 * j);
           y[j] = w;
         }
       } else {
@@ -829,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (j >= have) z[j] = (T)0.0f;
-          if (!__builtin_isfinite((float)z[j])) odd |= 1u << j, z[j] = (T)0.0f;
+          if (take && !__builtin_isfinite((float)z[j])) odd |= 1u << j, z[j] = (T)0.0f;
         }
         y = __builtin_bit_cast(u32x4, z);
       }

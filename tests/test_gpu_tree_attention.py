@@ -383,3 +383,37 @@ def test_key_scales_of_any_size(kind, power, nodes):
         got = c.run()
         assert np.isfinite(got).all()
         c.check(got)
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("nodes", [3, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_an_infinity_beside_a_page_that_is_not_there(kind, page, nodes, dim):
+    """It stays visible to those who see it, however many they are."""
+    past, row, value = 3 * page + 70, 5, 7
+    c = Call(kind, 1, 2, dim, page, [past], [nodes], None, seed=4)
+    whole = c.table[0].copy()
+    gone = np.zeros(past + nodes, bool)
+    gone[page : 2 * page] = True
+    c.table[0, 1] = c.n_pages
+    at = whole[0]
+    if kind == "i8":  # (no code for one: a scale)
+        c.pool[3][1, at, :, row] = float("nan")
+        odd = slice(None)
+    else:
+        if kind == "e4m3":
+            bytes_of(c.pool[1])[1, at, :, value, row] = 0x7F
+        else:
+            c.pool[1][1, at, :, value, row] = float("inf")
+        odd = value
+    got = c.run().reshape(nodes, 2, dim)
+    assert not np.isfinite(got[:, :, odd]).any()
+    if odd == value:
+        K, V = gather_any(c.pool, 1, whole[: -(-(past + nodes) // page)], past + nodes)
+        V[:, row, value] = 0
+        for j in range(nodes):
+            seen = (np.arange(past + nodes) <= past + j) & ~gone
+            want, tol = attend(c.q[j].double().cpu().numpy().reshape(2, -1), K[:, seen], V[:, seen])
+            rest = np.arange(dim) != value
+            assert np.all(np.abs(got[j] - want)[:, rest] <= tol[:, rest]), j
