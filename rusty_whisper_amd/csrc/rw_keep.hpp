@@ -74,7 +74,8 @@ __global__ __launch_bounds__(64) void k_tree_accept(const uint32_t *__restrict__
   __shared__ uint32_t st[ACCEPT], ss[ACCEPT];
   __shared__ int sp[ACCEPT];
   const int tree = blockIdx.x, lane = threadIdx.x;
-  const int s0 = starts[tree], n = s0 < 0 ? 0 : min(min(starts[tree + 1], rows) - s0, most);
+  // (an end below zero is taken as zero: its distance from s0 could pass 32 bits and come out positive)
+  const int s0 = starts[tree], n = s0 < 0 ? 0 : min(min(max(starts[tree + 1], 0), rows) - s0, most);
   const uint32_t *tok = tokens + s0, *smp = sampled + s0;
   const int32_t *par = parent + s0;
   if (n > 0 && n <= ACCEPT) {

@@ -96,7 +96,8 @@ struct TreeArgs {
 };
 
 // What tree i of a call is: its first row, its rows in this launch, the rows of
-// the sequence before it, the rows it may see, its row of the table.
+// the sequence before it, the rows it may see, its row of the table.  (An end below
+// zero is taken as zero: its distance from the first row could pass 32 bits and come out positive.)
 struct TreeSpan {
   int start, rows, past, n;
   const int32_t *table;
@@ -110,7 +111,7 @@ __device__ inline TreeSpan tree_span(const TreeArgs &a, int i) {
   int nodes = 0;
   if (a.starts) {
     s.start = a.starts[i];
-    nodes = s.start < 0 ? 0 : max(0, min(a.starts[i + 1], a.rows) - s.start);
+    nodes = s.start < 0 ? 0 : max(0, min(max(a.starts[i + 1], 0), a.rows) - s.start);
     s.rows = min(nodes, a.max_rows);
   } else {
     s.start = i, s.rows = 1;

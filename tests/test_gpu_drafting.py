@@ -263,3 +263,24 @@ def test_a_program(kind):
     p.book.release([seqs[2], seqs[0]])
     A.kv_copy_pages_dev(p.pages, *p.book.compact())
     p.step([child, seqs[1]])
+
+
+def test_trees_that_end_before_they_begin_or_behind_the_rows():
+    rng = np.random.default_rng(2)
+    n = 1500  # (past what is walked in LDS)
+    tokens, sampled = rng.integers(0, 2, n), rng.integers(0, 2, n)
+    parent = np.concatenate([np.array(p, np.int64) for p in trees(rng, [n])])
+    for starts, most in (([-1, 3, 2, 9], 5), ([1, -(2**31), 2, 9], 8), ([1, -(2**31) + 1, 0, 2000], 2000), ([2**31 - 1, -(2**31), 4, 900], 900),
+                         ([n - 3, -(2**31), n - 5, n + 7], 2000), ([n, 0, n, n + 1], 3)):
+        kept, count, nxt = accepted(tokens, parent, sampled, starts, most)
+        for i, (a, b) in enumerate(zip(starts, starts[1:])):
+            b = min(b, n, a + most)
+            path, follows = ([], 0xFFFFFFFF) if a < 0 or b <= a else accept(tokens[a:b], parent[a:b], sampled[a:b])
+            assert count[i] == len(path) and nxt[i] == follows, (starts, i)
+            assert kept[i].tolist() == path + [-1] * (most - len(path)), (starts, i)
+    # two trees without rows, one that the call's rows cut
+    tokens, sampled = np.array([1, 2, 2, 2, 2]), np.full(5, 2)
+    kept, count, nxt = accepted(tokens, np.zeros(5), sampled, [-1, 3, 2, 9], 5)
+    path, follows = accept(tokens[2:], np.zeros(3), sampled[2:])
+    assert count.tolist() == [0, 0, len(path)] and nxt.tolist() == [0xFFFFFFFF, 0xFFFFFFFF, follows]
+    assert kept.tolist() == [[-1] * 5, [-1] * 5, path + [-1] * (5 - len(path))]

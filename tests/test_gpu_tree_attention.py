@@ -417,3 +417,16 @@ def test_an_infinity_beside_a_page_that_is_not_there(kind, page, nodes, dim):
             want, tol = attend(c.q[j].double().cpu().numpy().reshape(2, -1), K[:, seen], V[:, seen])
             rest = np.arange(dim) != value
             assert np.all(np.abs(got[j] - want)[:, rest] <= tol[:, rest]), j
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "i8"])
+@pytest.mark.parametrize("nodes", [7, 40])
+def test_starts_at_the_ends_of_their_range(kind, nodes):
+    """Trees whose rows end before they begin, however far, have none."""
+    c = Call(kind, 2, 1, 64, 16, [20, 3, 40], [nodes] * 3, [np.ones((nodes, nodes), bool)] * 3, seed=6)
+    for a, b in ((1, -(2**31)), (1, -(2**31) + 1), (2, -(2**31)), (2**31 - 1, -(2**31)), (2**31 - 1, 0)):
+        c.starts = np.array([a, b, 3, 3 + nodes])
+        got = c.run()
+        first = 3 if b < 0 else b  # (rows b .. 2 are the second tree's)
+        assert np.all(got[:first] == 5) and np.all(got[3 + nodes :] == 5), (a, b)
+        assert np.isfinite(got).all() and not np.any(got[first : 3 + nodes] == 5), (a, b)
