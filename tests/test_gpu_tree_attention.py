@@ -430,3 +430,86 @@ def test_starts_at_the_ends_of_their_range(kind, nodes):
         first = 3 if b < 0 else b  # (rows b .. 2 are the second tree's)
         assert np.all(got[:first] == 5) and np.all(got[3 + nodes :] == 5), (a, b)
         assert np.isfinite(got).all() and not np.any(got[first : 3 + nodes] == 5), (a, b)
+
+
+# Up to 16 queries a key head: every type of pool straight from memory.
+SMALL = [(1, [13, 1, 0, 16, 5], [0, 17, 40, 121, 300]), (4, [4, 1, 3, 2], [70, 0, 255, 16]), (8, [2, 1], [33, 90])]
+
+
+def small_masks(rng, sizes):
+    """Ancestors; any bits, with a node that sees nothing and one that sees all; chains."""
+    some = [rng.random((n, n)) < 0.4 for n in sizes]
+    some[0][-1] = False
+    some[-1][0] = True
+    return [ancestors(p) if n else np.zeros((0, 0), bool) for n, p in zip(sizes, trees(rng, sizes))], some, None
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("group,sizes,past", SMALL)
+def test_few_queries_of_trees(kind, dim, page, group, sizes, past):
+    for masks in small_masks(np.random.default_rng(dim + page), sizes):
+        c = Call(kind, 2, group, dim, page, past, sizes, masks, seed=dim + page, gap=2)
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("dim,page", [(32, 256), (64, 16), (96, 16), (128, 128)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_few_queries_of_which_not_all_see_an_odd_row(kind, dim, page, what):
+    rng = np.random.default_rng(3)
+    sizes, past = [13, 16], [21, 60]
+    masks = [ancestors(p) for p in trees(rng, sizes)]
+    c = Call(kind, 2, 1, dim, page, past, sizes, masks, seed=3)
+    want = c.run()
+    bad = [int(np.argmin(np.abs(m.sum(0) - m.shape[0] / 3))) for m in masks]  # a third of them see it
+    for i, b in enumerate(bad):
+        assert 0 < masks[i][:, b].sum() < sizes[i]
+        spoil(c, i, b, what)
+    got = c.run()
+    for i, b in enumerate(bad):
+        for j in range(sizes[i]):
+            r = c.starts[i] + j
+            if masks[i][j][b]:
+                assert not np.isfinite(got[r]).any(), (i, j)
+            else:
+                assert np.array_equal(got[r], want[r]), (i, j)
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("page,dim", [(16, 32), (16, 128), (32, 96), (128, 64)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_few_queries_with_pages_that_are_not_there(kind, page, dim, masked):
+    rng = np.random.default_rng(page)
+    past, nodes = [300, 2 * page + 5], [4, 3]
+    masks = [rng.random((n, n)) < 0.6 for n in nodes] if masked else None
+    c = Call(kind, 1, 4, dim, page, past, nodes, masks, seed=11)
+    whole = c.table.copy()
+    gone = [np.zeros(p + m, bool) for p, m in zip(past, nodes)]
+    for i in range(2):
+        for at in (1, (past[i] + nodes[i] - 1) // page):
+            gone[i][at * page : (at + 1) * page] = True
+            c.table[c.seq[i]][at] = c.n_pages if at == 1 else -1
+    got = c.run()
+    for i in range(2):
+        total = past[i] + nodes[i]
+        K, V = gather_any(c.pool, 1, whole[c.seq[i]][: -(-total // page)], total)
+        for j in range(nodes[i]):
+            r = c.starts[i] + j
+            seen = np.arange(total) <= past[i] + j
+            if masked:
+                seen[past[i] :] = masks[i][j]
+            seen &= ~gone[i]
+            y, tol = attend(c.q[r].double().cpu().numpy().reshape(4, -1), K[:, seen], V[:, seen])
+            assert np.all(np.abs(got[r].reshape(4, -1) - y) <= tol), (i, j)
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("dim,page", [(32, 16), (64, 256), (96, 64), (128, 16)])
+@pytest.mark.parametrize("group,sizes,past", [(1, [13], [9001]), (4, [4, 2, 4], [9000, 4007, 20]), (16, [1, 1], [5000, 700])])
+def test_few_queries_of_trees_over_chunks_of_keys(kind, dim, page, group, sizes, past):
+    for masks in small_masks(np.random.default_rng(dim), sizes):
+        c = Call(kind, 1, group, dim, page, past, sizes, masks, seed=dim)
+        assert A.tree_attention_workspace_size(A.KvPages(*c.pool), c.rows, group, len(sizes), c.max_rows, c.max_len) > 0
+        c.check(c.run())
