@@ -821,11 +821,13 @@ def tree_accept_dev(tokens, parent, sampled, rows: int, starts, max_rows: int, k
     arrays of 32-bit integers; as many trees as n_kept has entries."""
     d = starts.get_device()
     n = n_kept.numel()
+    paths = _dense(kept, _I32, n * max_rows, "kept", d)
+    if hasattr(kept, "dim") and kept.dim() == 2 and kept.shape[1] != max_rows:
+        raise ValueError(f"kept must be [n_trees, max_rows], not rows of {kept.shape[1]} for trees of up to {max_rows}")
     check(lib().rw_rocm_tree_accept_dev(
         _dense(tokens, _I32, rows, "tokens", d, _U32), _dense(parent, _I32, rows, "parent", d),
-        _dense(sampled, _I32, rows, "sampled", d, _U32), rows, _dense(starts, _I32, n + 1, "starts", d), n, max_rows,
-        _dense(kept, _I32, n * max_rows, "kept", d), _dense(n_kept, _I32, n, "n_kept", d),
-        _dense(next_tokens, _I32, n, "next_tokens", d, _U32), stream))
+        _dense(sampled, _I32, rows, "sampled", d, _U32), rows, _dense(starts, _I32, n + 1, "starts", d), n, max_rows, paths,
+        _dense(n_kept, _I32, n, "n_kept", d), _dense(next_tokens, _I32, n, "next_tokens", d, _U32), stream))
 
 
 def kv_keep_rows_dev(pages: KvPages, table, past, kept, n_kept, seq=None, stream: int | None = None) -> None:

@@ -234,3 +234,12 @@ def test_tensors_that_end_too_early_are_refused(call, bad, needle):
 def test_tensors_that_just_suffice_reach_the_library(call):
     with pytest.raises(A.RwError):  # no device here, or tensors that are not on it
         call()
+
+
+def test_accepted_paths_of_another_width_are_refused():
+    """Rows of 7 nodes would be written 5 apart: the next call reads them 7 apart."""
+    for kept in (i32(2, 7), i32(4, 4)):
+        with pytest.raises(ValueError, match="kept must be"):
+            call_accept(kept=kept)
+    with pytest.raises(A.RwError):  # no device here, or tensors that are not on it
+        call_accept(kept=i32(10))
