@@ -527,7 +527,8 @@ int rw_rocm_paged_attention_dev(const rw_kv_pages *pages, size_t layer, const fl
  * rw_rocm_paged_attention_dev (heads, layout, precision, f16 pools' q as 8-bit ones'; a
  * row that sees nothing gets zeros), and a row of the pool that a node does not see may hold
  * anything, infinities and NaN too, also where other nodes see it.  Rows of q
- * and out in no tree are left as they were.  max_rows: the most nodes of a
+ * and out in no tree are left as they were.  A tree that begins below row 0 or ends before it begins
+ * has no rows, one that ends behind the call's is cut.  max_rows: the most nodes of a
  * tree (those beyond are left out); max_len: the largest past + nodes; rows counts q's.
  * starts, past and mask are on the device, read when the work runs.  n_trees x
  * max_rows x n_head <= 2^23. */
@@ -641,10 +642,9 @@ int rw_rocm_token_logprobs_dev(int dtype, const void *logits, size_t ld, size_t 
  * switches one off (temperature: 1).
  * Weights are formed in 64 bits and summed exactly, in steps of 2^-42 of the
  * largest: the same token at every call.  A row holding NaN or +inf, or only
- * -inf, and one whose settings are NaN or whose temperature is infinite gets
- * token 0xFFFFFFFF and NaN.  n_vocab <= 2^20, rows <= 2^23.  The workspace (NULL: one kept per
- * (device, stream), not for a stream that is being captured) holds
- * rw_rocm_sample_tokens_workspace_size bytes, 16-byte aligned. */
+ * -inf, and one whose settings are NaN or whose temperature is +infinity gets
+ * token 0xFFFFFFFF and NaN.  n_vocab <= 2^20, rows <= 2^23.  The call needs no workspace:
+ * rw_rocm_sample_tokens_workspace_size is 0 for every size, and NULL is taken in captured streams too. */
 size_t rw_rocm_sample_tokens_workspace_size(size_t rows, size_t n_vocab);
 int rw_rocm_sample_tokens_dev(int dtype, const void *logits, size_t ld, size_t rows, size_t n_vocab, const float *u,
                               const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,

@@ -18,15 +18,17 @@ using namespace rw;
 namespace rw {
 
 // How a launch cuts its trees' queries and keys, as PagedPlan does for single rows.
-// Queries: 16 per workgroup where no more are there and for f32 (whose products take 16
-// times bf16's time each, so that sharing loads gains nothing).  64 with keys and values through LDS
-// otherwise; f16 pools 128 from 65 on, since each value is there in two parts and a part
-// read from LDS then has two products: 4 chunks of 512 rows behind 4100, 8 heads of 4 x 128: 487 us by
-// 128, 626 by 64; bf16 and 8-bit pools 524 and 530 by 128, 512 and 528 by 64.
+// Queries: 16 per workgroup where no more are there, and for f32, for which k_tree_shared has no
+// form.  64 with keys and values through LDS otherwise; f16 pools 128 from 65 on, since each value is
+// there in two parts and a part read from LDS then has two products: 4 chunks of 512 rows behind 4100, 8
+// heads of 4 x 128: 466 us by 128, 538 by 64; bf16 557 and 439, int8 636 and 471, e4m3 514 and 447.  (f32 by 16:
+// 1980 us, where the products alone take 955 at a large f32 product's rate; by more is not built.)
 // Keys: in one chunk up to 256 KB a head.  One tree is cut as far as the join goes, a batch
-// into chunks of 192 KB, as many as fill the device's 512 workgroups some four times over:
-// 24 trees of up to 48 rows of 8 heads of 4 x 128, up to 6048 keys, i8: 600 in all 258 us, 1200 191, 2048 188, 4096 186; 61
-// single rows of up to 8191 keys, e4m3: chunks of 96 KB 126 us, 192 KB 110, 384 KB 111.
+// into chunks of 192 KB, but no more workgroups in all than fill the device's 512 places four times over,
+// the cap that acts in large batches.  By caps: 61 single rows of up to 8191 keys, 8 heads of 4 x 128, e4m3: 600
+// 121 us, 1024 (2 chunks) 112, 2048 (4, of 528 KB) 106, 4096 (8) 112, 8192 (11) 116; 24 trees of up to 48 rows, up to
+// 6048 keys, int8: 1024 (1) 272, 1200 (2) 178, 2048 (3) 188, 4096 (7) 172, 8192 (9) 176.  By sizes, where the cap leaves
+// the choice: 8 such rows by 96 KB 38 us, 192 30, 384 29; 4 such trees 65, 68, 78.
 struct TreePlan {
   int nq;         // queries per workgroup: 16 (k_tree_attn), 64 or 128 (k_tree_shared)
   size_t qtiles;  // workgroups per tree, key head and chunk

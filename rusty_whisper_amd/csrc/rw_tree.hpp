@@ -430,9 +430,10 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf,
 // chunk of keys).  A wavefront takes every PA_WAVES-th tile of keys, straight from memory, for
 // all of the workgroup's queries.
 // Bound, for long caches, by reading them: 61 rows of up to 8191 keys, 8 heads of 4 x 128, e4m3
-// (390 MB) 105 us, 3.7 TB/s.  A wavefront has some 8 tiles to read, so that the first loads'
-// way, the tile's chain (product, softmax, product) and the join are a quarter of it.  For short
-// ones by that chain once: 6 heads of 64, 28 keys 6.3 us (int8), 114 keys 7.9 us (f32).
+// (390 MB) 99 to 105 us, 3.7 to 3.9 TB/s.  A wavefront has some 8 tiles of 64 keys to read, so that the first loads'
+// way, the tile's chain (product, softmax, product) and the join are a quarter of it.  (8-bit heads
+// of 128 need all registers and keep 10, e4m3, or 4, int8, of a lane's in memory.)  For short
+// ones by that chain once: 6 heads of 64, 28 keys 6.4 us (int8), 114 keys 7.8 us (f32).
 template <class E, int DH>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   using M = TreeTile<E, DH>;
@@ -636,11 +637,14 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
 //
 // Bound by the matrix instructions and what must be done between them: with q and p in
 // parts a bf16 pool takes 6 products of 16 x 16 x 32 where one of bf16 would take 2 (f16:
-// 2 + 5, 8 bits: 2 + 3).  4 chunks of 512 rows behind 4100, 8 heads of 4 x 128, bf16: 513 us, 285
-// TFLOP/s of the formula's and 855 of the products done; the matrix units are busy 40 % of the
+// 2 + 5, 8 bits: 2 + 3).  4 chunks of 512 rows behind 4100, 8 heads of 4 x 128, bf16: 439 us in a row of
+// calls, 333 TFLOP/s of the formula's and 1000 of the products done; the matrix units are busy 40 % of the
 // time, with two wavefronts to a SIMD of which each has some 250 other instructions to 48
 // products.  (Straight from memory: 2.2 times that.  With the next tile's scores formed before this one's
-// softmax: 561 us.  With 128 queries: 524.)  24 trees of up to 48 rows, int8: 184 us.
+// softmax: a tenth more.  With 128 queries: 557.)  The same chunks over int8: 471 us; 173 M vector instructions, where
+// bf16 has 108 M, for the conversions and scales, 280 us of issue beside 146 of products.
+// 24 trees of up to 48 rows, int8: 186 us, with half of the wavefronts' places empty, as the lengths are
+// unlike: products are 29 us of it, vector instructions 61.
 
 // units (16 bytes, 8 values) of a tile row of UNITS: where unit `col` of row `row` lies
 template <int UNITS>
@@ -1042,7 +1046,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeArgs a, int nsplit, int n
 }
 
 // The same for up to JOIN_FEW chunks: a wavefront a query, a lane a chunk's weight.
-// (24 trees of 48 rows, 32 heads of 128, 3 chunks: 11.6 us, by a workgroup a query 30.1; 61 rows, 8 chunks: 5.6 and 5.5)
+// (24 trees of 48 rows, 32 heads of 128, 3 chunks: 11.6 us, by a workgroup a query 29.9; 61 rows, 4 chunks: 5.3 and 5.4)
 constexpr int JOIN_FEW = 64;
 template <int DH>
 __global__ __launch_bounds__(256) void k_tree_join_few(TreeArgs a, int nsplit, int nq, int queries) {

@@ -233,3 +233,24 @@ def test_a_min_p_above_1_keeps_the_first_alone(dtype, n):
             assert tok.tolist() == first and np.all(lp == 0), (p, kw)
     u = np.array([0.123457, 0.5000031, 0.987653, 0.76543], np.float32)
     check(logits, u, draw(logits, u, min_p=1.0), min_p=1.0)
+
+
+def test_a_call_needs_no_workspace():
+    """None at any size, so a captured call takes none either."""
+    assert all(A.sample_tokens_workspace_size(r, n) == 0 for r in (1, 61, 2**23) for n in (1, 51866, 2**20))
+    logits, u = torch.randn(3, 5003, device="cuda"), torch.rand(3, device="cuda")
+    tok, lp = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(3, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        A.sample_tokens_dev(logits, 3, 5003, u, tok, logprobs=lp, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        logits.normal_(std=2.0), u.uniform_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(logits, u.cpu().numpy(), (tok.cpu().numpy().view(np.uint32), lp.cpu().numpy()))
+
+
+def test_a_temperature_of_minus_infinity_takes_the_first():
+    x = torch.randn(2, 300, device="cuda")
+    tok, lp = draw(x, 0.9, t=np.array([-np.inf, np.inf], np.float32))
+    assert tok[0] == int(x[0].argmax()) and lp[0] == 0 and tok[1] == NONE and np.isnan(lp[1])
