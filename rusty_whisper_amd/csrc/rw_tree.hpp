@@ -12,7 +12,8 @@
 //           more of every value down to 2^-29 of its query's largest); the score times the key's
 //           scale and, where q is small, what brings q back to its own size
 //   values  as bf16, which has them too, times p s (p: the weight, s: the value's
-//           scale) in 3 bf16 parts, all of its bits.  (In 2, 5e-6 of the results was off; in 2 f16
+//           scale) in 3 bf16 parts, all of its bits down to 2^-109; so p is 2^40 times what it is
+//           elsewhere, and scales may be any number that f32 has.  (In 2, 5e-6 of the results was off; in 2 f16
 //           parts, of the largest p s at 2^10 .. 2^15, as little as in 3, but a small weight
 //           lost bits where the value of a large one is zero, and int8 has many zeros.)
 // f16 pools: q in those 2 parts, not 3; of p's 3 parts against v's 2 the product of the
@@ -329,7 +330,14 @@ template <int DH>
 struct TreeTile<E4M3, DH> : TreeTile8<E4M3, DH> {};
 
 // A query's running softmax (lane 16 h + r: query r) and its tile's output (lane
-// 16 h + r: queries 4 h .., values 16 i + r).
+// 16 h + r: queries 4 h .., values 16 i + r).  SCALED: weights, and so their sum and the
+// outputs, are 2^TREE_UP times as large (see above).  The maximum is a whole number then, so that
+// taking TREE_UP from it costs no bits; where a mean is not finite, the second turn takes the weights at PA_LOW.
+constexpr int TREE_UP = 40;
+template <bool SCALED>
+constexpr float tree_low() {
+  return SCALED ? PA_LOW * 0x1p-40f : PA_LOW;  // (2^-TREE_UP)
+}
 template <bool SCALED, bool WIDE, int ND>
 struct TreeSum {
   f4 o[ND];
@@ -350,7 +358,7 @@ struct TreeSum {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       // (each query's own: what others see changes no bit of it)
-      const float next = top > m + PA_SLACK ? top : m, f = pa_weight(m, next);
+      const float next = top > m + PA_SLACK ? (SCALED ? __builtin_floorf(top) : top) : m, f = pa_weight(m, next);
       m = next;
       sum *= f;
       f4 fr;
@@ -359,7 +367,7 @@ struct TreeSum {
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] *= fr;
     }
-    const float base = m == -__builtin_huge_valf() ? 0.0f : m;
+    const float base = m == -__builtin_huge_valf() ? 0.0f : SCALED ? m - TREE_UP : m;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], c, -base));
@@ -509,7 +517,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   float low;
   const float c = tree_q<M>(a.q + row_of(mine) * a.ldq + (int64_t)head_of(mine) * DH, r < nq, h, qf, low);
 
-  for (float scale = 1.0f;; scale = PA_LOW) {
+  for (float scale = 1.0f;; scale = tree_low<M::SCALED>()) {
     TreeSum<M::SCALED, M::WIDE, ND> acc;
     acc.clear();
 
@@ -849,7 +857,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
     if (special) atomicOr(&flags[t % 3], special);
   };
 
-  for (float scale = 1.0f;; scale = PA_LOW) {
+  for (float scale = 1.0f;; scale = tree_low<S::SCALED>()) {
     TreeSum<S::SCALED, S::WIDE, ND> acc[QW];
 #pragma unroll
     for (int x = 0; x < QW; ++x) acc[x].clear();

@@ -339,3 +339,21 @@ def test_queries_and_key_scales_of_any_size(kind, q_power, k_power, group):
     got = attention(pool, 0, q, heads * group, table, lens, 200)
     assert np.isfinite(got).all()
     check_attention(pool, kind, 0, q, heads * group, table, lens, np.arange(3), got)
+
+
+@pytest.mark.parametrize("kind", KINDS8)
+@pytest.mark.parametrize("power", [-140, -126, -118, -112, -100, -60, 60, 80, 100, 112])
+@pytest.mark.parametrize("group,length", [(1, 200), (20, 200), (2, 9000)])
+def test_value_scales_of_any_size(kind, power, group, length):
+    """Of one chunk and of several; subnormal results are multiples of 2^-149 (a mean of every wavefront and chunk, its
+    share of the whole, the whole: at most 6 half steps, and 2 for every chunk)."""
+    dim, page = 128, 32
+    table = tables([length], page, 290, 1)
+    pool = any_pool(kind, 1, 290, 1, page, dim, 2)
+    pool[3] = torch.from_numpy(np.ldexp(pool[3].double().cpu().numpy(), power).astype(np.float32)).cuda()
+    q = torch.randn(1, group * dim, device="cuda", generator=torch.Generator("cuda").manual_seed(3)) * 2
+    got = attention(pool, 0, q, group, table, [length], length)
+    K, V = gather_any(pool, 0, table[0], length)
+    want, tol = attend(q[0].double().cpu().numpy().reshape(group, -1), K, V)
+    err = np.abs(got[0].reshape(group, -1) - want)
+    assert np.all(err <= tol + (6 + 2 * 64) * 2.0**-150), (float(err.max()), float(np.abs(want).max()))

@@ -513,3 +513,27 @@ def test_few_queries_of_trees_over_chunks_of_keys(kind, dim, page, group, sizes,
         c = Call(kind, 1, group, dim, page, past, sizes, masks, seed=dim)
         assert A.tree_attention_workspace_size(A.KvPages(*c.pool), c.rows, group, len(sizes), c.max_rows, c.max_len) > 0
         c.check(c.run())
+
+
+@pytest.mark.parametrize("kind", list(POOLS))
+@pytest.mark.parametrize("power", [-140, -126, -118, -112, -100, -60, 60, 80, 100, 112])
+@pytest.mark.parametrize("nodes", [3, 40])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 128)])
+def test_values_of_any_size(kind, power, nodes, dim, page):
+    """Down to where results are subnormal: there they are rounded to multiples of 2^-149, a wavefront's mean
+    once, its share of the whole once (up to four of them), the whole once: 6 half steps.  Sums of weights and values
+    that have no scale are subnormal themselves: one half step more for each of n products and, for tiles of 16 keys at
+    least, for a rescaling of the sum (weights' sum is 1 at least, so dividing makes none of these larger)."""
+    if kind == "f16":
+        power = max(-14, min(power, 12))
+    c = Call(kind, 1, 2, dim, page, [141], [nodes], None, seed=8)
+    i = 3 if kind in TOP else 1
+    c.pool[i] = scaled_by(c.pool[i], power).to(c.pool[i].dtype)
+    got = c.run()
+    K, V = gather_any(c.pool, 1, c.table[0], 141 + nodes)
+    for j in range(nodes):
+        n = 141 + j + 1
+        want, tol = attend(c.q[j].double().cpu().numpy().reshape(2, -1), K[:, :n], V[:, :n])
+        err = np.abs(got[j].reshape(2, -1) - want)
+        steps = 6 if kind in TOP else 6 + n + n / 16
+        assert np.all(err <= tol + steps * 2.0**-150), (j, float(err.max()), float(np.abs(want).max()))
