@@ -332,11 +332,13 @@ struct TreeTile<E4M3, DH> : TreeTile8<E4M3, DH> {};
 // A query's running softmax (lane 16 h + r: query r) and its tile's output (lane
 // 16 h + r: queries 4 h .., values 16 i + r).  SCALED: weights, and so their sum and the
 // outputs, are 2^TREE_UP times as large (see above).  The maximum is a whole number then, so that
-// taking TREE_UP from it costs no bits; where a mean is not finite, the second turn takes the weights at PA_LOW.
-constexpr int TREE_UP = 40;
+// taking TREE_UP from it costs no bits.  Means that are not finite come from a second turn with
+// the weights' own size (one row's scale of 2^100 may pass the range where its values are zeros and others' are not),
+// those that then are not from a third at PA_LOW; without scales, these are the two turns.
+constexpr int TREE_UP = 40;  // PA_LOW undoes it
 template <bool SCALED>
-constexpr float tree_low() {
-  return SCALED ? PA_LOW * 0x1p-40f : PA_LOW;  // (2^-TREE_UP)
+constexpr float tree_last() {
+  return SCALED ? PA_LOW * PA_LOW : PA_LOW;
 }
 template <bool SCALED, bool WIDE, int ND>
 struct TreeSum {
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   float low;
   const float c = tree_q<M>(a.q + row_of(mine) * a.ldq + (int64_t)head_of(mine) * DH, r < nq, h, qf, low);
 
-  for (float scale = 1.0f;; scale = tree_low<M::SCALED>()) {
+  for (float scale = 1.0f;; scale *= PA_LOW) {
     TreeSum<M::SCALED, M::WIDE, ND> acc;
     acc.clear();
 
@@ -600,7 +602,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
         over |= qr < nq && !__builtin_isfinite(y);
       }
     }
-    if (!M::WIDE || !first || !__builtin_amdgcn_ballot_w64(over)) break;
+    if (!M::WIDE || scale == tree_last<M::SCALED>() || !__builtin_amdgcn_ballot_w64(over)) break;
     t = t0;
     begin();
   }
@@ -857,7 +859,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
     if (special) atomicOr(&flags[t % 3], special);
   };
 
-  for (float scale = 1.0f;; scale = tree_low<S::SCALED>()) {
+  for (float scale = 1.0f;; scale *= PA_LOW) {
     TreeSum<S::SCALED, S::WIDE, ND> acc[QW];
 #pragma unroll
     for (int x = 0; x < QW; ++x) acc[x].clear();
@@ -997,7 +999,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
         }
       }
     }
-    if (!S::WIDE || again || !__syncthreads_or(over)) break;
+    if (!S::WIDE || scale == tree_last<S::SCALED>() || !__syncthreads_or(over)) break;
   }
 }
 

@@ -537,3 +537,23 @@ def test_values_of_any_size(kind, power, nodes, dim, page):
         err = np.abs(got[j].reshape(2, -1) - want)
         steps = 6 if kind in TOP else 6 + n + n / 16
         assert np.all(err <= tol + steps * 2.0**-150), (j, float(err.max()), float(np.abs(want).max()))
+
+
+@pytest.mark.parametrize("kind", list(TOP))
+@pytest.mark.parametrize("large,small", [(100, 0), (100, -80), (75, -90), (40, -90), (112, -60)])
+@pytest.mark.parametrize("nodes", [3, 40])
+def test_value_scales_of_unlike_size(kind, large, small, nodes):
+    """Where the rows of large scales hold zeros, the others' values count: every weight's share of them is
+    off by 2^-133 of 2^0, as those with a scale of 2^100 leave it (bf16's last place), which is in the bound's own n + 8 half steps."""
+    c = Call(kind, 1, 2, 64, 16, [141], [nodes], None, seed=8)
+    n = 141 + nodes
+    rows = np.arange(n)
+    at, slot = c.table[0][rows // 16], rows % 16
+    power = np.where(rows % 5 == 0, large, small)
+    c.pool[3][1, at, 0, slot] = scaled_by(torch.ones(n, device="cuda"), power) * c.pool[3][1, at, 0, slot]
+    big = rows % 5 == 0
+    for r in rows[big]:
+        bytes_of(c.pool[1])[1, at[r], 0, :32, slot[r]] = 0
+    got = c.run()
+    assert np.isfinite(got).all()
+    c.check(got)
