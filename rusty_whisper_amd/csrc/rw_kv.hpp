@@ -289,6 +289,16 @@ __device__ inline void pa_add(const float (&p)[PaTile<E>::PER], const typename P
 // a mean of finite values, rounded past f32's largest, is that
 __device__ inline float pa_largest(float x) { return __builtin_copysignf(__FLT_MAX__, x); }
 
+// bf16 has nothing below 2^-133: of a query whose largest value (`top`: this lane's) is below
+// 2^-80, the third part of smaller ones, and in the end the second, would be lost, while its keys may be as
+// large.  The exponent that it is divided by: -60 for such a query, whose scores stay below 2^115
+__device__ inline int pa_small(float top) {
+  if (!__builtin_amdgcn_ballot_w64(top < 0x1p-80f)) return 0;
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  return top < 0x1p-80f ? -60 : 0;
+}
+
 // exp2(x) for x <= 0 or -inf against a maximum that may be -inf itself
 __device__ inline float pa_weight(float m, float top) {
   return m == -__builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
@@ -383,7 +393,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
   if (t < end) now = where(t), load_k(t, now);
 
   // q, in the scores' operand order; f16: each query's values scaled by a
-  // power of two so that the largest lies in [2^14, 2^15), undone in `c`
+  // power of two so that the largest lies in [2^14, 2^15), undone in `c`; bf16: queries
+  // that lie below pa_small(), by 2^60
   Op qf[PARTS][NC];
   float c = PA_LOG2E / __builtin_sqrtf((float)DH);
   {
@@ -404,10 +415,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_paged_attn(
       e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
       c = ldexpf(c, e);
     }
+    if (std::is_same_v<E, BF16>) e = pa_small(top), c = ldexpf(c, e);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       Op o[PARTS];
-      if (std::is_same_v<E, F16>)
+      if (!std::is_same_v<E, F32>)
 #pragma unroll
         for (int j = 0; j < PER; ++j) x[i][j] = ldexpf(x[i][j], -e);
       pa_parts<E>(x[i], o);

@@ -422,11 +422,13 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf,
     const int before = M::SCALED ? min(e - 4, 0) : 0;
     low = ldexpf(low, before);
     c = ldexpf(c, e - before);
+  } else if (M::PARTS > 1) {
+    e = pa_small(top), c = ldexpf(c, e);
   }
 #pragma unroll
   for (int s = 0; s < M::STEPS; ++s) {
     typename M::QOp o[M::PARTS];
-    if (M::MOVE != 1.0f)
+    if (M::PARTS > 1)
 #pragma unroll
       for (int j = 0; j < M::VAL; ++j) y[s][j] = ldexpf(y[s][j], -e);
     M::q_parts(y[s], o);

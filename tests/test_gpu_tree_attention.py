@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from _draft import POOLS, TOP, ancestors, any_pool, bytes_of, gather_any, trees, words
-from _paged import attend, i32, tables
+from _paged import attend, i32, norm_tol, tables
 from rusty_whisper_amd import _abi as A
 
 pytestmark = pytest.mark.gpu
@@ -557,3 +557,27 @@ def test_value_scales_of_unlike_size(kind, large, small, nodes):
     got = c.run()
     assert np.isfinite(got).all()
     c.check(got)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("power", [-116, -60, 60, 79, 82, 100, 112, 120, 124])
+@pytest.mark.parametrize("nodes", [0, 3, 40])
+def test_keys_of_any_size(kind, power, nodes):
+    """Keys of 2^power of the usual size and queries of 2^-power of theirs: the scores, and errors, are the usual ones.
+    (nodes 0: single rows)"""
+    c = Call(kind, 1, 2, 64, 32, [141], [max(nodes, 3)], None, seed=5)
+    c.pool[0] = scaled_by(c.pool[0], power).to(POOLS[kind])
+    c.q = scaled_by(c.q, -power)
+    if nodes:
+        got = c.run()
+    else:
+        out = torch.empty_like(c.q)
+        A.paged_attention_dev(A.KvPages(*c.pool), 1, c.q, 3, 2, i32(c.table), i32([142, 143, 144]), 144, out, seq=i32([0, 0, 0]))
+        torch.cuda.synchronize()
+        got = out.double().cpu().numpy()
+    c.check(got)
+    # far below the bound, which takes all roundings to fall one way
+    K, V = gather_any(c.pool, 1, c.table[0], 144)
+    want = attend(c.q[0].double().cpu().numpy().reshape(2, -1), K[:, :142], V[:, :142])[0]
+    sigma = float(np.std(c.q[0].double().cpu().numpy()) * np.std(K))
+    assert np.linalg.norm(got[0].reshape(2, -1) - want) <= norm_tol(sigma, 64, 142) * np.linalg.norm(want)
