@@ -12,8 +12,8 @@
 //           more of every value down to 2^-29 of its query's largest); the score times the key's
 //           scale and, where q is small, what brings q back to its own size
 //   values  as bf16, which has them too, times p s (p: the weight, s: the value's
-//           scale) in 3 bf16 parts, all of its bits down to 2^-109; so p is 2^40 times what it is
-//           elsewhere, and scales may be any number that f32 has.  (In 2, 5e-6 of the results was off; in 2 f16
+//           scale) in 3 bf16 parts, all of its bits down to 2^-109; so s enters at 2^40 times its
+//           size, and may be any number that f32 has.  (In 2, 5e-6 of the results was off; in 2 f16
 //           parts, of the largest p s at 2^10 .. 2^15, as little as in 3, but a small weight
 //           lost bits where the value of a large one is zero, and int8 has many zeros.)
 // f16 pools: q in those 2 parts, not 3; of p's 3 parts against v's 2 the product of the
@@ -330,15 +330,20 @@ template <int DH>
 struct TreeTile<E4M3, DH> : TreeTile8<E4M3, DH> {};
 
 // A query's running softmax (lane 16 h + r: query r) and its tile's output (lane
-// 16 h + r: queries 4 h .., values 16 i + r).  SCALED: weights, and so their sum and the
-// outputs, are 2^TREE_UP times as large (see above).  The maximum is a whole number then, so that
-// taking TREE_UP from it costs no bits.  Means that are not finite come from a second turn with
-// the weights' own size (one row's scale of 2^100 may pass the range where its values are zeros and others' are not),
-// those that then are not from a third at PA_LOW; without scales, these are the two turns.
-constexpr int TREE_UP = 40;  // PA_LOW undoes it
+// 16 h + r: queries 4 h .., values 16 i + r).  Turns over the keys: the weights at
+// their own size; where means are not finite, at PA_LOW.  SCALED: before these, with the values' scales, and so
+// the outputs, 2^40 times as large (see above).  (One row's scale of 2^100 passes the range then, also where its
+// values are zeros and others' are not, which at PA_LOW would lose bits.  2^40 in the exponential's argument would
+// cost no product, but the argument's own bits: 4.1e-7 off in place of 2.3e-7.)
+struct TreeTurn {
+  float scale, up;  // of weights; of values' scales
+  bool first;
+};
+constexpr float TREE_UP = 0x1p40f;
 template <bool SCALED>
-constexpr float tree_last() {
-  return SCALED ? PA_LOW * PA_LOW : PA_LOW;
+__device__ inline TreeTurn tree_turn(int i) {
+  if (SCALED) return TreeTurn{i < 2 ? 1.0f : PA_LOW, i == 0 ? TREE_UP : 1.0f, i == 0};
+  return TreeTurn{i == 0 ? 1.0f : PA_LOW, 1.0f, i == 0};
 }
 template <bool SCALED, bool WIDE, int ND>
 struct TreeSum {
@@ -360,7 +365,7 @@ struct TreeSum {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       // (each query's own: what others see changes no bit of it)
-      const float next = top > m + PA_SLACK ? (SCALED ? __builtin_floorf(top) : top) : m, f = pa_weight(m, next);
+      const float next = top > m + PA_SLACK ? top : m, f = pa_weight(m, next);
       m = next;
       sum *= f;
       f4 fr;
@@ -369,7 +374,7 @@ struct TreeSum {
 #pragma unroll
       for (int i = 0; i < ND; ++i) o[i] *= fr;
     }
-    const float base = m == -__builtin_huge_valf() ? 0.0f : SCALED ? m - TREE_UP : m;
+    const float base = m == -__builtin_huge_valf() ? 0.0f : m;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], c, -base));
@@ -385,10 +390,10 @@ struct TreeSum {
       if (seen[e] > 0.0f) o[i][e] = __builtin_nanf("");
   }
   // what makes of a query's o its mean (0: it saw nothing); sum is then the query's
-  __device__ float mean() {
+  __device__ float mean(float up) {
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    return sum == 0.0f ? 0.0f : 1.0f / sum;
+    return sum == 0.0f ? 0.0f : 1.0f / (sum * up);
   }
 };
 
@@ -444,7 +449,7 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf,
 // Bound, for long caches, by reading them: 61 rows of up to 8191 keys, 8 heads of 4 x 128, e4m3
 // (390 MB) 99 to 105 us, 3.7 to 3.9 TB/s.  A wavefront has some 8 tiles of 64 keys to read, so that the first loads'
 // way, the tile's chain (product, softmax, product) and the join are a quarter of it.  (8-bit heads
-// of 128 need all registers and keep 10, e4m3, or 4, int8, of a lane's in memory.)  For short
+// of 128 need all registers and keep 14, e4m3, or 6, int8, of a lane's in memory.)  For short
 // ones by that chain once: 6 heads of 64, 28 keys 6.4 us (int8), 114 keys 7.8 us (f32).
 template <class E, int DH>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
@@ -521,7 +526,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
   float low;
   const float c = tree_q<M>(a.q + row_of(mine) * a.ldq + (int64_t)head_of(mine) * DH, r < nq, h, qf, low);
 
-  for (float scale = 1.0f;; scale *= PA_LOW) {
+  for (int i = 0;; ++i) {
+    const TreeTurn turn = tree_turn<M::SCALED>(i);
     TreeSum<M::SCALED, M::WIDE, ND> acc;
     acc.clear();
 
@@ -578,7 +584,10 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
         for (int j = 0; j < PER; ++j)
           if (!(sees >> j & 1)) y[j] = NEG_INF;
       }
-      acc.template weigh<PER>(y, c, vsc, sees, h, scale);
+      if constexpr (M::SCALED)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) vsc[u] *= turn.up;
+      acc.template weigh<PER>(y, c, vsc, sees, h, turn.scale);
       tile.add(y, acc.o);
       if (odd_any)
 #pragma unroll
@@ -587,10 +596,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
     }
 
     // the wavefront's means
-    const bool first = scale == 1.0f;
     bool over = false;
-    const float inv = acc.mean();
-    if (first && h == 0) sm[wv][r] = acc.m, sl[wv][r] = acc.sum;
+    const float inv = acc.mean(turn.up);
+    if (turn.first && h == 0) sm[wv][r] = acc.m, sl[wv][r] = acc.sum;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int qr = 4 * h + i;
@@ -599,12 +607,12 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
       for (int d = 0; d < ND; ++d) {
         const float y = acc.o[d][i] * f;
         float &mean = so[wv][qr][16 * d + r];
-        if (!M::WIDE || first) mean = y;
+        if (!M::WIDE || turn.first) mean = y;
         else if (!__builtin_isfinite(mean)) mean = __builtin_isinf(y) && __builtin_isfinite(acc.o[d][i]) ? pa_largest(y) : y;
         over |= qr < nq && !__builtin_isfinite(y);
       }
     }
-    if (!M::WIDE || scale == tree_last<M::SCALED>() || !__builtin_amdgcn_ballot_w64(over)) break;
+    if (!M::WIDE || turn.scale != 1.0f || !__builtin_amdgcn_ballot_w64(over)) break;
     t = t0;
     begin();
   }
@@ -794,6 +802,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
       kscale = a.ks[row], vscale = a.vs[row];
     }
   };
+  TreeTurn turn;
   // ... goes to LDS
   auto store = [&](int t, bool edge) __attribute__((always_inline)) {
     typename S::Lds &l = lds[t & 1];
@@ -817,7 +826,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
         }
       }
     };
-    if (S::SCALED && tid < KEYS) l.ks[tid] = kscale, l.vs[tid] = vscale;
+    if (S::SCALED && tid < KEYS) l.ks[tid] = kscale, l.vs[tid] = vscale * turn.up;
     if (!edge && !__builtin_amdgcn_ballot_w64(vbad != 0)) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
@@ -861,7 +870,8 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
     if (special) atomicOr(&flags[t % 3], special);
   };
 
-  for (float scale = 1.0f;; scale *= PA_LOW) {
+  for (int i = 0;; ++i) {
+    turn = tree_turn<S::SCALED>(i);
     TreeSum<S::SCALED, S::WIDE, ND> acc[QW];
 #pragma unroll
     for (int x = 0; x < QW; ++x) acc[x].clear();
@@ -932,7 +942,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
               for (int j = 0; j < 8; ++j)
                 if (!(sees[x] >> j & 1)) y[j] = NEG_INF;
             }
-            acc[x].template weigh<8>(y, c[x], vsc, sees[x], h, scale);
+            acc[x].template weigh<8>(y, c[x], vsc, sees[x], h, turn.scale);
             pa_parts<BF16>(y, pf[x]);
           }
           // (two outputs in turn: a matrix instruction waits for the one before it on the same)
@@ -973,12 +983,12 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
     }
 
     // the means, to where they go (a second time: where the first ones are not finite)
-    const bool again = scale != 1.0f;
+    const bool again = !turn.first;
     bool over = false;
     const int64_t runs = (int64_t)a.rows * heads * gridDim.y;
 #pragma unroll
     for (int x = 0; x < QW; ++x) {
-      const float inv = acc[x].mean();
+      const float inv = acc[x].mean(turn.up);
       const int mine = w0 + 16 * x + r;
       if (!direct && !again && h == 0 && mine < nq) {
         const int64_t run = ((int64_t)row_of(mine) * heads + head_of(mine)) * gridDim.y + blockIdx.y;
@@ -1001,7 +1011,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_shared(TreeArgs a) {
         }
       }
     }
-    if (!S::WIDE || scale == tree_last<S::SCALED>() || !__syncthreads_or(over)) break;
+    if (!S::WIDE || turn.scale != 1.0f || !__syncthreads_or(over)) break;
   }
 }
 
