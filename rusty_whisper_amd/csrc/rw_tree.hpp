@@ -447,7 +447,7 @@ __device__ __forceinline__ float tree_q(const float *p, bool real, int h, T &qf,
 // chunk of keys).  A wavefront takes every PA_WAVES-th tile of keys, straight from memory, for
 // all of the workgroup's queries.
 // Bound, for long caches, by reading them: 61 rows of up to 8191 keys, 8 heads of 4 x 128, e4m3
-// (390 MB) 99 to 105 us, 3.7 to 3.9 TB/s.  A wavefront has some 8 tiles of 64 keys to read, so that the first loads'
+// (390 MB) 103 us, 3.8 TB/s.  A wavefront has some 8 tiles of 64 keys to read, so that the first loads'
 // way, the tile's chain (product, softmax, product) and the join are a quarter of it.  (8-bit heads
 // of 128 need all registers and keep 14, e4m3, or 6, int8, of a lane's in memory.)  For short
 // ones by that chain once: 6 heads of 64, 28 keys 6.4 us (int8), 114 keys 7.8 us (f32).
@@ -661,8 +661,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void k_tree_attn(TreeArgs a) {
 // calls, 333 TFLOP/s of the formula's and 1000 of the products done; the matrix units are busy 40 % of the
 // time, with two wavefronts to a SIMD of which each has some 250 other instructions to 48
 // products.  (Straight from memory: 2.2 times that.  With the next tile's scores formed before this one's
-// softmax: a tenth more.  With 128 queries: 557.)  The same chunks over int8: 471 us; 173 M vector instructions, where
-// bf16 has 108 M, for the conversions and scales, 280 us of issue beside 146 of products.
+// softmax: a tenth more.  With 128 queries: 557.)  The same chunks over int8: 468 us; 173 M vector instructions, where
+// bf16 has 109 M, for the conversions and scales, 280 us of issue beside 146 of products.
 // 24 trees of up to 48 rows, int8: 186 us, with half of the wavefronts' places empty, as the lengths are
 // unlike: products are 29 us of it, vector instructions 61.
 
