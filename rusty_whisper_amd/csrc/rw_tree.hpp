@@ -329,22 +329,24 @@ struct TreeTile<I8, DH> : TreeTile8<I8, DH> {};
 template <int DH>
 struct TreeTile<E4M3, DH> : TreeTile8<E4M3, DH> {};
 
-// A query's running softmax (lane 16 h + r: query r) and its tile's output (lane
-// 16 h + r: queries 4 h .., values 16 i + r).  Turns over the keys: the weights at
-// their own size; where means are not finite, at PA_LOW.  SCALED: before these, with the values' scales, and so
-// the outputs, 2^40 times as large (see above).  (One row's scale of 2^100 passes the range then, also where its
-// values are zeros and others' are not, which at PA_LOW would lose bits.  2^40 in the exponential's argument would
-// cost no product, but the argument's own bits: 4.1e-7 off in place of 2.3e-7.)
+// Turns over the keys: the weights at their own size; where means are not finite, at PA_LOW.  SCALED:
+// before these, with the values' scales, and so the outputs, 2^40 times as large (see above).  (One row's scale of
+// 2^100 passes the range then, also where its values are zeros and others' are not, which at PA_LOW would lose
+// bits.  2^40 in the exponential's argument would cost no product, but the argument's own bits: 4.1e-7 off in
+// place of 2.3e-7.)
+constexpr float TREE_UP = 0x1p40f;
 struct TreeTurn {
   float scale, up;  // of weights; of values' scales
   bool first;
 };
-constexpr float TREE_UP = 0x1p40f;
 template <bool SCALED>
 __device__ inline TreeTurn tree_turn(int i) {
   if (SCALED) return TreeTurn{i < 2 ? 1.0f : PA_LOW, i == 0 ? TREE_UP : 1.0f, i == 0};
   return TreeTurn{i == 0 ? 1.0f : PA_LOW, 1.0f, i == 0};
 }
+
+// A query's running softmax (lane 16 h + r: query r) and its tile's output (lane
+// 16 h + r: queries 4 h .., values 16 i + r).
 template <bool SCALED, bool WIDE, int ND>
 struct TreeSum {
   f4 o[ND];
